@@ -8,7 +8,11 @@ from .attention import (backward, check_device, decode, decode_combine, decode_c
                         decode_paged, decode_splitkv, default_scale, device_error_flags, forward,
                         forward_only, forward_varlen)
 from ._lib import lib_path
+from .quantcache import (QuantCache, append_paged_quant, decode_paged_quant, read_paged_quant,
+                         select_pages)
 
 __all__ = ["forward", "forward_only", "forward_varlen", "backward", "decode", "decode_splitkv", "decode_combine",
-           "decode_combine_ranks", "decode_merge_splits", "decode_paged", "device_error_flags", "check_device", "default_scale", "lib_path"]
+           "decode_combine_ranks", "decode_merge_splits", "decode_paged", "device_error_flags", "check_device", "default_scale", "lib_path",
+           "QuantCache", "append_paged_quant", "read_paged_quant", "decode_paged_quant",
+           "select_pages"]
 __version__ = "0.1.0"

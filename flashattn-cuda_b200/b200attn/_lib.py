@@ -55,6 +55,20 @@ _SIGNATURES = {
     # q k v o dO lse dq dk dv ws | B H Hkv N Nk D dtype causal | scale stream
     "b2a_backward": (_c_int, [_vp] * 10 + [_c_int] * 8 + [_c_float, _vp]),
     "b2a_backward_workspace_floats": (ctypes.c_int64, [_c_int] * 4),
+    "b2a_kvq_block_bytes": (ctypes.c_int64, [_c_int] * 3),
+    # k_new v_new k_strides v_strides data index index_scale bt lens
+    # | B Hkv T D page max_pages num_pages bits dtype advance | stream
+    "b2a_kvq_append_paged": (_c_int, [_vp] * 9 + [_c_int] * 10 + [_vp]),
+    # data bt start cu k_out v_out | B Hkv D page max_pages num_pages total max_len bits dtype | stream
+    "b2a_kvq_read_paged": (_c_int, [_vp] * 6 + [_c_int] * 10 + [_vp]),
+    # q q_strides index index_scale bt lens keys pages
+    # | B H Hkv D page max_pages num_pages top_k dtype | stream
+    "b2a_kvq_select_pages": (_c_int, [_vp] * 8 + [_c_int] * 9 + [_vp]),
+    "b2a_kvq_decode_splits": (_c_int, [_c_int, _c_int, ctypes.c_int64]),
+    # q q_strides data bt lens pages | n_pages | o_part l_part o lse
+    # | B H Hkv D page max_pages num_pages splits bits dtype | scale stream
+    "b2a_kvq_decode_paged": (_c_int, [_vp] * 6 + [_c_int] + [_vp] * 4 + [_c_int] * 10
+                             + [_c_float, _vp]),
     "b2a_device_error": (_c_int, [ctypes.POINTER(ctypes.c_uint32)]),
     "b2a_selftest_wait_timeout": (_c_int, [_c_int, _vp]),
 }

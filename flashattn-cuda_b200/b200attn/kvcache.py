@@ -30,14 +30,20 @@ class PagePool:
         if dtype not in _DT:
             raise ValueError("dtype must be torch.float16 or torch.bfloat16")
         self.page_size, self.max_pages = page_size, max_pages
-        self.k_pool = torch.zeros(num_pages, num_kv_heads, page_size, head_dim, dtype=dtype,
-                                  device=device)
-        self.v_pool = torch.zeros_like(self.k_pool)
+        self._make_storage(num_pages, page_size, num_kv_heads, head_dim, dtype, device)
         self.block_table = torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=device)
         self.kv_lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(max_seqs)]
         self._lens: List[int] = [0] * max_seqs
+
+    def _make_storage(self, num_pages, page_size, num_kv_heads, head_dim, dtype, device):
+        self.k_pool = torch.zeros(num_pages, num_kv_heads, page_size, head_dim, dtype=dtype,
+                                  device=device)
+        self.v_pool = torch.zeros_like(self.k_pool)
+
+    def _write(self, k_new, v_new, block_table, kv_lens):
+        append_paged(k_new, v_new, self.k_pool, self.v_pool, block_table, kv_lens, advance=True)
 
     @property
     def num_free(self) -> int:
@@ -83,11 +89,11 @@ class PagePool:
             self.reserve(s, T)
         if seqs == list(range(B)):
             bt, lens = self.block_table[:B], self.kv_lens[:B]
-            append_paged(k_new, v_new, self.k_pool, self.v_pool, bt, lens, advance=True)
+            self._write(k_new, v_new, bt, lens)
         else:
             idx = torch.tensor(seqs, dtype=torch.long, device=self.kv_lens.device)
             bt, lens = self.block_table[idx].contiguous(), self.kv_lens[idx].contiguous()
-            append_paged(k_new, v_new, self.k_pool, self.v_pool, bt, lens, advance=True)
+            self._write(k_new, v_new, bt, lens)
             self.kv_lens[idx] = lens
         for s in seqs:
             self._lens[s] += T

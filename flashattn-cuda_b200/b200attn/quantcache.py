@@ -1,0 +1,350 @@
+"""Paged KV cache held in 4 or 8 bits: write, read back, attend, select pages.
+
+`QuantCache` is the storage (one tensor of packed blocks, and an optional
+index of page bounds); `append_paged_quant`, `read_paged_quant`,
+`decode_paged_quant` and `select_pages` are the operators over it, with the
+block table and lengths that `append_paged` / `decode_paged` take.
+`QuantPagePool` adds the host-side page allocator of `PagePool`.
+
+A serving step over a quantised cache:
+
+    append_paged_quant(k_new, v_new, cache, block_table, kv_lens)
+    O, L = decode_paged_quant(q, cache, block_table, kv_lens)
+
+and for long contexts, reading only the pages that matter to the query (the
+cache needs an index):
+
+    pages = select_pages(q, cache, block_table, kv_lens, top_k=128)
+    O, L = decode_paged_quant(q, cache, block_table, kv_lens, pages=pages)
+
+The formats and the arithmetic are specified in include/b200attn.h.  The
+reference has no KV cache; the decode math is its online softmax
+(cuda/flash_attn_fa3_db_full.cu:250-300).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional
+
+import torch
+
+from . import _lib
+from .attention import _DT, _decode_q, _on_device, _ptr, _stream
+from .kvcache import PagePool
+
+GROUP = 64  # channels that share one (scale, min)
+
+
+def block_bytes(head_dim: int, page_size: int, bits: int) -> int:
+    """Bytes of one (page, KV head) block."""
+    n = _lib.load().b2a_kvq_block_bytes(head_dim, page_size, bits)
+    if n == 0:
+        raise RuntimeError("head_dim must be 64 or 128, page_size 16, 32 or 64 and bits 4 or 8")
+    return n
+
+
+class QuantCache:
+    """Storage of a quantised paged KV cache.
+
+    data: uint8 [P, Hkv, block_bytes]; index: int8 [P, Hkv, 2, D] with
+    index_scale fp32 [P, Hkv], or both None for a cache without an index.
+    dtype is that of the keys and values written and read (float16 or bfloat16).
+    """
+
+    __slots__ = ("data", "index", "index_scale", "page_size", "head_dim", "bits", "dtype")
+
+    def __init__(self, data: torch.Tensor, *, page_size: int, head_dim: int, bits: int,
+                 dtype: torch.dtype, index: Optional[torch.Tensor] = None,
+                 index_scale: Optional[torch.Tensor] = None):
+        if dtype not in _DT:
+            raise RuntimeError("dtype must be torch.float16 or torch.bfloat16")
+        if (data.dim() != 3 or data.dtype != torch.uint8 or not data.is_contiguous()
+                or data.shape[2] != block_bytes(head_dim, page_size, bits)):
+            raise RuntimeError("data must be contiguous uint8 [P, Hkv, block_bytes]")
+        if (index is None) != (index_scale is None):
+            raise RuntimeError("index and index_scale must be given together")
+        if index is not None:
+            P, Hkv, _ = data.shape
+            if (index.shape != (P, Hkv, 2, head_dim) or index.dtype != torch.int8
+                    or index_scale.shape != (P, Hkv) or index_scale.dtype != torch.float32
+                    or not (index.is_contiguous() and index_scale.is_contiguous())
+                    or index.device != data.device or index_scale.device != data.device):
+                raise RuntimeError("index must be contiguous int8 [P, Hkv, 2, D] and index_scale "
+                                   "fp32 [P, Hkv] on data's device")
+        self.data, self.index, self.index_scale = data, index, index_scale
+        self.page_size, self.head_dim, self.bits, self.dtype = page_size, head_dim, bits, dtype
+
+    @classmethod
+    def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+              bits: int = 4, dtype: torch.dtype = torch.float16, index: bool = False,
+              device="cuda") -> "QuantCache":
+        """A cache of `num_pages` pages that all read back as zero."""
+        data = torch.zeros(num_pages, num_kv_heads, block_bytes(head_dim, page_size, bits),
+                           dtype=torch.uint8, device=device)
+        idx = sc = None
+        if index:
+            idx = torch.zeros(num_pages, num_kv_heads, 2, head_dim, dtype=torch.int8,
+                              device=device)
+            sc = torch.zeros(num_pages, num_kv_heads, dtype=torch.float32, device=device)
+        return cls(data, page_size=page_size, head_dim=head_dim, bits=bits, dtype=dtype,
+                   index=idx, index_scale=sc)
+
+    @property
+    def num_pages(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def num_kv_heads(self) -> int:
+        return self.data.shape[1]
+
+    def codes(self, side: int) -> torch.Tensor:
+        """View of the K (0) or V (1) codes: uint8 [P, Hkv, page_size, D*bits/8]."""
+        row = self.head_dim * self.bits // 8
+        n = self.page_size * row
+        return self.data[..., side * n:(side + 1) * n].unflatten(-1, (self.page_size, row))
+
+    def params(self, side: int) -> torch.Tensor:
+        """View of the K (0) or V (1) params: dtype [P, Hkv, page_size, D/64, 2] (scale, min)."""
+        groups = self.head_dim // GROUP
+        n = self.page_size * groups * 4
+        at = 2 * self.page_size * (self.head_dim * self.bits // 8) + side * n
+        return self.data[..., at:at + n].view(self.dtype).unflatten(-1, (self.page_size, groups, 2))
+
+
+def _check_table(cache: QuantCache, block_table: torch.Tensor, rows: torch.Tensor, what: str,
+                 n: int) -> None:
+    """block_table int32 [B, max_pages] and `rows` int32 [n], contiguous, on the cache's device."""
+    dev = cache.data.device
+    if not cache.data.is_cuda:
+        raise RuntimeError("the cache must be on a CUDA device")
+    if (block_table.dim() != 2 or block_table.dtype != torch.int32
+            or not block_table.is_contiguous() or block_table.device != dev):
+        raise RuntimeError("block_table must be contiguous int32 [B, max_pages] on the cache's device")
+    if (rows.shape != (n,) or rows.dtype != torch.int32 or not rows.is_contiguous()
+            or rows.device != dev):
+        raise RuntimeError(f"{what} must be contiguous int32 [{n}] on the cache's device")
+
+
+def _row_strides(t: torch.Tensor, n: int):
+    """(t, element strides of its first n dims) with t copied where its rows are not contiguous
+    or not 16-byte aligned; a dim of size 1 has stride 0."""
+    shape, st = t.shape, t.stride()
+    if st[-1] != 1 or t.data_ptr() & 15 or any(s & 7 for i, s in enumerate(st[:n]) if shape[i] > 1):
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = t.stride()
+    return t, (ctypes.c_int64 * n)(*(st[i] if shape[i] > 1 else 0 for i in range(n)))
+
+
+def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCache,
+                       block_table: torch.Tensor, kv_lens: torch.Tensor,
+                       advance: bool = True) -> None:
+    """Quantise k_new, v_new [B, Hkv, T, D] (cache.dtype, any strides) and write them at
+    positions kv_lens[b] + t of the sequences in block_table (b2a_kvq_append_paged); with
+    `advance`, kv_lens += T on the device.  Updates the index of a cache that has one.
+    No page may be owned by two of the sequences that write to it."""
+    if k_new.dim() != 4 or k_new.shape != v_new.shape:
+        raise RuntimeError("k_new and v_new must both be [B, Hkv, T, D]")
+    B, Hkv, T, D = k_new.shape
+    if Hkv != cache.num_kv_heads or D != cache.head_dim:
+        raise RuntimeError("k_new must match the cache's KV heads and head dim")
+    if k_new.dtype != cache.dtype or v_new.dtype != cache.dtype:
+        raise RuntimeError("k_new and v_new must have the cache's dtype")
+    _check_table(cache, block_table, kv_lens, "kv_lens", B)
+    dev = cache.data.device
+    if k_new.device != dev or v_new.device != dev:
+        raise RuntimeError("k_new and v_new must be on the cache's device")
+    if block_table.shape[0] != B:
+        raise RuntimeError("block_table must have one row per sequence")
+    if B == 0 or T == 0:
+        return
+    lib = _lib.load()
+    with _on_device(dev):
+        kn, ks = _row_strides(k_new, 3)
+        vn, vs = _row_strides(v_new, 3)
+        _lib.check(lib.b2a_kvq_append_paged(
+            kn.data_ptr(), vn.data_ptr(), ks, vs, cache.data.data_ptr(), _ptr(cache.index),
+            _ptr(cache.index_scale), block_table.data_ptr(), kv_lens.data_ptr(), B, Hkv, T, D,
+            cache.page_size, block_table.shape[1], cache.num_pages, cache.bits,
+            _DT[cache.dtype], int(bool(advance)), _stream(dev)))
+
+
+def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                     total: int, max_len: int, start: Optional[torch.Tensor] = None,
+                     out=None) -> list:
+    """Read tokens back: [K, V], each [total, Hkv, D] in cache.dtype, packed token-major as
+    forward_varlen takes them.  Sequence b's tokens start[b] .. (None: from 0), as many as
+    cu_seqlens[b+1] - cu_seqlens[b] (int32 [B+1], device), go to rows cu_seqlens[b] .. ;
+    total = cu_seqlens[B] and max_len, a bound of every length, are host numbers.
+    `out` = (K, V) to write into; rows that no sequence owns are left as they were."""
+    B = block_table.shape[0]
+    _check_table(cache, block_table, cu_seqlens, "cu_seqlens", B + 1)
+    if start is not None:
+        _check_table(cache, block_table, start, "start", B)
+    dev = cache.data.device
+    shape = (int(total), cache.num_kv_heads, cache.head_dim)
+    if shape[0] < 0 or max_len < 0:
+        raise RuntimeError("total and max_len must be >= 0")
+    if out is not None:
+        K, V = out
+        for t in (K, V):
+            if (t.shape != shape or t.dtype != cache.dtype or not t.is_contiguous()
+                    or t.device != dev):
+                raise RuntimeError("out must be two contiguous [total, Hkv, D] tensors of the "
+                                   "cache's dtype on its device")
+    with _on_device(dev):
+        if out is None:
+            K = torch.empty(shape, dtype=cache.dtype, device=dev)
+            V = torch.empty(shape, dtype=cache.dtype, device=dev)
+        if B > 0 and total > 0 and max_len > 0:
+            _lib.check(_lib.load().b2a_kvq_read_paged(
+                cache.data.data_ptr(), block_table.data_ptr(), _ptr(start),
+                cu_seqlens.data_ptr(), K.data_ptr(), V.data_ptr(), B, shape[1], shape[2],
+                cache.page_size, block_table.shape[1], cache.num_pages, shape[0], int(max_len),
+                cache.bits, _DT[cache.dtype], _stream(dev)))
+    return [K, V]
+
+
+def _check_query(q: torch.Tensor, cache: QuantCache):
+    q3, had_len = _decode_q(q)
+    if not q3.is_cuda or q3.device != cache.data.device:
+        raise RuntimeError("q must be a CUDA tensor on the cache's device")
+    if q3.dtype != cache.dtype:
+        raise RuntimeError("q must have the cache's dtype")
+    H, Hkv = q3.shape[1], cache.num_kv_heads
+    if q3.shape[2] != cache.head_dim or H == 0 or H % Hkv != 0:
+        raise RuntimeError("q must be [B, H, D] with the cache's head dim and H a multiple of Hkv")
+    return q3, had_len
+
+
+def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
+                 kv_lens: torch.Tensor, top_k: int) -> torch.Tensor:
+    """The top_k pages of every (sequence, KV head) for the queries q [B, H, D] (or
+    [B, H, 1, D]): int32 [B, Hkv, top_k], logical page numbers, ascending, -1 behind the
+    last.  A page's score is an upper bound, from the cache's index, of its keys' products
+    with the group's query heads, in 8 bits (b2a_kvq_select_pages)."""
+    q3, _ = _check_query(q, cache)
+    if cache.index is None:
+        raise RuntimeError("select_pages needs a cache with an index")
+    if top_k <= 0:
+        raise RuntimeError("top_k must be > 0")
+    B, H, D = q3.shape
+    _check_table(cache, block_table, kv_lens, "kv_lens", B)
+    if block_table.shape[0] != B:
+        raise RuntimeError("block_table must have one row per sequence")
+    dev = cache.data.device
+    Hkv, max_pages = cache.num_kv_heads, block_table.shape[1]
+    with _on_device(dev):
+        pages = torch.empty((B, Hkv, int(top_k)), dtype=torch.int32, device=dev)
+        if B == 0:
+            return pages
+        keys = torch.empty(B * Hkv * max_pages, dtype=torch.int32, device=dev)
+        qc, qs = _row_strides(q3, 2)
+        _lib.check(_lib.load().b2a_kvq_select_pages(
+            qc.data_ptr(), qs, cache.index.data_ptr(), cache.index_scale.data_ptr(),
+            block_table.data_ptr(), kv_lens.data_ptr(), keys.data_ptr(), pages.data_ptr(), B, H,
+            Hkv, D, cache.page_size, max_pages, cache.num_pages, int(top_k), _DT[cache.dtype],
+            _stream(dev)))
+    return pages
+
+
+def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
+                       kv_lens: torch.Tensor, scale: Optional[float] = None,
+                       pages: Optional[torch.Tensor] = None,
+                       splits: Optional[int] = None) -> list:
+    """Decode attention over a quantised cache: [O, L] shaped like q ([B, H, D] or
+    [B, H, 1, D]); kv_lens may hold zeros (O = 0, L = -inf).  `pages` int32 [B, Hkv, n]
+    (from select_pages) restricts each KV head to those pages; negative entries are skipped.
+    `splits` overrides the number of pieces a sequence is cut into."""
+    q3, had_len = _check_query(q, cache)
+    B, H, D = q3.shape
+    _check_table(cache, block_table, kv_lens, "kv_lens", B)
+    if block_table.shape[0] != B:
+        raise RuntimeError("block_table must have one row per sequence")
+    dev, Hkv = cache.data.device, cache.num_kv_heads
+    n_pages = 0
+    if pages is not None:
+        if (pages.dim() != 3 or pages.shape[:2] != (B, Hkv) or pages.shape[2] == 0
+                or pages.dtype != torch.int32 or not pages.is_contiguous()
+                or pages.device != dev):
+            raise RuntimeError("pages must be contiguous int32 [B, Hkv, n] on the cache's device")
+        n_pages = pages.shape[2]
+    lib = _lib.load()
+    with _on_device(dev):
+        O = torch.empty((B, H, D), dtype=cache.dtype, device=dev)
+        L = torch.empty((B, H), dtype=torch.float32, device=dev)
+        if B > 0:
+            most = min(n_pages, block_table.shape[1]) if n_pages else block_table.shape[1]
+            S = (lib.b2a_kvq_decode_splits(B, Hkv, most * cache.page_size) if splits is None
+                 else int(splits))
+            part = (torch.empty(B * H * S * (D + 1), dtype=torch.float32, device=dev)
+                    if S > 1 else None)
+            po = _ptr(part)
+            qc, qs = _row_strides(q3, 2)
+            _lib.check(lib.b2a_kvq_decode_paged(
+                qc.data_ptr(), qs, cache.data.data_ptr(), block_table.data_ptr(),
+                kv_lens.data_ptr(), _ptr(pages), n_pages, po,
+                None if po is None else po + 4 * B * H * S * D, O.data_ptr(), L.data_ptr(), B, H,
+                Hkv, D, cache.page_size, block_table.shape[1], cache.num_pages, S, cache.bits,
+                _DT[cache.dtype], float(D) ** -0.5 if scale is None else float(scale),
+                _stream(dev)))
+    if had_len:
+        return [O.unsqueeze(2), L.unsqueeze(2)]
+    return [O, L]
+
+
+class QuantPagePool(PagePool):
+    """PagePool over a QuantCache: the same allocator (reserve / release / lengths), with
+    `append` quantising, and `read`, `decode` over the sequences it holds.
+
+    index=True keeps the page bounds that decode(top_k=...) selects by.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 max_seqs: int, max_pages: int, dtype=torch.float16, device="cuda",
+                 bits: int = 4, index: bool = False):
+        self._bits, self._index = bits, index
+        super().__init__(num_pages, page_size, num_kv_heads, head_dim, max_seqs, max_pages,
+                         dtype, device)
+
+    def _make_storage(self, num_pages, page_size, num_kv_heads, head_dim, dtype, device):
+        self.cache = QuantCache.empty(num_pages, page_size, num_kv_heads, head_dim, self._bits,
+                                      dtype, self._index, device)
+
+    def _write(self, k_new, v_new, block_table, kv_lens):
+        append_paged_quant(k_new, v_new, self.cache, block_table, kv_lens, advance=True)
+
+    def _rows(self, seqs: Optional[List[int]], n: int):
+        """(block table rows, lengths) of `seqs` (default 0..n-1)."""
+        seqs = list(range(n)) if seqs is None else list(seqs)
+        if seqs == list(range(len(seqs))):
+            return seqs, self.block_table[:len(seqs)], self.kv_lens[:len(seqs)]
+        idx = torch.tensor(seqs, dtype=torch.long, device=self.kv_lens.device)
+        return seqs, self.block_table[idx], self.kv_lens[idx]
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, seqs: Optional[List[int]] = None):
+        """Quantise and append k_new, v_new [B, Hkv, T, D] to `seqs` (default 0..B-1), each
+        sequence at most once."""
+        if seqs is not None and len(set(seqs)) != len(list(seqs)):
+            raise RuntimeError("a sequence may appear only once in one append")
+        super().append(k_new, v_new, seqs)
+
+    def read(self, seqs: Optional[List[int]] = None) -> list:
+        """[K, V, cu_seqlens, max_len] of the whole of `seqs` (default: all), as
+        forward_varlen takes them."""
+        seqs, bt, _ = self._rows(seqs, len(self._lens))
+        lens = [self._lens[s] for s in seqs]
+        cu = torch.tensor([0] + lens, dtype=torch.int64).cumsum(0).to(torch.int32)
+        cu = cu.to(self.kv_lens.device)
+        most = max(lens, default=0)
+        K, V = read_paged_quant(self.cache, bt, cu, sum(lens), most)
+        return [K, V, cu, most]
+
+    def decode(self, q: torch.Tensor, seqs: Optional[List[int]] = None,
+               scale: Optional[float] = None, top_k: Optional[int] = None) -> list:
+        """[O, L] of the queries q [B, H, D], one per sequence of `seqs` (default 0..B-1);
+        with top_k over that many pages of each KV head only."""
+        seqs, bt, lens = self._rows(seqs, q.shape[0])
+        most = max((len(self._pages[s]) for s in seqs), default=0)
+        bt = bt[:, :max(most, 1)].contiguous()  # the widest sequence's pages: fewer empty splits
+        pages = None if top_k is None else select_pages(q, self.cache, bt, lens, top_k)
+        return decode_paged_quant(q, self.cache, bt, lens, scale=scale, pages=pages)

@@ -45,6 +45,8 @@ int take_error_flags_backward(uint32_t* flags);
 int take_error_flags_decode(uint32_t* flags);
 int take_error_flags_selftest(uint32_t* flags);
 int take_error_flags_exchange(uint32_t* flags);
+int take_error_flags_kvquant(uint32_t* flags);
+int take_error_flags_kvquant_decode(uint32_t* flags);
 
 // Defines take_error_flags_<unit>() for the unit that expands it.
 #define B2A_DEFINE_ERROR_READER(unit)                                          \
@@ -83,6 +85,27 @@ int kv_append_dispatch(const void* k_new, const void* v_new, void* k_pool, void*
                        const int32_t* block_table, int32_t* kv_lens, int B, int Hkv, int T, int D,
                        int page_size, int max_pages, int num_pages, int advance,
                        cudaStream_t stream);
+// Quantised paged KV cache (strides in elements: batch, head, token).
+int kvq_append_dispatch(const void* k_new, const void* v_new, const int64_t* k_strides,
+                        const int64_t* v_strides, void* data, int8_t* index, float* index_scale,
+                        const int32_t* block_table, int32_t* kv_lens, int B, int Hkv, int T, int D,
+                        int page_size, int max_pages, int num_pages, int bits, int dtype,
+                        int advance, cudaStream_t stream);
+int kvq_read_dispatch(const void* data, const int32_t* block_table, const int32_t* start,
+                      const int32_t* cu, void* k_out, void* v_out, int B, int Hkv, int D,
+                      int page_size, int max_pages, int num_pages, int total, int max_len,
+                      int bits, int dtype, cudaStream_t stream);
+int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* index,
+                        const float* index_scale, const int32_t* block_table,
+                        const int32_t* kv_lens, uint32_t* keys, int32_t* pages, int B, int H,
+                        int Hkv, int D, int page_size, int max_pages, int num_pages, int top_k,
+                        int dtype, cudaStream_t stream);
+int kvq_decode_splits(int B, int Hkv, long long max_tokens);
+int kvq_decode_dispatch(const void* q, int64_t q_b, int64_t q_h, const void* data,
+                        const int32_t* block_table, const int32_t* kv_lens, const int32_t* pages,
+                        int n_list, float* o_part, float* l_part, void* o, float* lse, int B,
+                        int H, int Hkv, int D, int page_size, int max_pages, int num_pages,
+                        int splits, int bits, int dtype, float scale, cudaStream_t stream);
 // combine_dispatch's dtype for an fp32 merged partial (o, lse) instead of O.
 constexpr int kCombineF32 = 100;
 // ranks > 1: partials of `ranks` ranks, rank r's o / l blocks `rank_stride`

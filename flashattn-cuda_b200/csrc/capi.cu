@@ -10,6 +10,7 @@
 #include <mutex>
 
 #include "b2a_host.h"
+#include "kvquant.cuh"
 
 namespace b2a {
 
@@ -446,6 +447,164 @@ int b2a_kv_append_paged(const void* k_new, const void* v_new, void* k_pool, void
                             static_cast<cudaStream_t>(stream));
 }
 
+// ------------------------------------------------- quantised paged KV cache
+
+// A device pointer that needs `align` bytes of alignment (4: arrays of words).
+static int check_ptr_align(const void* p, const char* what, unsigned align) {
+  B2A_TRY(check_device_ptr(p, what, false));
+  if (reinterpret_cast<uintptr_t>(p) % align != 0) {
+    char buf[128];
+    snprintf(buf, sizeof buf, "%s must be %u-byte aligned", what, align);
+    return set_error(B2A_ERR_MISALIGNED, buf);
+  }
+  return B2A_OK;
+}
+
+static int kvq_checks(int B, int Hkv, int D, int page_size, int max_pages, int num_pages, int bits,
+                      int dtype) {
+  B2A_TRY(common_checks(dtype));
+  if (D != 64 && D != 128) return set_error(B2A_ERR_UNSUPPORTED, "Head dimension must be 64 or 128");
+  if (bits != 4 && bits != 8) return set_error(B2A_ERR_UNSUPPORTED, "bits must be 4 or 8");
+  if (page_size != 16 && page_size != 32 && page_size != 64)
+    return set_error(B2A_ERR_UNSUPPORTED, "page_size must be 16, 32 or 64");
+  if (B <= 0 || Hkv <= 0 || max_pages <= 0 || num_pages <= 0)
+    return set_error(B2A_ERR_INVALID_ARG, "B, Hkv, max_pages and num_pages must be > 0");
+  if (B > 65535 || Hkv > 65535) return set_error(B2A_ERR_INVALID_ARG, "B and Hkv must be <= 65535");
+  if ((int64_t)max_pages * page_size > 0x7fff0000)
+    return set_error(B2A_ERR_INVALID_ARG, "max_pages * page_size too large");
+  return B2A_OK;
+}
+
+static int kvq_heads(int H, int Hkv) {
+  if (H <= 0 || H % Hkv != 0) return set_error(B2A_ERR_INVALID_ARG, "H must be a multiple of Hkv");
+  if (H / Hkv > 8)
+    return set_error(B2A_ERR_UNSUPPORTED, "GQA group H/Hkv must be at most 8");
+  return B2A_OK;
+}
+
+// Rows of 8 values are read as 16 bytes: every stride is a multiple of 8.
+static int kvq_strides(const int64_t* s, int n, const char* what) {
+  if (s == nullptr) return set_error(B2A_ERR_INVALID_ARG, "strides must not be null");
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0 || s[i] % 8 != 0) {
+      char buf[128];
+      snprintf(buf, sizeof buf, "%s strides must be multiples of 8 elements", what);
+      return set_error(B2A_ERR_MISALIGNED, buf);
+    }
+  return B2A_OK;
+}
+
+int64_t b2a_kvq_block_bytes(int D, int page_size, int bits) {
+  if ((D != 64 && D != 128) || (bits != 4 && bits != 8) ||
+      (page_size != 16 && page_size != 32 && page_size != 64))
+    return 0;
+  return kvq::block_bytes(D, page_size, bits);
+}
+
+int b2a_kvq_append_paged(const void* k_new, const void* v_new, const int64_t* k_strides,
+                         const int64_t* v_strides, void* data, int8_t* index, float* index_scale,
+                         const int32_t* block_table, int32_t* kv_lens, int B, int Hkv, int T,
+                         int D, int page_size, int max_pages, int num_pages, int bits, int dtype,
+                         int advance_lens, void* stream) {
+  t_last_error[0] = 0;
+  B2A_TRY(kvq_checks(B, Hkv, D, page_size, max_pages, num_pages, bits, dtype));
+  if (T <= 0) return set_error(B2A_ERR_INVALID_ARG, "T must be > 0");
+  if ((index == nullptr) != (index_scale == nullptr))
+    return set_error(B2A_ERR_INVALID_ARG, "index and index_scale must be given together");
+  B2A_TRY(kvq_strides(k_strides, 3, "k_new"));
+  B2A_TRY(kvq_strides(v_strides, 3, "v_new"));
+  B2A_TRY(check_device_ptr(k_new, "k_new"));
+  B2A_TRY(check_device_ptr(v_new, "v_new"));
+  B2A_TRY(check_device_ptr(data, "data"));
+  if (index != nullptr) {
+    B2A_TRY(check_device_ptr(index, "index"));
+    B2A_TRY(check_ptr_align(index_scale, "index_scale", 4));
+  }
+  B2A_TRY(check_ptr_align(block_table, "block_table", 4));
+  B2A_TRY(check_ptr_align(kv_lens, "kv_lens", 4));
+  return kvq_append_dispatch(k_new, v_new, k_strides, v_strides, data, index, index_scale,
+                             block_table, kv_lens, B, Hkv, T, D, page_size, max_pages, num_pages,
+                             bits, dtype, advance_lens, static_cast<cudaStream_t>(stream));
+}
+
+int b2a_kvq_read_paged(const void* data, const int32_t* block_table, const int32_t* start,
+                       const int32_t* cu_seqlens, void* k_out, void* v_out, int B, int Hkv, int D,
+                       int page_size, int max_pages, int num_pages, int total, int max_len,
+                       int bits, int dtype, void* stream) {
+  t_last_error[0] = 0;
+  B2A_TRY(kvq_checks(B, Hkv, D, page_size, max_pages, num_pages, bits, dtype));
+  if (total <= 0 || max_len <= 0)
+    return set_error(B2A_ERR_INVALID_ARG, "total and max_len must be > 0");
+  B2A_TRY(check_device_ptr(data, "data"));
+  B2A_TRY(check_ptr_align(block_table, "block_table", 4));
+  if (start != nullptr) B2A_TRY(check_ptr_align(start, "start", 4));
+  B2A_TRY(check_ptr_align(cu_seqlens, "cu_seqlens", 4));
+  B2A_TRY(check_device_ptr(k_out, "k_out"));
+  B2A_TRY(check_device_ptr(v_out, "v_out"));
+  return kvq_read_dispatch(data, block_table, start, cu_seqlens, k_out, v_out, B, Hkv, D,
+                           page_size, max_pages, num_pages, total, max_len, bits, dtype,
+                           static_cast<cudaStream_t>(stream));
+}
+
+int b2a_kvq_select_pages(const void* q, const int64_t* q_strides, const int8_t* index,
+                         const float* index_scale, const int32_t* block_table,
+                         const int32_t* kv_lens, uint32_t* keys, int32_t* pages, int B, int H,
+                         int Hkv, int D, int page_size, int max_pages, int num_pages, int top_k,
+                         int dtype, void* stream) {
+  t_last_error[0] = 0;
+  B2A_TRY(kvq_checks(B, Hkv, D, page_size, max_pages, num_pages, 8, dtype));
+  B2A_TRY(kvq_heads(H, Hkv));
+  if (top_k <= 0) return set_error(B2A_ERR_INVALID_ARG, "top_k must be > 0");
+  B2A_TRY(kvq_strides(q_strides, 2, "q"));
+  B2A_TRY(check_device_ptr(q, "q"));
+  B2A_TRY(check_device_ptr(index, "index"));
+  B2A_TRY(check_ptr_align(index_scale, "index_scale", 4));
+  B2A_TRY(check_ptr_align(block_table, "block_table", 4));
+  B2A_TRY(check_ptr_align(kv_lens, "kv_lens", 4));
+  B2A_TRY(check_ptr_align(keys, "keys", 4));
+  B2A_TRY(check_ptr_align(pages, "pages", 4));
+  return kvq_select_dispatch(q, q_strides[0], q_strides[1], index, index_scale, block_table,
+                             kv_lens, keys, pages, B, H, Hkv, D, page_size, max_pages, num_pages,
+                             top_k, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int b2a_kvq_decode_splits(int B, int Hkv, int64_t max_tokens) {
+  if (B <= 0 || Hkv <= 0 || max_tokens <= 0) return 1;
+  return kvq_decode_splits(B, Hkv, max_tokens);
+}
+
+int b2a_kvq_decode_paged(const void* q, const int64_t* q_strides, const void* data,
+                         const int32_t* block_table, const int32_t* kv_lens, const int32_t* pages,
+                         int n_pages, float* o_part, float* l_part, void* o, float* lse, int B,
+                         int H, int Hkv, int D, int page_size, int max_pages, int num_pages,
+                         int splits, int bits, int dtype, float scale, void* stream) {
+  t_last_error[0] = 0;
+  B2A_TRY(kvq_checks(B, Hkv, D, page_size, max_pages, num_pages, bits, dtype));
+  B2A_TRY(kvq_heads(H, Hkv));
+  if (splits <= 0 || splits > 65535)
+    return set_error(B2A_ERR_INVALID_ARG, "splits must be in 1 .. 65535");
+  if (pages != nullptr && (n_pages <= 0 || (int64_t)n_pages * page_size > 0x7fff0000))
+    return set_error(B2A_ERR_INVALID_ARG, "n_pages must be > 0 and n_pages * page_size < 2^31");
+  if ((int64_t)B * H > 0x7fffffff) return set_error(B2A_ERR_INVALID_ARG, "B*H too large");
+  if (!(scale > 0.f)) return set_error(B2A_ERR_INVALID_ARG, "scale must be > 0");
+  B2A_TRY(kvq_strides(q_strides, 2, "q"));
+  B2A_TRY(check_device_ptr(q, "q"));
+  B2A_TRY(check_device_ptr(data, "data"));
+  B2A_TRY(check_ptr_align(block_table, "block_table", 4));
+  B2A_TRY(check_ptr_align(kv_lens, "kv_lens", 4));
+  if (pages != nullptr) B2A_TRY(check_ptr_align(pages, "pages", 4));
+  if (splits > 1) {
+    B2A_TRY(check_device_ptr(o_part, "o_part"));
+    B2A_TRY(check_ptr_align(l_part, "l_part", 4));
+  }
+  B2A_TRY(check_device_ptr(o, "O"));
+  if (lse != nullptr) B2A_TRY(check_ptr_align(lse, "L", 4));
+  return kvq_decode_dispatch(q, q_strides[0], q_strides[1], data, block_table, kv_lens, pages,
+                             n_pages, o_part, l_part, o, lse, B, H, Hkv, D, page_size, max_pages,
+                             num_pages, splits, bits, dtype, scale,
+                             static_cast<cudaStream_t>(stream));
+}
+
 int b2a_device_error(uint32_t* flags) {
   t_last_error[0] = 0;
   if (flags == nullptr) return set_error(B2A_ERR_INVALID_ARG, "flags must not be null");
@@ -459,6 +618,8 @@ int b2a_device_error(uint32_t* flags) {
   B2A_TRY(take_error_flags_decode(&v));
   B2A_TRY(take_error_flags_selftest(&v));
   B2A_TRY(take_error_flags_exchange(&v));
+  B2A_TRY(take_error_flags_kvquant(&v));
+  B2A_TRY(take_error_flags_kvquant_decode(&v));
   *flags = v;
   if (v & 1u) {
     char buf[160];

@@ -1,0 +1,146 @@
+// kvquant.cuh -- the format of the quantised paged KV cache, shared by its
+// write / read-back kernels (kvquant_sm100.cu) and its attention
+// (kvquant_decode_sm100.cu).
+//
+// The block of one (page, KV head) is one contiguous piece of memory,
+//   [K codes | V codes | K params | V params],
+// so that a bulk copy fetches everything attention needs of a page at once.
+// Codes are token-major rows of D*bits/8 bytes, low nibble first at 4 bits.
+// Params hold one (scale, min) pair in the cache's dtype per token and group
+// of kGroup channels; a code c stands for scale*c + min.
+#pragma once
+#include "sm100_ptx.cuh"
+
+namespace b2a {
+namespace kvq {
+
+constexpr int kGroup = 64;  // channels sharing one (scale, min): 4.5 / 8.5 bits an element
+// Steps below this are stored as 0 (the group reads back as its min), so that
+// the reciprocal of a step is always a finite fp32.
+constexpr float kTinyStep = 7.8886090522101181e-31f;  // 2^-100
+
+__host__ __device__ constexpr int row_bytes(int D, int bits) { return D * bits / 8; }
+__host__ __device__ constexpr int block_bytes(int D, int page, int bits) {
+  return 2 * page * (row_bytes(D, bits) + D / kGroup * 4);
+}
+
+// 8 consecutive values of a row as four packed pairs.
+template <bool BF16>
+struct Vec8 {
+  typename Elem<BF16>::T2 v[4];
+};
+
+template <bool BF16>
+__device__ __forceinline__ typename Elem<BF16>::T2 min2_nan(typename Elem<BF16>::T2 a,
+                                                            typename Elem<BF16>::T2 b) {
+  return __hmin2_nan(a, b);
+}
+template <bool BF16>
+__device__ __forceinline__ typename Elem<BF16>::T2 max2_nan(typename Elem<BF16>::T2 a,
+                                                            typename Elem<BF16>::T2 b) {
+  return __hmax2_nan(a, b);
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// fp32 -> dtype with directed rounding (x >= 0), back in fp32
+template <bool BF16>
+__device__ __forceinline__ float round_up(float x) {
+  if constexpr (BF16) return __bfloat162float(__float2bfloat16_ru(x));
+  else return __half2float(__float2half_ru(x));
+}
+template <bool BF16>
+__device__ __forceinline__ float round_down(float x) {
+  if constexpr (BF16) return __bfloat162float(__float2bfloat16_rd(x));
+  else return __half2float(__float2half_rd(x));
+}
+template <bool BF16>
+__device__ __forceinline__ float round_near(float x) {
+  const float2 r = Elem<BF16>::unpack(Elem<BF16>::pack(x, 0.f));
+  return r.x;
+}
+
+// The step of a group with extremes lo, hi (both finite) and n = 2^bits - 1:
+// (hi - lo) / n rounded up to dtype, so that n steps from lo reach hi; rounded
+// down where lo + n*step would leave the dtype's range.  Halves keep hi - lo
+// finite for any finite bf16.  Explicit roundings: the result is specified to
+// the bit.
+template <bool BF16, int BITS>
+__device__ __forceinline__ float group_step(float lo, float hi) {
+  constexpr float n = (float)((1 << BITS) - 1);
+  const float want = __fmul_rn(__fsub_rn(0.5f * hi, 0.5f * lo), 2.0f / n);
+  float s = round_up<BF16>(want);
+  if (!finite(round_near<BF16>(__fmaf_rn(n, s, lo)))) s = round_down<BF16>(want);
+  return s < kTinyStep ? 0.f : s;
+}
+
+// Round to nearest even of 0 <= x <= 255 as an integer in the low mantissa bits.
+__device__ __forceinline__ uint32_t small_rint(float x) {
+  return __float_as_uint(__fadd_rn(x, 8388608.f)) & 0xffu;
+}
+
+// Codes of 8 values of a group (lo, step): one word at 4 bits, two at 8.
+template <bool BF16, int BITS>
+__device__ __forceinline__ uint2 encode8(const Vec8<BF16>& x, float lo, float step) {
+  constexpr float n = (float)((1 << BITS) - 1);
+  uint2 w = make_uint2(0u, 0u);
+  if (step > 0.f) {  // also false for a NaN step: codes 0
+    const float inv = __frcp_rn(0.5f * step), lo2 = 0.5f * lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Elem<BF16>::unpack(x.v[i]);
+      const uint32_t c0 = small_rint(fminf(__fmul_rn(__fsub_rn(0.5f * f.x, lo2), inv), n));
+      const uint32_t c1 = small_rint(fminf(__fmul_rn(__fsub_rn(0.5f * f.y, lo2), inv), n));
+      if constexpr (BITS == 4) {
+        w.x |= (c0 | (c1 << 4)) << (8 * i);
+      } else {
+        const uint32_t p = c0 | (c1 << 8);
+        if (i < 2) w.x |= p << (16 * i);
+        else w.y |= p << (16 * (i - 2));
+      }
+    }
+  }
+  return w;
+}
+
+// The values that 8 codes stand for: one fused multiply-add in fp32, rounded
+// once to dtype.
+template <bool BF16, int BITS>
+__device__ __forceinline__ Vec8<BF16> decode8(uint2 w, float step, float lo) {
+  Vec8<BF16> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t c0, c1;
+    if constexpr (BITS == 4) {
+      c0 = (w.x >> (8 * i)) & 15u;
+      c1 = (w.x >> (8 * i + 4)) & 15u;
+    } else {
+      const uint32_t p = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
+      c0 = p & 255u;
+      c1 = (p >> 8) & 255u;
+    }
+    r.v[i] = Elem<BF16>::pack(__fmaf_rn((float)c0, step, lo), __fmaf_rn((float)c1, step, lo));
+  }
+  return r;
+}
+
+// a (scale, min) pair of the cache's dtype in fp32
+template <bool BF16>
+__device__ __forceinline__ float2 param(uint32_t raw) {
+  typename Elem<BF16>::T2 h;
+  *reinterpret_cast<uint32_t*>(&h) = raw;
+  return Elem<BF16>::unpack(h);
+}
+
+// A signed 8-bit scale for values of magnitude up to `top`: NaN when top is
+// not finite; codes are 0 where it is below kTinyStep.
+__device__ __forceinline__ float scale127(float top) {
+  return finite(top) ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fc00000);
+}
+__device__ __forceinline__ int code127(float v, float scale, float inv) {
+  if (!(scale >= kTinyStep)) return 0;
+  return __float2int_rn(fminf(fmaxf(__fmul_rn(v, inv), -127.f), 127.f));
+}
+
+}  // namespace kvq
+}  // namespace b2a

@@ -256,8 +256,104 @@ int b2a_decode_paged_noalloc(const void* q, const void* k_pool,
                              int dtype, float scale, void* stream);
 
 /*
+ * Quantised paged KV cache.  The pool `data` is [P, Hkv, block] bytes with
+ * block = b2a_kvq_block_bytes(D, page_size, bits); the block of one (page, KV
+ * head) is [K codes | V codes | K params | V params]:
+ *   codes   [page_size, D*bits/8] bytes, token-major, low nibble first at 4
+ *           bits; bits in {4, 8}
+ *   params  [page_size, D/64, 2] values of dtype: (scale, min) of each token's
+ *           groups of 64 channels; code c stands for scale*c + min
+ * so 4.5 or 8.5 bits an element.  page_size in {16, 32, 64}, D in {64, 128}.
+ * The optional index holds channel bounds of each page's keys for
+ * b2a_kvq_select_pages: index [P, Hkv, 2, D] int8 (minima, maxima) and
+ * index_scale [P, Hkv] fp32.  No counterpart in the reference.
+ * b2a_kvq_block_bytes returns 0 for a format that is not built.
+ */
+int64_t b2a_kvq_block_bytes(int D, int page_size, int bits);
+
+/*
+ * Quantise and append T new tokens per sequence: the write path of the cache,
+ * with b2a_kv_append_paged's block table, lengths, advance_lens and error bit
+ * 2 (a sequence whose kv_lens is negative is dropped too).  k_new, v_new are
+ * [B,Hkv,T,D] with element strides k_strides / v_strides = {batch, head,
+ * token}, multiples of 8; rows are contiguous and 16-byte aligned.
+ *   With n = 2^bits - 1 and a group's extremes lo, hi: scale = (hi - lo)/n
+ * rounded up to dtype (down where lo + n*scale would leave its range; 0 below
+ * 2^-100), min = lo, code = rint((x - lo)/scale), each step in fp32: the codes
+ * are the same to the bit on every call.  A group that holds a NaN or an
+ * infinity reads back as NaN.
+ *   With index != NULL the bounds of every page that is written to are set
+ * from all its tokens (those already there are read back): symmetric int8
+ * codes of the read-back keys' minima and maxima with one scale.  A page must
+ * not appear twice among the pages written by one call.
+ */
+int b2a_kvq_append_paged(const void* k_new, const void* v_new,
+                         const int64_t* k_strides, const int64_t* v_strides,
+                         void* data, int8_t* index, float* index_scale,
+                         const int32_t* block_table, int32_t* kv_lens, int B,
+                         int Hkv, int T, int D, int page_size, int max_pages,
+                         int num_pages, int bits, int dtype, int advance_lens,
+                         void* stream);
+
+/*
+ * Read tokens back as packed token-major rows, the layout of
+ * b2a_prefill_fwd_varlen: tokens start[b] .. start[b] + n_b - 1 of sequence b
+ * (start == NULL: from 0), n_b = cu_seqlens[b+1] - cu_seqlens[b], go to rows
+ * cu_seqlens[b].. of k_out, v_out [total, Hkv, D] (dtype), each value one fp32
+ * multiply-add rounded once.  max_len bounds every n_b.  Rows that no sequence
+ * owns are left as they were.  A page that the block table lacks sets bit 1 of
+ * the device error word and its rows read as zero; a sequence with bad
+ * cu_seqlens or start, or longer than max_len, sets bit 3 and is not read.
+ */
+int b2a_kvq_read_paged(const void* data, const int32_t* block_table,
+                       const int32_t* start, const int32_t* cu_seqlens,
+                       void* k_out, void* v_out, int B, int Hkv, int D,
+                       int page_size, int max_pages, int num_pages, int total,
+                       int max_len, int bits, int dtype, void* stream);
+
+/*
+ * The top_k pages of every (sequence, KV head) by a cheap score: pages
+ * [B, Hkv, top_k] int32, logical page numbers in ascending order, -1 behind
+ * the last.  Query heads are rounded to int8 with one scale each; a page's
+ * score is the largest, over the group's heads, of
+ * (sum_d max(q8*min8, q8*max8) * q_scale) * index_scale, with the sum exact
+ * and each product rounded to fp32.  The last page of a sequence is always
+ * selected and ties go to the lowest page; a score that is NaN counts as
+ * +infinity.  q is [B,H,D] with element strides {batch, head}, multiples of 8;
+ * H/Hkv <= 8.  keys is scratch of B*Hkv*max_pages words.
+ */
+int b2a_kvq_select_pages(const void* q, const int64_t* q_strides,
+                         const int8_t* index, const float* index_scale,
+                         const int32_t* block_table, const int32_t* kv_lens,
+                         uint32_t* keys, int32_t* pages, int B, int H, int Hkv,
+                         int D, int page_size, int max_pages, int num_pages,
+                         int top_k, int dtype, void* stream);
+
+/*
+ * Decode attention (query length 1) over the quantised cache, split over the
+ * tokens: O [B,H,D] (dtype) and lse [B,H] (may be NULL) as b2a_decode_paged.
+ * kv_lens[b] may be 0 (O = 0, lse = -inf).  pages == NULL attends to the whole
+ * cache; else to the n_pages logical pages that pages [B, Hkv, n_pages] lists
+ * for each KV head (entries that are negative or lie behind the sequence's end
+ * are skipped; a page listed twice counts twice).  splits > 1 needs the fp32
+ * scratch o_part [B,H,splits,D] and l_part [B,H,splits];
+ * b2a_kvq_decode_splits gives the number that suits B, Hkv and the most tokens
+ * one sequence attends to.  A bad block-table entry sets bit 1 of the device
+ * error word and reads page 0 instead.  H/Hkv <= 8.
+ */
+int b2a_kvq_decode_splits(int B, int Hkv, int64_t max_tokens);
+int b2a_kvq_decode_paged(const void* q, const int64_t* q_strides,
+                         const void* data, const int32_t* block_table,
+                         const int32_t* kv_lens, const int32_t* pages,
+                         int n_pages, float* o_part, float* l_part, void* o,
+                         float* lse, int B, int H, int Hkv, int D,
+                         int page_size, int max_pages, int num_pages,
+                         int splits, int bits, int dtype, float scale,
+                         void* stream);
+
+/*
  * Device error word written by the kernels (bit 0: a bounded pipeline wait
- * timed out; bit 1: a paged-decode block-table entry was out of range;
+ * timed out; bit 1: a paged-decode or read-back block-table entry was out of range;
  * bit 2: a KV append found no page for a position; bit 3: a varlen sequence
  * was longer than max_seqlen_q or cu_seqlens was not non-decreasing; bit 4:
  * the backward kernel found too little shared memory to align its tiles and

@@ -1,0 +1,692 @@
+"""Quantised paged KV cache: format and refusals (CPU); write, read-back, page
+selection and attention on the GPU against the numpy oracle.
+
+What the format specifies to the bit is compared to the bit.  Attention is held
+to a bound made of its roundings: with u = eps/2 of the dtype, O is rounded
+once (u |O|), and the attention kernel may round each probability times its
+value's step once (u sum_i p_i step_i code_i, plus, in fp16, half the smallest
+subnormal of a product scaled to at most 1 for every token); scores and sums are fp32.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention as ora
+from oracle import quantcache as oq
+
+NAME = {torch.float16: "float16", torch.bfloat16: "bfloat16"}
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+# ------------------------------------------------------------------------ CPU
+def test_block_bytes():
+    from b200attn import quantcache as qc
+    assert qc.block_bytes(128, 16, 4) == 2 * 16 * (64 + 8)
+    assert qc.block_bytes(64, 64, 8) == 2 * 64 * (64 + 4)
+    for bad in ((96, 16, 4), (128, 24, 4), (128, 16, 5), (0, 0, 0)):
+        with pytest.raises(RuntimeError, match="head_dim"):
+            qc.block_bytes(*bad)
+
+
+def test_cache_views_cover_the_block():
+    from b200attn import QuantCache
+    c = QuantCache.empty(3, 16, 2, 128, bits=4, index=True, device="cpu")
+    for i, side in enumerate((0, 1)):
+        c.codes(side).fill_(1 + i)
+        c.params(side).view(torch.int16).fill_(0x0303 + i * 0x0101)
+    n = torch.bincount(c.data.flatten().long(), minlength=5).tolist()
+    per = 3 * 2 * 16
+    assert n[0] == 0 and n[1:5] == [per * 64, per * 64, per * 8, per * 8]
+    assert c.num_pages == 3 and c.num_kv_heads == 2
+
+
+def test_cache_refuses_wrong_storage():
+    from b200attn import QuantCache
+    ok = dict(page_size=16, head_dim=64, bits=4, dtype=F16)
+    data = torch.zeros(2, 1, 2 * 16 * 36, dtype=torch.uint8)
+    QuantCache(data, **ok)
+    with pytest.raises(RuntimeError, match="data"):
+        QuantCache(data[..., :-1].contiguous(), **ok)
+    with pytest.raises(RuntimeError, match="data"):
+        QuantCache(data.float(), **ok)
+    with pytest.raises(RuntimeError, match="dtype"):
+        QuantCache(data, **dict(ok, dtype=torch.float32))
+    idx, sc = torch.zeros(2, 1, 2, 64, dtype=torch.int8), torch.zeros(2, 1)
+    QuantCache(data, index=idx, index_scale=sc, **ok)
+    with pytest.raises(RuntimeError, match="together"):
+        QuantCache(data, index=idx, **ok)
+    with pytest.raises(RuntimeError, match="index"):
+        QuantCache(data, index=idx[:, :, :1], index_scale=sc, **ok)
+
+
+def test_pool_bookkeeping_and_duplicate_sequences():
+    from b200attn.quantcache import QuantPagePool
+    pool = QuantPagePool(10, 16, 2, 64, max_seqs=3, max_pages=8, device="cpu", bits=8, index=True)
+    pool.reserve(0, 17)
+    assert pool.num_free == 8 and pool.cache.index is not None
+    k = torch.zeros(2, 2, 1, 64, dtype=F16)
+    with pytest.raises(RuntimeError, match="once"):
+        pool.append(k, k, seqs=[1, 1])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        pool.append(k, k, seqs=[1, 2])
+
+
+def test_entry_points_refuse_on_the_host():
+    import b200attn as b
+    c = b.QuantCache.empty(4, 16, 2, 64, index=True, device="cpu")
+    bt, kl = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    k = torch.zeros(1, 2, 3, 64, dtype=F16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        b.append_paged_quant(k, k, c, bt, kl)
+    with pytest.raises(RuntimeError, match="dtype"):
+        b.append_paged_quant(k.float(), k.float(), c, bt, kl)
+    with pytest.raises(RuntimeError, match="KV heads"):
+        b.append_paged_quant(k[:, :1], k[:, :1], c, bt, kl)
+    with pytest.raises(RuntimeError, match="both"):
+        b.append_paged_quant(k, k[:, :, :2], c, bt, kl)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        b.read_paged_quant(c, bt, torch.zeros(2, dtype=torch.int32), 0, 0)
+    q = torch.zeros(1, 4, 64, dtype=F16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        b.decode_paged_quant(q, c, bt, kl)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        b.select_pages(q, c, bt, kl, 1)
+
+
+def test_library_refuses_bad_formats_without_a_device():
+    from b200attn import _lib
+    lib = _lib.load()
+    assert lib.b2a_kvq_block_bytes(128, 16, 3) == 0
+    assert lib.b2a_kvq_decode_splits(0, 8, 100) == 1
+    assert lib.b2a_kvq_decode_splits(1, 8, 16) == 1
+    for B, n in ((1, 131072), (64, 32768), (1, 1 << 31)):
+        assert 1 <= lib.b2a_kvq_decode_splits(B, 8, n) <= 65535
+
+
+def test_oracle_quantiser_keeps_within_half_a_step():
+    """Every finite value reads back within half a step, plus the rounding of the result."""
+    rng = np.random.default_rng(0)
+    for dtype in ("float16", "bfloat16"):
+        for bits in (4, 8):
+            x = oq.round_to(rng.standard_normal((50, 128)) * np.exp(rng.standard_normal((50, 1)) * 3), dtype)
+            c, s, lo = oq.quantise(x, bits, dtype)
+            half = np.repeat(s, 64, -1) * 0.5
+            assert (np.abs(oq.values(c, s, lo) - x) <= half * (1 + 1e-5)).all()
+
+
+# ------------------------------------------------------------------------ GPU
+def table_for(lens, page, rng, spare=2, width=None):
+    """Random page permutation: (block table int32 [B, max_pages], number of pages)."""
+    n = [-(-int(x) // page) for x in lens]
+    P = sum(n) + spare
+    perm = rng.permutation(P).astype(np.int32)
+    bt = np.full((len(lens), max(max(n), 1) if width is None else width), -1, np.int32)
+    at = 0
+    for b, k in enumerate(n):
+        bt[b, :k] = perm[at:at + k]
+        at += k
+    return bt, P
+
+
+def np_of(t):
+    """float32 values of a 16-bit tensor."""
+    return t.float().cpu().numpy()
+
+
+class Filled:
+    """A cache with `lens` tokens per sequence, written through append_paged_quant, and what
+    the oracle says it holds."""
+
+    def __init__(self, B, Hkv, D, page, bits, dt, lens, seed=0, index=False, amp=1.0, width=None):
+        import b200attn
+        rng = np.random.default_rng(seed)
+        self.page, self.D, self.bits, self.dt, self.name = page, D, bits, dt, NAME[dt]
+        self.lens = list(lens)
+        self.bt, P = table_for(lens, page, rng, width=width)
+        self.cache = b200attn.QuantCache.empty(P, page, Hkv, D, bits=bits, dtype=dt, index=index)
+        # stale bytes in every block, NaN params among them
+        self.cache.data.copy_(torch.from_numpy(rng.integers(0, 256, self.cache.data.shape, np.uint8)))
+        self.btg = torch.from_numpy(self.bt).cuda()
+        self.k, self.v = [], []
+        for b, n in enumerate(lens):
+            for out, s in ((self.k, 1), (self.v, 2)):
+                x = torch.from_numpy(ora.seeded_normal((1, Hkv, max(n, 1), D), seed + 10 * b + s) * amp)
+                out.append(x.to(dt)[:, :, :n].cuda())
+            if n:
+                b200attn.append_paged_quant(self.k[b], self.v[b], self.cache, self.btg[b:b + 1],
+                                            torch.zeros(1, dtype=torch.int32, device="cuda"))
+        self.kl = torch.tensor(self.lens, dtype=torch.int32, device="cuda")
+
+    def codes(self, b, side):
+        """(codes, scale, min) of sequence b: [Hkv, n, ...]."""
+        x = np_of((self.k, self.v)[side][b])[0]
+        return oq.quantise(x, self.bits, self.name)
+
+
+def check_attention(f, q, O, L, scale=None, pages=None):
+    """O, L against 64 bits within the bound in this file's docstring."""
+    u = torch.finfo(f.dt).eps / 2
+    Hkv = f.cache.num_kv_heads
+    B, H, D = q.shape
+    G = H // Hkv
+    scale = D ** -0.5 if scale is None else scale
+    qn, On, Ln = np_of(q), np_of(O), L.cpu().numpy()
+    for b in range(B):
+        n = f.lens[b]
+        parts = [f.codes(b, s) for s in (0, 1)] if n else None
+        for h in range(Hkv):
+            heads = slice(h * G, (h + 1) * G)
+            if n == 0:
+                assert (On[b, heads] == 0).all() and np.isneginf(Ln[b, heads]).all()
+                continue
+            use = np.arange(n)
+            if pages is not None:
+                lp = pages[b, h][(pages[b, h] >= 0) & (pages[b, h] * f.page < n)]
+                use = np.concatenate([np.arange(p * f.page, min(n, (p + 1) * f.page)) for p in lp]
+                                     or [np.zeros(0, int)]).astype(int)
+            k = oq.values(*(x[h][use] for x in parts[0]))
+            v = oq.values(*(x[h][use] for x in parts[1]))
+            Or, Lr = oq.attend(qn[b, heads], k, v, scale)
+            if len(use) == 0:
+                assert (On[b, heads] == 0).all() and np.isneginf(Ln[b, heads]).all()
+                continue
+            s = qn[b, heads].astype(np.float64) @ k.T * scale
+            e = np.exp(s - s.max(-1, keepdims=True))
+            p = e / e.sum(-1, keepdims=True)
+            sc = np.repeat(parts[1][1][h][use].astype(np.float64), 64, -1)
+            c = parts[1][0][h][use]
+            # fp32: scores are sums of D products, off by a few 2^-24 of their size, and the
+            # probabilities by as much relatively; 2^-17 of it covers sums and exponentials
+            size = (np.abs(qn[b, heads]).astype(np.float64) @ np.abs(k).T * scale).max(-1, keepdims=True)
+            fp32 = 2.0 ** -17 * (1 + size)
+            sub = 2.0 ** -25 * len(use) * sc.max() * (2 ** f.bits - 1) / e.sum(-1, keepdims=True) * 2
+            tol = 1.01 * u * (np.abs(Or) + p @ (sc * c)) + fp32 * (p @ np.abs(v) + p @ (sc * c)) \
+                + (sub if f.dt == F16 else 0) + (2.0 ** -25 if f.dt == F16 else 0)
+            bad = np.abs(On[b, heads] - Or) > tol
+            assert not bad.any(), (b, h, np.abs(On[b, heads] - Or)[bad][:4], tol[bad][:4])
+            assert (np.abs(Ln[b, heads] - Lr) <= fp32[:, 0] * 2).all(), (b, h, Ln[b, heads] - Lr)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,page,bits,dt,start,T", [
+    (128, 16, 4, F16, [0, 5, 31, 16], 1), (128, 16, 4, BF16, [0, 5, 31, 16], 40),
+    (64, 32, 8, F16, [1, 0, 63], 77), (64, 64, 4, BF16, [3], 200), (128, 64, 8, BF16, [0, 100], 1),
+    (128, 32, 8, F16, [7, 2], 33), (64, 16, 4, F16, [15, 16, 17, 0, 2], 16)], ids=str)
+def test_append_is_exact_to_the_bit(D, page, bits, dt, start, T):
+    """Codes and params of the written slots are the oracle's; every other byte is as it was."""
+    import b200attn
+    B, Hkv = len(start), 3
+    rng = np.random.default_rng(1)
+    bt, P = table_for([s + T for s in start], page, rng)
+    cache = b200attn.QuantCache.empty(P, page, Hkv, D, bits=bits, dtype=dt)
+    cache.data.copy_(torch.from_numpy(rng.integers(0, 256, cache.data.shape, np.uint8)))
+    before = cache.data.cpu().numpy()
+    x = [torch.from_numpy(ora.seeded_normal((B, T, Hkv, D), 5 + i)).to(dt).cuda() for i in (0, 1)]
+    kl = torch.tensor(start, dtype=torch.int32, device="cuda")
+    # a [B, Hkv, T, D] view of token-major rows: strided, not copied
+    b200attn.append_paged_quant(x[0].transpose(1, 2), x[1].transpose(1, 2), cache,
+                                torch.from_numpy(bt).cuda(), kl)
+    assert kl.tolist() == [s + T for s in start]
+    want = torch.from_numpy(before.copy())
+    shadow = b200attn.QuantCache(want, page_size=page, head_dim=D, bits=bits, dtype=dt)
+    for side in (0, 1):
+        c, s, lo = oq.quantise(np_of(x[side]), bits, NAME[dt])      # [B, T, Hkv, ...]
+        if bits == 4:
+            c = c[..., ::2] | c[..., 1::2] << 4
+        par = torch.from_numpy(np.stack((s, lo), -1)).to(dt)
+        for b in range(B):
+            for t in range(T):
+                pos = start[b] + t
+                pg, sl = int(bt[b, pos // page]), pos % page
+                shadow.codes(side)[pg, :, sl] = torch.from_numpy(c[b, t])
+                shadow.params(side)[pg, :, sl] = par[b, t]
+    assert torch.equal(cache.data.cpu(), want)
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+def test_append_of_extreme_values(dt, bits):
+    """Constants, zeros, the type's extremes, subnormals, NaN and infinities."""
+    import b200attn
+    big, tiny = torch.finfo(dt).max, torch.finfo(dt).smallest_normal
+    sub = tiny * torch.finfo(dt).eps
+    g = torch.Generator().manual_seed(0)
+    rows = [torch.zeros(128), torch.full((128,), 3.25), torch.full((128,), -big),
+            torch.linspace(-big, big, 128), torch.linspace(0, big, 128),
+            torch.randn(128, generator=g) * tiny, torch.randint(0, 9, (128,), generator=g) * sub,
+            torch.cat((torch.full((64,), big), torch.full((64,), float("nan")))),
+            torch.randn(128, generator=g), torch.randn(128, generator=g), torch.randn(128, generator=g),
+            torch.linspace(-1, 1, 128) * big]
+    rows[9][70], rows[10][3] = float("inf"), -float("inf")
+    x = torch.stack(rows).to(dt)
+    T = len(rows)
+    cache = b200attn.QuantCache.empty(1, 16, 1, 128, bits=bits, dtype=dt, index=True)
+    bt = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    kl = torch.zeros(1, dtype=torch.int32, device="cuda")
+    xg = x[None, None].cuda()
+    b200attn.append_paged_quant(xg, xg, cache, bt, kl)
+    c, s, lo = oq.quantise(np_of(x), bits, NAME[dt])
+    got = oq.unpack(cache.data.cpu().numpy(), 16, 128, bits, NAME[dt])
+    for side in (0, 1):
+        for a, w in zip(got[side], (c, s, lo)):
+            np.testing.assert_array_equal(a[0, 0, :T], w)
+    K, V = b200attn.read_paged_quant(cache, bt, torch.tensor([0, T], dtype=torch.int32, device="cuda"), T, T)
+    np.testing.assert_array_equal(np_of(K)[:, 0], oq.read_back(c, s, lo, NAME[dt]))
+    np.testing.assert_array_equal(np_of(V)[:, 0], oq.read_back(c, s, lo, NAME[dt]))
+    # a finite group stays finite (a linspace over all of bf16's range passes fp32's itself)
+    fine = np.isfinite(np_of(x).reshape(T, 2, 64)).all(-1)
+    assert fine[:3].all() and fine[-1].all() and (np.isfinite(np_of(K).reshape(T, 2, 64)).all(-1) == fine).all()
+    assert np.isnan(cache.index_scale.item()) and not cache.index.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,page,bits,dt", [(128, 16, 4, F16), (64, 32, 8, BF16), (64, 64, 4, F16),
+                                            (128, 64, 8, F16), (128, 32, 4, BF16)], ids=str)
+def test_read_back(D, page, bits, dt):
+    """Whole sequences and ranges of them, packed; other rows of `out` are left as they were."""
+    import b200attn
+    lens = [1, 100, 0, 64, 37]
+    f = Filled(5, 2, D, page, bits, dt, lens, seed=3)
+    want = [[oq.read_back(*f.codes(b, s), NAME[dt]).transpose(1, 0, 2) if n else np.zeros((0, 2, D))
+             for b, n in enumerate(lens)] for s in (0, 1)]
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    out = b200attn.read_paged_quant(f.cache, f.btg, torch.from_numpy(cu).cuda(), int(cu[-1]), max(lens))
+    for s in (0, 1):
+        np.testing.assert_array_equal(np_of(out[s]), np.concatenate(want[s]))
+    # ranges, into rows that leave gaps: 7 free rows at the end
+    start = [0, 33, 0, 15, 36]
+    take = [1, 40, 0, 49, 1]
+    cu = np.concatenate(([0], np.cumsum(take))).astype(np.int32)
+    total = int(cu[-1]) + 7
+    out = [torch.full((total, 2, D), 9.0, dtype=dt, device="cuda") for _ in (0, 1)]
+    res = b200attn.read_paged_quant(f.cache, f.btg, torch.from_numpy(cu).cuda(), total, 49,
+                                    start=torch.tensor(start, dtype=torch.int32, device="cuda"), out=out)
+    assert res[0] is out[0]
+    for s in (0, 1):
+        w = np.concatenate([want[s][b][start[b]:start[b] + take[b]] for b in range(5)])
+        np.testing.assert_array_equal(np_of(out[s])[:-7], w)
+        assert (out[s][-7:] == 9).all()
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+def test_bad_pages_and_lengths_are_flagged():
+    import b200attn
+    dt = F16
+    cache = b200attn.QuantCache.empty(4, 16, 1, 64, dtype=dt, index=True)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    k = torch.ones(3, 1, 20, 64, dtype=dt, device="cuda")
+    b200attn.device_error_flags()
+    # sequence 0: negative length; 1: second page missing; 2: page number past the pool
+    bt = i32([0, 1], [2, -1], [7, 3])
+    b200attn.append_paged_quant(k, k, cache, bt, i32(-4, 0, 0), advance=False)
+    assert b200attn.device_error_flags() & 4
+    got = cache.params(0)[:, 0, :, 0, 1].cpu()
+    assert (got[2] == 1).all() and (got[3, :4] == 1).all() and not got[3, 4:].any() and not got[:2].any()
+    # reading: a missing page reads as zero
+    out = b200attn.read_paged_quant(cache, i32([2, -1]), i32(0, 20), 20, 20)
+    assert b200attn.device_error_flags() & 2
+    assert (out[0][:16] == 1).all() and not out[0][16:].any()
+    # a longer sequence than max_len, and a prefix sum past total: not read
+    keep = [torch.full((20, 1, 64), 5.0, dtype=dt, device="cuda") for _ in (0, 1)]
+    b200attn.read_paged_quant(cache, i32([2, 3]), i32(0, 20), 20, 19, out=keep)
+    assert b200attn.device_error_flags() & 8 and (keep[0] == 5).all()
+    b200attn.read_paged_quant(cache, i32([2, 3]), i32(0, 21), 20, 21, out=keep)
+    assert b200attn.device_error_flags() & 8 and (keep[0] == 5).all()
+    # attention and selection: page 0 instead, and a length that the table cannot hold
+    q = torch.ones(1, 1, 64, dtype=dt, device="cuda")
+    b200attn.decode_paged_quant(q, cache, i32([9]), i32(5))
+    assert b200attn.device_error_flags() & 2
+    b200attn.decode_paged_quant(q, cache, i32([2]), i32(17))
+    assert b200attn.device_error_flags() & 2
+    assert b200attn.select_pages(q, cache, i32([2]), i32(17), 1).tolist() == [[[0]]]
+    assert b200attn.device_error_flags() & 2
+    O, L = b200attn.decode_paged_quant(q, cache, i32([2]), i32(-1))
+    assert not O.any() and torch.isneginf(L).all()
+    assert b200attn.device_error_flags() & 2
+
+
+DECODE = [
+    # B, H, Hkv, D, page, bits, dtype, lens
+    (4, 32, 8, 128, 16, 4, F16, [1, 15, 16, 17]),
+    (3, 8, 2, 128, 16, 4, BF16, [1000, 64, 513]),
+    (4, 3, 3, 64, 32, 8, F16, [0, 63, 300, 64]),
+    (2, 14, 2, 64, 64, 4, BF16, [129, 4000]),
+    (2, 5, 1, 128, 64, 8, F16, [777, 65]),
+    (1, 16, 2, 128, 32, 8, BF16, [2050]),
+    (3, 8, 1, 64, 16, 4, F16, [5000, 0, 31]),
+    (2, 6, 2, 128, 32, 4, F16, [333, 1]),
+    (1, 8, 8, 64, 16, 8, BF16, [48]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hkv,D,page,bits,dt,lens", DECODE, ids=str)
+def test_decode(B, H, Hkv, D, page, bits, dt, lens):
+    import b200attn
+    f = Filled(B, Hkv, D, page, bits, dt, lens, seed=7)
+    q = torch.from_numpy(ora.seeded_normal((B, H, D), 9)).to(dt).cuda()
+    for splits in (None, 1, 3, 40):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_attention(f, q, O, L)
+    O4, L4 = b200attn.decode_paged_quant(q[:, :, None], f.cache, f.btg, f.kl, scale=0.3)
+    assert O4.shape == (B, H, 1, D) and L4.shape == (B, H, 1)
+    check_attention(f, q, O4[:, :, 0], L4[:, :, 0], scale=0.3)
+    again = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl)
+    first = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl)
+    assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("amp", [1e-4, 30.0])
+def test_decode_amplitudes(dt, amp):
+    """Small and large keys and values: what the probabilities are scaled by follows the data."""
+    import b200attn
+    f = Filled(2, 2, 128, 16, 4, dt, [900, 70], seed=17, amp=amp)
+    q = torch.from_numpy(ora.seeded_normal((2, 8, 128), 19)).to(dt).cuda()
+    O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, scale=0.01)
+    check_attention(f, q, O, L, scale=0.01)
+
+
+@pytest.mark.gpu
+def test_decode_of_growing_values():
+    """Values whose step grows by 2^8 along the sequence, and shrinks again."""
+    import b200attn
+    f = Filled(1, 1, 64, 16, 8, F16, [640], seed=27)
+    ramp = torch.exp2(8 - (torch.arange(640) - 320).abs() / 40)[None, None, :, None].cuda()
+    f.v[0] = (f.v[0].float() * ramp).half()
+    b200attn.append_paged_quant(f.k[0], f.v[0], f.cache, f.btg,
+                                torch.zeros(1, dtype=torch.int32, device="cuda"))
+    q = torch.from_numpy(ora.seeded_normal((1, 4, 64), 29)).half().cuda()
+    for splits in (1, 2):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_attention(f, q, O, L)
+
+
+@pytest.mark.gpu
+def test_decode_propagates_nan_and_hides_none():
+    """A token with a NaN in K makes its heads' outputs NaN (not zero); other heads keep theirs."""
+    import b200attn
+    f = Filled(2, 2, 64, 16, 4, F16, [300, 20], seed=37)
+    q = torch.from_numpy(ora.seeded_normal((2, 4, 64), 39)).half().cuda()
+    want = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl)
+    k = f.k[0].clone()
+    k[0, 1, 250, 3] = float("nan")
+    b200attn.append_paged_quant(k, f.v[0], f.cache, f.btg[:1],
+                                torch.zeros(1, dtype=torch.int32, device="cuda"))
+    for splits in (1, 5):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        assert O[0, 2:].isnan().all() and L[0, 2:].isnan().all()
+        assert torch.isfinite(O[0, :2]).all() and torch.isfinite(O[1]).all()
+        torch.testing.assert_close(O[1], want[0][1], atol=2e-3, rtol=2e-3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hkv,D,page,bits,dt,lens,top", [
+    (3, 8, 2, 128, 16, 4, F16, [1000, 64, 513], 5), (2, 6, 2, 64, 32, 8, BF16, [1, 3000], 24),
+    (2, 8, 1, 64, 16, 4, BF16, [0, 9000], 100), (1, 5, 5, 128, 64, 8, F16, [4100], 1),
+    (1, 4, 1, 128, 16, 4, F16, [5000], 400), (4, 7, 1, 64, 16, 8, F16, [16, 17, 2000, 1999], 125)], ids=str)
+def test_index_select_and_sparse_decode(B, H, Hkv, D, page, bits, dt, lens, top):
+    import b200attn
+    f = Filled(B, Hkv, D, page, bits, dt, lens, seed=47, index=True)
+    G = H // Hkv
+    idx, isc = f.cache.index.cpu().numpy(), f.cache.index_scale.cpu().numpy()
+    q = torch.from_numpy(ora.seeded_normal((B, H, D), 49)).to(dt).cuda()
+    pages = b200attn.select_pages(q, f.cache, f.btg, f.kl, top)
+    got = pages.cpu().numpy()
+    for b, n in enumerate(lens):
+        count = -(-n // page)
+        phys = f.bt[b, :count]
+        if n:
+            c, s, lo = f.codes(b, 0)
+            k = oq.read_back(c, s, lo, NAME[dt])
+        for h in range(Hkv):
+            for p in range(count):
+                ci, si = oq.bounds(k[h, p * page:min(n, (p + 1) * page)])
+                np.testing.assert_array_equal(idx[phys[p], h], ci)
+                assert isc[phys[p], h] == si
+            want = oq.select(np_of(q)[b, h * G:(h + 1) * G], idx[phys, h], isc[phys, h], count, top)
+            np.testing.assert_array_equal(got[b, h], want)
+    for splits in (None, 1, 7):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, pages=pages, splits=splits)
+        check_attention(f, q, O, L, pages=got)
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+def test_index_follows_single_appends():
+    """Token by token, through a page that held an older sequence's keys."""
+    import b200attn
+    B, Hkv, D, page = 2, 2, 128, 16
+    f = Filled(B, Hkv, D, page, 4, BF16, [3 * page, page], seed=57, index=True)
+    kl = torch.tensor([0, 14], dtype=torch.int32, device="cuda")      # sequence 0 starts again
+    lens = [0, 14]
+    held = [np.zeros((Hkv, 0, D), np.float32), oq.read_back(*f.codes(1, 0), "bfloat16")[:, :14]]
+    bt = torch.cat((f.btg[:, :1], f.btg[:1, 1:2].expand(2, 1)), 1)
+    bt[1, 1] = f.cache.num_pages - 1
+    bt = bt.contiguous()
+    for step in range(18):                # up to the table's 32 tokens
+        x = torch.from_numpy(ora.seeded_normal((B, Hkv, 1, D), 100 + step)).to(BF16)
+        b200attn.append_paged_quant(x.cuda(), x.cuda(), f.cache, bt, kl)
+        y = oq.read_back(*oq.quantise(np_of(x), 4, "bfloat16"), "bfloat16")
+        for b in range(B):
+            held[b] = np.concatenate((held[b], y[b]), 1)
+            lens[b] += 1
+            p = (lens[b] - 1) // page
+            for h in range(Hkv):
+                ci, si = oq.bounds(held[b][h, p * page:])
+                np.testing.assert_array_equal(f.cache.index[bt[b, p], h].cpu().numpy(), ci)
+                assert f.cache.index_scale[bt[b, p], h].item() == si
+    assert kl.tolist() == lens
+
+
+@pytest.mark.gpu
+def test_select_ties_and_non_finite_scores():
+    """Equal pages: the lowest are taken.  A page or query that is not finite is never left out."""
+    import b200attn
+    D, page, n = 64, 16, 40
+    cache = b200attn.QuantCache.empty(n, page, 1, D, dtype=F16, index=True)
+    cache.index.fill_(5)
+    cache.index_scale.fill_(0.25)
+    bt = torch.arange(n, dtype=torch.int32, device="cuda")[None].contiguous()
+    kl = torch.tensor([n * page - 3], dtype=torch.int32, device="cuda")
+    q = torch.from_numpy(ora.seeded_normal((1, 4, D), 3)).half().cuda()
+    pick = lambda k: b200attn.select_pages(q, cache, bt, kl, k)[0, 0].tolist()  # noqa: E731
+    assert pick(4) == [0, 1, 2, n - 1]
+    cache.index_scale[20], cache.index_scale[7] = float("nan"), 100.0
+    assert pick(3) == ([7, 20, n - 1] if (q.float().sum(-1) > 0).any() else [0, 20, n - 1])
+    assert pick(n + 5) == list(range(n)) + [-1] * 5
+    q[0, 1, 3] = float("nan")                                      # every page scores +infinity
+    assert pick(4) == [0, 1, 2, 3]
+    q.zero_()
+    assert pick(2) == [20, n - 1]
+
+
+@pytest.mark.gpu
+def test_page_lists_of_the_caller():
+    """Negative and out-of-range entries are skipped wherever they stand; none left: O = 0."""
+    import b200attn
+    f = Filled(1, 2, 64, 16, 8, F16, [200], seed=67)
+    q = torch.from_numpy(ora.seeded_normal((1, 4, 64), 69)).half().cuda()
+    lists = np.array([[[-1, 3, -7, 12, 0, 99, -1, -1, 5], [-1] * 9]], np.int32)
+    for splits in (1, 2, 9):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, pages=torch.from_numpy(lists).cuda(),
+                                           splits=splits)
+        check_attention(f, q, O, L, pages=lists)
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Pages whose bytes lie past 4 GiB of the pool."""
+    import b200attn
+    Hkv, D, page = 8, 128, 64
+    per = Hkv * 2 * page * (64 + 8)
+    P = (1 << 32) // per + 40
+    cache = b200attn.QuantCache(torch.empty(P, Hkv, per // Hkv, dtype=torch.uint8, device="cuda"),
+                                page_size=page, head_dim=D, bits=4, dtype=F16)
+    n = 300
+    bt = torch.arange(P - 1, P - 6, -1, dtype=torch.int32, device="cuda")[None].contiguous()
+    kl = torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, v = (torch.from_numpy(ora.seeded_normal((1, Hkv, n, D), s)).half().cuda() for s in (1, 2))
+    b200attn.append_paged_quant(k, v, cache, bt, kl)
+    c = [oq.quantise(np_of(x)[0], 4, "float16") for x in (k, v)]
+    out = b200attn.read_paged_quant(cache, bt, torch.tensor([0, n], dtype=torch.int32, device="cuda"), n, n)
+    for s in (0, 1):
+        np.testing.assert_array_equal(np_of(out[s]).transpose(1, 0, 2), oq.read_back(*c[s], "float16"))
+    q = torch.from_numpy(ora.seeded_normal((1, 32, D), 3)).half().cuda()
+    f = Filled.__new__(Filled)
+    f.cache, f.lens, f.page, f.bits, f.dt, f.name, f.k, f.v = cache, [n], page, 4, F16, "float16", [k], [v]
+    O, L = b200attn.decode_paged_quant(q, cache, bt, kl)
+    check_attention(f, q, O, L)
+
+
+@pytest.mark.gpu
+def test_strided_and_misaligned_inputs():
+    """Views of one fused projection, and rows that are not 16-byte aligned (copied)."""
+    import b200attn
+    f = Filled(2, 2, 64, 16, 4, F16, [50, 33], seed=77)
+    qkv = torch.from_numpy(ora.seeded_normal((2, 8 + 4, 64), 5)).half().cuda()
+    q = qkv[:, :8]
+    want = b200attn.decode_paged_quant(q.contiguous(), f.cache, f.btg, f.kl)
+    got = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl)
+    assert torch.equal(want[0], got[0])
+    odd = torch.zeros(2 * 8 * 64 + 1, dtype=F16, device="cuda")[1:].view(2, 8, 64)
+    odd.copy_(q)
+    assert torch.equal(want[0], b200attn.decode_paged_quant(odd, f.cache, f.btg, f.kl)[0])
+    k = qkv[:, 8:10, None]
+    a, b = f.cache.data.clone(), f.cache.data.clone()
+    kl = f.kl.clone()
+    for data, x in ((a, k), (b, k.contiguous())):
+        c = b200attn.QuantCache(data, page_size=16, head_dim=64, bits=4, dtype=F16)
+        b200attn.append_paged_quant(x, x, c, f.btg, kl - 1, advance=False)
+    assert torch.equal(a, b) and not torch.equal(a, f.cache.data)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    import b200attn as b
+    c = b.QuantCache.empty(4, 16, 1, 64, dtype=F16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    bt, kl = torch.zeros(1, 4, **i32), torch.ones(1, **i32)
+    q = torch.zeros(1, 9, 64, dtype=F16, device="cuda")
+    with pytest.raises(RuntimeError, match="at most 8"):
+        b.decode_paged_quant(q, c, bt, kl)
+    q = q[:, :2]
+    with pytest.raises(RuntimeError, match="dtype"):
+        b.decode_paged_quant(q.bfloat16(), c, bt, kl)
+    with pytest.raises(RuntimeError, match="index"):
+        b.select_pages(q, c, bt, kl, 2)
+    with pytest.raises(RuntimeError, match="scale"):
+        b.decode_paged_quant(q, c, bt, kl, scale=-1.0)
+    with pytest.raises(RuntimeError, match="splits"):
+        b.decode_paged_quant(q, c, bt, kl, splits=0)
+    with pytest.raises(RuntimeError, match="pages"):
+        b.decode_paged_quant(q, c, bt, kl, pages=torch.zeros(1, 2, 3, **i32))
+    with pytest.raises(RuntimeError, match="block_table"):
+        b.decode_paged_quant(q, c, bt.long(), kl)
+    with pytest.raises(RuntimeError, match="kv_lens"):
+        b.decode_paged_quant(q, c, bt, torch.ones(2, **i32))
+    with pytest.raises(RuntimeError, match="max_pages"):
+        b.decode_paged_quant(q, c, bt[:, :0], kl)
+    e = b.decode_paged_quant(q[:0], c, bt[:0], kl[:0])
+    assert e[0].shape == (0, 2, 64)
+    K, V = b.read_paged_quant(c, bt, torch.zeros(2, **i32), 0, 0)
+    assert K.shape == (0, 1, 64)
+    b.append_paged_quant(torch.zeros(1, 1, 0, 64, dtype=F16, device="cuda"),
+                         torch.zeros(1, 1, 0, 64, dtype=F16, device="cuda"), c, bt, kl)
+    assert kl.tolist() == [1]
+
+
+@pytest.mark.gpu
+def test_serving_run_together():
+    """Prompt, chunked prefill over the read-back cache, decode steps, sparse decode: a
+    QuantPagePool as a server uses it, next to attention over the read-back values."""
+    import b200attn
+    from b200attn.quantcache import QuantPagePool
+    B, H, Hkv, D, page, dt = 3, 8, 2, 128, 16, BF16
+    pool = QuantPagePool(80, page, Hkv, D, max_seqs=B, max_pages=24, dtype=dt, bits=8, index=True)
+    k, v = (torch.from_numpy(ora.seeded_normal((B, Hkv, 70, D), s)).to(dt).cuda() for s in (1, 2))
+    pool.append(k, v)
+    k1, v1 = (torch.from_numpy(ora.seeded_normal((2, Hkv, 21, D), s)).to(dt).cuda() for s in (3, 4))
+    pool.append(k1, v1, seqs=[2, 0])
+    assert pool.lengths() == [91, 70, 91] and pool.kv_lens.tolist() == [91, 70, 91]
+    K, V, cu, most = pool.read()
+    assert cu.tolist() == [0, 91, 161, 252] and most == 91
+    # the last 21 tokens' queries of sequences 0 and 2, as a prefill chunk over the cache
+    K2, V2, cu2, _ = pool.read(seqs=[0, 2])
+    assert torch.equal(K2, torch.cat((K[:91], K[161:]))) and torch.equal(V2[91:], V[161:])
+    Q = torch.from_numpy(ora.seeded_normal((42, H, D), 5)).to(dt).cuda()
+    cq = torch.tensor([0, 21, 42], dtype=torch.int32, device="cuda")
+    O, L = b200attn.forward_varlen(Q, K2, V2, cq, cu2, 21, causal=True)
+    # the last query of each chunk sees all keys: the decode step of the same query agrees
+    Od, Ld = pool.decode(Q[[20, 41]].contiguous(), seqs=[0, 2])
+    torch.testing.assert_close(Od.float(), O[[20, 41]].float(), atol=1e-2, rtol=2e-2)
+    torch.testing.assert_close(Ld, L[:, [20, 41]].t(), atol=1e-2, rtol=1e-3)
+    all_pages = pool.decode(Q[[20, 41]].contiguous(), seqs=[0, 2], top_k=6)
+    torch.testing.assert_close(all_pages[0].float(), Od.float(), atol=1e-2, rtol=2e-2)
+    few = pool.decode(Q[:3].contiguous(), top_k=2)
+    assert torch.isfinite(few[0].float()).all()
+    pool.release(1)
+    assert pool.lengths()[1] == 0 and pool.kv_lens.tolist()[1] == 0
+    O1, L1 = pool.decode(Q[:3].contiguous())
+    assert not O1[1].any() and torch.isneginf(L1[1]).all()
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+def test_captured_step_and_side_streams():
+    """A captured step (append, select, decode) replays on new inputs, next to a second graph of
+    the same cache layout and eager calls on another stream."""
+    import b200attn
+    B, H, Hkv, D, page = 2, 8, 2, 64, 16
+    fs = [Filled(B, Hkv, D, page, 4, F16, [600, 90], seed=87 + i, index=True, width=48) for i in (0, 1)]
+    graphs = []
+    for f in fs:
+        # pages for growth past the last full one
+        f.x = torch.zeros(B, Hkv, 1, D, dtype=F16, device="cuda")
+        f.q = torch.zeros(B, H, D, dtype=F16, device="cuda")
+
+        def step(f=f):
+            b200attn.append_paged_quant(f.x, f.x, f.cache, f.btg, f.at, advance=False)
+            pages = b200attn.select_pages(f.q, f.cache, f.btg, f.kl, 9)
+            return b200attn.decode_paged_quant(f.q, f.cache, f.btg, f.kl, pages=pages, splits=3) + [pages]
+
+        f.at = f.kl - 1                      # overwrite each sequence's last token
+        f.step = step
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            f.out = step()
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in fs]
+    for it in range(3):
+        for f, g, s in zip(fs, graphs, streams):
+            f.x.copy_(torch.from_numpy(ora.seeded_normal((B, Hkv, 1, D), 200 + it)).half())
+            f.q.copy_(torch.from_numpy(ora.seeded_normal((B, H, D), 300 + it)).half())
+            s.wait_stream(torch.cuda.current_stream())
+        for f, g, s in zip(fs, graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for f in fs:
+            got = [t.clone() for t in f.out]
+            want = f.step()
+            torch.cuda.synchronize()
+            for a, w in zip(got, want):
+                assert torch.equal(a, w)
+            for b in range(B):
+                f.k[b][0, :, -1] = f.x[b, :, 0]
+                f.v[b][0, :, -1] = f.x[b, :, 0]
+            check_attention(f, f.q, got[0], got[1], pages=got[2].cpu().numpy())
+    assert b200attn.device_error_flags() == 0
