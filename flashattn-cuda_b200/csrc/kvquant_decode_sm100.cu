@@ -176,129 +176,79 @@ __global__ void __launch_bounds__(kSelThreads)
 }
 
 // ------------------------------------------------------------------- attention
-// One CTA per (split, KV head, sequence).  Its four warps take the split's
-// 32-token steps in turn and work alone: each has its own ring of stages that
-// its lanes fill with bulk copies (a whole block per page, one copy), its own
+// One CTA per (split, KV head, sequence).  Its warps take the split's 64-token
+// steps in turn and work alone: each has its own ring of stages that its lanes
+// fill with bulk copies (one copy a page: a block is contiguous), its own
 // online softmax and its own accumulators, so the loop has no barrier between
 // warps; they merge once at the end.
 //
-// Both products run on the tensor cores on the raw codes, which are exact in
-// 16 bits; the (scale, min) pairs are applied outside them in fp32:
+// Both products run on the tensor cores on the raw codes, and the (scale, min)
+// pairs are applied outside them in fp32:
 //   S[tok, h] = sum_g kscale[tok, g] (code . q)_g + kmin[tok, g] qsum[h, g]
 //   O[h, d]   = sum_tok (p vscale[tok, g]) code[tok, d] + sum_tok p vmin[tok, g]
-// so K is used exactly and each p*vscale is the only value rounded to 16 bits.
-// In fp16 the scales are brought to at most 2 by a running power of two, so
-// that p*vscale neither overflows nor sinks into subnormals.
+// so K is used exactly and p*vscale is the only value rounded to 16 bits.
+//   Codes are not converted: a code c in the low mantissa bits of an fp16 with
+// zero exponent IS the subnormal c * 2^-24, which the tensor cores multiply
+// exactly, so unpacking is one mask a pair (and a shift by 8 every second one).
+// Codes masked in place at bits 4-7 are 16 c * 2^-24; the 16 is taken out of q
+// (K) or of the finished channel (V).  Both cache dtypes use fp16 operands: a
+// query head is brought to [2^12, 2^13) by a power of two, and p*vscale to at
+// most 2 by a running one, so neither overflows nor loses bits that matter.
 //
 // The token dimension is M of both products (A = K codes [tok, d], and A =
 // V codes transposed [d, tok]) and the heads are N = 8, so no row of the
 // matrix instructions is wasted for groups of 8 and P needs only an 8x8
 // transpose (movmatrix) between them.  Contraction and output channels are
 // dealt to lanes so that a lane's operand is a run of codes as they lie in
-// memory: unpacking is mask, or-in an exponent, subtract.
+// memory.
 template <int D, int BITS>
 struct DecCfg {
-  static constexpr int kStep = 32;  // tokens per step
+  static constexpr int kStep = 64;  // tokens per step
   static constexpr int kRow = row_bytes(D, BITS);
   static constexpr int kNG = D / kGroup;
-  static constexpr uint32_t kStage = kStep * (2 * kRow + 2 * kNG * 4);
-  static constexpr int kStages = (D == 128 && BITS == 8) ? 2 : 3;
-  static constexpr uint32_t kRing = 4 * kStages * kStage;
-  static constexpr uint32_t kMerge = 4 * (8 * (D + 4) + 16) * 4;
-  static constexpr uint32_t kBody = kRing > kMerge ? kRing : kMerge;
-  static constexpr uint32_t kOffBar = kBody;
-  static constexpr uint32_t kOffValid = kOffBar + 4 * kStages * 8;       // [warp][stage] int2
-  static constexpr uint32_t kOffAbort = kOffValid + 4 * kStages * 8;
-  static constexpr uint32_t kSmem = kOffAbort + 16;
+  static constexpr int kStage = kStep * (2 * kRow + 2 * kNG * 4);
+  // Two stages of 9 or 17 KB a warp; three CTAs of 74 or 70 KB fit an SM.
+  static constexpr int kWarps = (D == 128 && BITS == 8) ? 2 : 4;
+  static constexpr int kStages = 2;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kPad = D + 4;  // merge row, padded against bank conflicts
+  static constexpr int kMerge = kWarps * (8 * kPad + 16) * 4;
+  static constexpr int kOffBar = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kOffValid = kOffBar + kWarps * kStages * 8;  // [warp][stage] int4
+  static constexpr int kOffAbort = kOffValid + kWarps * kStages * 16;
+  static constexpr int kSmem = kOffAbort + 16;
 };
 
-// D[16x8] += A[16x16] B[16x8]
-template <bool BF16>
+// D[16x8] += A[16x16] B[16x8], fp16 operands, fp32 accumulators
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (BF16) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-// (a & b) | c
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b) {
-  using T2 = typename Elem<BF16>::T2;
-  T2 r = __hadd2(*reinterpret_cast<T2*>(&a), *reinterpret_cast<T2*>(&b));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-  using T2 = typename Elem<BF16>::T2;
-  T2 r = __hfma2(*reinterpret_cast<T2*>(&a), *reinterpret_cast<T2*>(&b), *reinterpret_cast<T2*>(&c));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-
-// The four 4-bit codes at bits 4j of each 16-bit half of x, j = 0..3, as exact
-// pairs (low half, high half).  A code is or-ed into the mantissa of a power of
-// two (fp16: 1024 at bits 0-3, and 64 * 16 at bits 4-7; bf16, with 7 mantissa
-// bits: 128 at bits 0-3), which is then subtracted.
-template <bool BF16>
+// The four 4-bit codes at bits 4j of each 16-bit half of x as pairs of fp16
+// subnormals: r[0], r[2] hold c * 2^-24, r[1], r[3] hold 16 c * 2^-24.
 __device__ __forceinline__ void unpack4(uint32_t x, uint32_t* r) {
-  if constexpr (BF16) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      r[j] = add2<true>(and_or(x >> (4 * j), 0x000f000fu, 0x43004300u), 0xc300c300u);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      r[j] = add2<false>(and_or(x, 0x000f000fu, 0x64006400u), 0xe400e400u);
-      r[j + 1] = fma2<false>(and_or(x, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);
-      x >>= 8;
-    }
-  }
+  r[0] = x & 0x000f000fu;
+  r[1] = x & 0x00f000f0u;
+  x >>= 8;
+  r[2] = x & 0x000f000fu;
+  r[3] = x & 0x00f000f0u;
 }
-// The 8-bit codes of x = [c, *, c', *] as an exact pair.  fp16: 1024 + c.
-// bf16 (8 significant bits): 16 (128 + high nibble) - 2176 + (128 + low nibble).
-template <bool BF16>
-__device__ __forceinline__ uint32_t unpack8(uint32_t x) {
-  if constexpr (BF16) {
-    const uint32_t lo = and_or(x, 0x000f000fu, 0x43004300u);
-    const uint32_t hi = and_or(x >> 4, 0x000f000fu, 0x43004300u);
-    return add2<true>(fma2<true>(hi, 0x41804180u, 0xc508c508u), lo);
-  } else {
-    return add2<false>(and_or(x, 0x00ff00ffu, 0x64006400u), 0xe400e400u);
-  }
-}
-
-template <int NG, bool BF16>
-__device__ __forceinline__ void load_params(const uint8_t* p, float2* out) {
-  if constexpr (NG == 2) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    out[0] = param<BF16>(w.x);
-    out[1] = param<BF16>(w.y);
-  } else {
-    out[0] = param<BF16>(*reinterpret_cast<const uint32_t*>(p));
-  }
+// 2^e as fp32, e clamped to the normal range
+__device__ __forceinline__ float pow2i(int e) {
+  return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
 }
 
 template <int D, int BITS, bool BF16>
-__global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
+__global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
     decode_kernel(const void* __restrict__ q, long long q_b, long long q_h,
                   const uint8_t* __restrict__ data, const int32_t* __restrict__ block_table,
                   const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ pages,
@@ -307,7 +257,9 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
                   int tps, int page_shift, int max_pages, int num_pages, float scale_log2) {
   using C = DecCfg<D, BITS>;
   using T1 = typename Elem<BF16>::T;
-  constexpr int ROW = C::kRow, NG = C::kNG, S = C::kStages, STEP = C::kStep;
+  using T2 = typename Elem<BF16>::T2;
+  constexpr int ROW = C::kRow, NG = C::kNG, S = C::kStages, STEP = C::kStep, W = C::kWarps;
+  constexpr int SL = STEP / 16;  // 16-token slabs per step
   extern __shared__ __align__(128) uint8_t smem[];
   const int split = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -320,45 +272,45 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
   const int t_begin = split * tps, t_end = min(span, t_begin + tps);
   const size_t row0 = (size_t)b * H + hkv * G;  // first query head
   if (t_begin >= t_end) {  // no token: an empty partial, or the whole answer
-    for (int i = threadIdx.x; i < G; i += 128) {
+    for (int i = threadIdx.x; i < G; i += 32 * W) {
       if (splits > 1) l_part[(row0 + i) * splits + split] = -INFINITY;
       else if (lse != nullptr) lse[row0 + i] = -INFINITY;
     }
     if (splits == 1)
-      for (int i = threadIdx.x; i < G * D; i += 128)
+      for (int i = threadIdx.x; i < G * D; i += 32 * W)
         static_cast<T1*>(out)[row0 * D + i] = Elem<BF16>::from(0.f);
     return;
   }
 
   // ---------------------------------------------------------------- the ring
-  // A stage holds STEP tokens as blocks of pg = min(page, STEP) tokens.
-  const int pg = min(page_size, STEP);
-  const int np = STEP / pg;  // blocks per stage: 1 or 2
+  const int np_shift = 6 - page_shift;  // log2 of the blocks per stage: 1, 2 or 4
+  const uint32_t blk = (uint32_t)block_bytes(D, 1, BITS) << page_shift;
   uint8_t* ring = smem + warp * S * C::kStage;
-  const uint32_t bar0 = smem_u32(smem + C::kOffBar) + warp * S * 8;
-  int2* s_valid = reinterpret_cast<int2*>(smem + C::kOffValid) + warp * S;
+  const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(smem + C::kOffBar) + warp * S * 8;
+  int* s_valid = reinterpret_cast<int*>(smem + C::kOffValid) + warp * S * 4;  // tokens per slab
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffAbort);
   if (lane < S) mbar_init(bar0 + 8 * lane, 1u);
   if (threadIdx.x == 0) *abort_flag = 0;
   fence_mbar_init();
   __syncthreads();
   const int steps = (t_end - t_begin + STEP - 1) / STEP;
-  const int n = (steps - warp + 3) >> 2;  // this warp's steps
+  const int n = (steps - warp + W - 1) / W;  // this warp's steps
   const int32_t* list = pages == nullptr ? nullptr : pages + ((size_t)b * Hkv + hkv) * n_list;
   const int32_t* table = block_table + (size_t)b * max_pages;
 
-  // Block `lane` (< np) of this warp's step i: its pool page (-1: nothing to
-  // read) and tokens.
-  auto lookup = [&](int i, int& page, int& valid) {
+  // Page numbers are looked up 32 blocks at a time, one a lane, and one window
+  // ahead, so that the two dependent loads are off the loop's path.
+  auto lookup = [&](int k, int& page, int& valid) {  // this warp's block k
     page = -1;
     valid = 0;
-    const int pos = t_begin + (warp + 4 * i) * STEP + lane * pg;
-    if (i >= n || lane >= np || pos >= t_end) return;
+    const int i = k >> np_shift;
+    if (i >= n) return;
+    const int pos = t_begin + (warp + W * i) * STEP + ((k & ((1 << np_shift) - 1)) << page_shift);
+    if (pos >= t_end) return;
     int lp = pos >> page_shift;
     if (list != nullptr) lp = list[lp];
     if (lp < 0 || lp >= max_pages) return;
-    const int first = (lp << page_shift) + (pos & (page_size - 1));
-    valid = min(max(len - first, 0), pg);
+    valid = min(max(len - (lp << page_shift), 0), page_size);
     if (valid == 0) return;
     page = table[lp];
     if (page < 0 || page >= num_pages) {
@@ -366,50 +318,41 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
       page = 0;
     }
   };
-  auto issue = [&](int i, int page, int valid) {
-    const int st = i % S;
-    const uint32_t dst = smem_u32(ring + st * C::kStage), bar = bar0 + 8 * st;
-    const int other = __shfl_sync(0xffffffffu, valid, 1);
-    const unsigned some = __ballot_sync(0xffffffffu, valid > 0);
-    const uint32_t blk = (uint32_t)(pg * (2 * ROW + 2 * NG * 4));
-    if (lane == 0) {
-      s_valid[st] = make_int2(valid, np == 2 ? other : 0);
-      mbar_arrive_expect_tx(bar, __popc(some) * blk);
+  int page0, valid0, page1, valid1;
+  lookup(lane, page0, valid0);
+  lookup(32 + lane, page1, valid1);
+  auto issue = [&](int i, int st) {  // copy step i's blocks into stage st
+    const int k = i << np_shift;
+    if ((k & 31) == 0 && k > 0) {
+      page0 = page1;
+      valid0 = valid1;
+      lookup(k + 32 + lane, page1, valid1);
     }
+    const int page = __shfl_sync(0xffffffffu, page0, (k + lane) & 31);
+    const int valid = __shfl_sync(0xffffffffu, valid0, (k + lane) & 31);
+    // slab `lane` (< 4) lies in block lane / (page / 16)
+    const int slab = __shfl_sync(0xffffffffu, valid0, (k + (lane >> (page_shift - 4))) & 31) -
+                     16 * (lane & ((1 << (page_shift - 4)) - 1));
+    const bool copy = lane < (1 << np_shift) && valid > 0;
+    const int some = __popc(__ballot_sync(0xffffffffu, copy));
+    if (lane < 4) s_valid[4 * st + lane] = min(max(slab, 0), 16);
+    const uint32_t bar = bar0 + 8 * st;
+    if (lane == 0) mbar_arrive_expect_tx(bar, some * blk);
     __syncwarp();
-    const size_t bytes = (size_t)block_bytes(D, 1, BITS) << page_shift;
-    if (page_size <= STEP) {
-      if (valid > 0) bulk_load(dst + lane * blk, data + ((size_t)page * Hkv + hkv) * bytes, blk, bar);
-    } else if (some) {  // a part of a page: its rows of the four pieces
-      const int pool = __shfl_sync(0xffffffffu, page, 0);
-      const int off = (t_begin + (warp + 4 * i) * STEP) & (page_size - 1);
-      if (lane < 4) {
-        const uint8_t* src = data + ((size_t)pool * Hkv + hkv) * bytes;
-        const int side = lane & 1;
-        if (lane < 2)
-          bulk_load(dst + side * STEP * ROW, src + (side * page_size + off) * ROW, STEP * ROW, bar);
-        else
-          bulk_load(dst + 2 * STEP * ROW + side * STEP * NG * 4,
-                    src + 2 * page_size * ROW + (side * page_size + off) * NG * 4, STEP * NG * 4,
-                    bar);
-      }
-    }
+    if (copy)
+      bulk_load(ring0 + st * C::kStage + lane * blk, data + ((size_t)page * Hkv + hkv) * blk, blk,
+                bar);
   };
-  int pageA, validA;
-#pragma unroll 1
-  for (int i = 0; i < S; ++i) {
-    lookup(i, pageA, validA);
-    if (i < n) issue(i, pageA, validA);
-  }
-  lookup(S, pageA, validA);  // the next step's, one step ahead
+  for (int i = 0; i < min(n, S); ++i) issue(i, i);
 
   // ------------------------------------------------------------------ queries
   // B fragments of S: lane (g, t) holds head g's channels 64*grp + 16 t + 0..15
-  // in the order in which a K row's codes unpack.
+  // in the order in which a K row's codes unpack, over 16 where those are 16 c.
   uint32_t qb[NG * 4][2];
-  float qsum[NG][2];  // of heads 2t, 2t+1
+  float qsum[NG][2], sl2[2];  // of heads 2t, 2t+1
   {
     const T1* qp = static_cast<const T1*>(q) + b * q_b + (long long)(hkv * G + g) * q_h + 16 * t;
+    float f[NG][16], top = 0.f;
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
       uint32_t u[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
@@ -417,35 +360,58 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
         *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(qp + gr * 64);
         *reinterpret_cast<uint4*>(u + 4) = *reinterpret_cast<const uint4*>(qp + gr * 64 + 8);
       }
-      float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float2 f = param<BF16>(u[j]);
-        sum += f.x + f.y;
+        const float2 v = param<BF16>(u[j]);
+        f[gr][2 * j] = v.x;
+        f[gr][2 * j + 1] = v.y;
+        top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+      }
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int shift = 139 - (int)(__float_as_uint(top) >> 23);  // to [2^12, 2^13)
+    const float mul = pow2i(shift);
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        f[gr][j] *= mul;
+        sum += f[gr][j];
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= pow2i(-24);  // the codes' factor
       qsum[gr][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
       qsum[gr][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (BITS == 4) {
-          const uint32_t a = u[4 * (k / 2) + (k & 1)], z = u[4 * (k / 2) + (k & 1) + 2];
-          qb[gr * 4 + k][0] = __byte_perm(a, z, 0x5410);
-          qb[gr * 4 + k][1] = __byte_perm(a, z, 0x7632);
+          const float* x = &f[gr][8 * (k / 2) + 2 * (k & 1)];
+          qb[gr * 4 + k][0] = pack2_u32<false>(x[0], x[4]);
+          qb[gr * 4 + k][1] = pack2_u32<false>(x[1] * 0.0625f, x[5] * 0.0625f);
         } else {
-          qb[gr * 4 + k][0] = u[2 * k];
-          qb[gr * 4 + k][1] = u[2 * k + 1];
+          const float* x = &f[gr][4 * k];
+          qb[gr * 4 + k][0] = pack2_u32<false>(x[0], x[1]);
+          qb[gr * 4 + k][1] = pack2_u32<false>(x[2], x[3]);
         }
       }
     }
+    const int e = 24 - min(max(shift, -126), 127);
+    const float s2 = scale_log2 * pow2i(e);  // what a score in these units is in log2
+    sl2[0] = __shfl_sync(0xffffffffu, s2, 8 * t);
+    sl2[1] = __shfl_sync(0xffffffffu, s2, 8 * t + 4);
   }
 
   // --------------------------------------------------------------------- loop
-  float o[NG][4][4];    // [group][tile][(d even, head 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
-  float omin[NG][2];    // sum of p * vmin over this lane's tokens
+  float o[NG][4][4];  // [group][tile][(d even, head 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
+  float omin[NG][2];  // sum of p * vmin over this lane's tokens
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  int vexp = 0;         // fp16: biased exponent of the largest value scale so far
+  // value scales are multiplied by vmul = 2^(127 - vexp), vexp the biased
+  // exponent of the largest so far
+  int vexp = 1;
+  float vmul = pow2i(126);
 #pragma unroll
   for (int gr = 0; gr < NG; ++gr) {
     omin[gr][0] = omin[gr][1] = 0.f;
@@ -454,44 +420,53 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[gr][i][e] = 0.f;
   }
-  // Offsets of 16-token slab s in a stage: pg = 16 puts each slab in a block of
-  // its own, pg = 32 both in one.
-  const uint32_t BLK16 = 16 * (2 * ROW + 2 * NG * 4);
-  const uint32_t code_step = np == 2 ? BLK16 : 16 * ROW;
-  const uint32_t par_step = np == 2 ? BLK16 : 16 * NG * 4;
-  const uint32_t v_off = pg * ROW, kp_off = 2 * pg * ROW, vp_off = kp_off + pg * NG * 4;
+  // Slab s of a stage: codes at (s >> 1) * code_hi + (s & 1) * code_lo, params
+  // likewise; 16-token pages put each slab in a block of its own.
+  const uint32_t code_lo = page_shift == 4 ? blk : 16 * ROW;
+  const uint32_t code_hi = page_shift == 6 ? 32 * ROW : page_shift == 5 ? blk : 2 * blk;
+  const uint32_t par_lo = page_shift == 4 ? blk : 16 * NG * 4;
+  const uint32_t par_hi = page_shift == 6 ? 32 * NG * 4 : page_shift == 5 ? blk : 2 * blk;
+  const uint32_t v_off = ROW << page_shift, vp_off = (NG * 4) << page_shift;
   const int tok = (g >> 1) + (g & 1) * 4;  // S row g is token `tok` of the slab, row g+8 8 later
 
   bool ok = true;
+  int st = 0;
+  uint32_t phase = 0;
   for (int i = 0; i < n; ++i) {
-    const int st = i % S;
-    if (!mbar_wait(bar0 + 8 * st, (i / S) & 1, abort_flag)) {
+    if (!mbar_wait(bar0 + 8 * st, phase, abort_flag)) {
       ok = false;
       break;
     }
     const uint8_t* stage = ring + st * C::kStage;
-    const int2 vd = s_valid[st];
-    // tokens of each slab
-    const int nv[2] = {np == 2 ? vd.x : min(vd.x, 16), np == 2 ? vd.y : max(vd.x - 16, 0)};
+    const int4 nv4 = *reinterpret_cast<const int4*>(s_valid + 4 * st);
+    const int nv[4] = {nv4.x, nv4.y, nv4.z, nv4.w};  // tokens of each slab
 
     // ---- S = K q^T
-    float s[2][4];
-    float2 vp[2][2][NG];  // (scale, min) of V of rows g, g+8
+    float s[SL][4];
+    uint32_t vpar[SL][2][NG];  // (scale, min) of V of rows g, g+8
 #pragma unroll
-    for (int sl = 0; sl < 2; ++sl) {
-      if (nv[sl] <= 0) {  // the same in every lane
+    for (int sl = 0; sl < SL; ++sl) {
+      if (nv[sl] == 0) {  // the same in every lane
         s[sl][0] = s[sl][1] = s[sl][2] = s[sl][3] = -INFINITY;
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) vp[sl][0][gr] = vp[sl][1][gr] = make_float2(0.f, 0.f);
+        for (int gr = 0; gr < NG; ++gr) vpar[sl][0][gr] = vpar[sl][1][gr] = 0u;
         continue;
       }
-      const uint8_t* kc = stage + sl * code_step + tok * ROW;
-      const uint8_t* kp = stage + kp_off + sl * par_step + tok * NG * 4;
-      float2 par[2][NG];
-      load_params<NG, BF16>(kp, par[0]);
-      load_params<NG, BF16>(kp + 8 * NG * 4, par[1]);
-      load_params<NG, BF16>(kp + (vp_off - kp_off), vp[sl][0]);
-      load_params<NG, BF16>(kp + (vp_off - kp_off) + 8 * NG * 4, vp[sl][1]);
+      const uint8_t* kc = stage + (sl >> 1) * code_hi + (sl & 1) * code_lo + tok * ROW;
+      const uint8_t* kp =
+          stage + 2 * v_off + (sl >> 1) * par_hi + (sl & 1) * par_lo + tok * NG * 4;
+      uint32_t kpar[2][NG];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if constexpr (NG == 2) {
+          *reinterpret_cast<uint2*>(kpar[r]) = *reinterpret_cast<const uint2*>(kp + r * 8 * NG * 4);
+          *reinterpret_cast<uint2*>(vpar[sl][r]) =
+              *reinterpret_cast<const uint2*>(kp + vp_off + r * 8 * NG * 4);
+        } else {
+          kpar[r][0] = *reinterpret_cast<const uint32_t*>(kp + r * 8 * NG * 4);
+          vpar[sl][r][0] = *reinterpret_cast<const uint32_t*>(kp + vp_off + r * 8 * NG * 4);
+        }
+      }
       s[sl][0] = s[sl][1] = s[sl][2] = s[sl][3] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
@@ -502,11 +477,11 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             uint32_t a[4], z[4];
-            unpack4<BF16>(w ? x.y : x.x, a);
-            unpack4<BF16>(w ? y.y : y.x, z);
-            mma16816<BF16>(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2 * w][0], qb[gr * 4 + 2 * w][1]);
-            mma16816<BF16>(acc, a[2], z[2], a[3], z[3], qb[gr * 4 + 2 * w + 1][0],
-                           qb[gr * 4 + 2 * w + 1][1]);
+            unpack4(w ? x.y : x.x, a);
+            unpack4(w ? y.y : y.x, z);
+            mma16816(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2 * w][0], qb[gr * 4 + 2 * w][1]);
+            mma16816(acc, a[2], z[2], a[3], z[3], qb[gr * 4 + 2 * w + 1][0],
+                     qb[gr * 4 + 2 * w + 1][1]);
           }
         } else {
           const uint4 x = *reinterpret_cast<const uint4*>(kc + gr * 64 + t * 16);
@@ -514,26 +489,29 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            mma16816<BF16>(acc, unpack8<BF16>(__byte_perm(xs[w], 0, 0x4140)),
-                           unpack8<BF16>(__byte_perm(ys[w], 0, 0x4140)),
-                           unpack8<BF16>(__byte_perm(xs[w], 0, 0x4342)),
-                           unpack8<BF16>(__byte_perm(ys[w], 0, 0x4342)), qb[gr * 4 + w][0],
-                           qb[gr * 4 + w][1]);
+            mma16816(acc, __byte_perm(xs[w], 0, 0x4140), __byte_perm(ys[w], 0, 0x4140),
+                     __byte_perm(xs[w], 0, 0x4342), __byte_perm(ys[w], 0, 0x4342),
+                     qb[gr * 4 + w][0], qb[gr * 4 + w][1]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 pr = par[e >> 1][gr];
-          s[sl][e] = fmaf(pr.x, acc[e], fmaf(pr.y, qsum[gr][e & 1], s[sl][e]));
+        for (int r = 0; r < 2; ++r) {
+          const float2 pr = param<BF16>(kpar[r][gr]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            s[sl][2 * r + h] =
+                fmaf(pr.x, acc[2 * r + h], fmaf(pr.y, qsum[gr][h], s[sl][2 * r + h]));
         }
       }
       // tokens past the end: whatever their slots hold is dropped here
+      if (nv[sl] < 16) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-        if (tok + 8 * r >= nv[sl]) {
-          s[sl][2 * r] = s[sl][2 * r + 1] = -INFINITY;
+        for (int r = 0; r < 2; ++r)
+          if (tok + 8 * r >= nv[sl]) {
+            s[sl][2 * r] = s[sl][2 * r + 1] = -INFINITY;
 #pragma unroll
-          for (int gr = 0; gr < NG; ++gr) vp[sl][r][gr] = make_float2(0.f, 0.f);
-        }
+            for (int gr = 0; gr < NG; ++gr) vpar[sl][r][gr] = 0u;
+          }
+      }
     }
 
     // ---- online softmax, per head over the step's tokens (rows: lanes of one t)
@@ -541,46 +519,45 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
     bool moved = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float mx = fmaxf(fmaxf(s[0][h], s[0][h + 2]), fmaxf(s[1][h], s[1][h + 2]));
+      float mx = fmaxf(s[0][h], s[0][h + 2]);
+#pragma unroll
+      for (int sl = 1; sl < SL; ++sl) mx = fmax3(mx, s[sl][h], s[sl][h + 2]);
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float mn = fmaxf(m[h], mx * scale_log2);
+      const float mn = fmaxf(m[h], mx * sl2[h]);
       const float mu = mn == -INFINITY ? 0.f : mn;
       alpha[h] = ex2_mufu(m[h] - mu);
       moved = moved || alpha[h] != 1.f;
       m[h] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int sl = 0; sl < 2; ++sl)
+      for (int sl = 0; sl < SL; ++sl)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float p = ex2_mufu(fmaf(s[sl][2 * r + h], scale_log2, -mu));
+          const float p = ex2_mufu(fmaf(s[sl][2 * r + h], sl2[h], -mu));
           s[sl][2 * r + h] = p;
           sum += p;
         }
       l[h] = l[h] * alpha[h] + sum;
     }
-    float ao[2] = {alpha[0], alpha[1]};  // of o, which also follows vexp
-    float vmul = 1.f;
-    if constexpr (!BF16) {
-      float big = 0.f;
+    T2 big = *reinterpret_cast<T2*>(&vpar[0][0][0]);  // largest value scale, in .x
 #pragma unroll
-      for (int sl = 0; sl < 2; ++sl)
+    for (int sl = 0; sl < SL; ++sl)
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int gr = 0; gr < NG; ++gr) big = fmaxf(big, vp[sl][r][gr].x);
-      const int e = min((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23), 253);
-      if (e > vexp) {  // the same in every lane
-        const float f = __uint_as_float((uint32_t)max(127 - (e - vexp), 0) << 23);
-        ao[0] *= f;
-        ao[1] *= f;
-        moved = true;
-        vexp = e;
-      }
-      vmul = __uint_as_float((uint32_t)(254 - vexp) << 23);
+        for (int gr = 0; gr < NG; ++gr) big = __hmax2(big, *reinterpret_cast<T2*>(&vpar[sl][r][gr]));
+    const float vbig = Elem<BF16>::unpack(big).x;
+    float f = 1.f;
+    if (__any_sync(0xffffffffu, vbig * vmul >= 2.f)) {
+      const int e = min((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vbig)) >> 23), 253);
+      f = pow2i(vexp - e);
+      moved = true;
+      vexp = e;
+      vmul = pow2i(127 - e);
     }
     if (__any_sync(0xffffffffu, moved)) {
+      const float ao[2] = {alpha[0] * f, alpha[1] * f};
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
         omin[gr][0] *= alpha[0];
@@ -594,55 +571,58 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
 
     // ---- O += V^T P
 #pragma unroll
-    for (int sl = 0; sl < 2; ++sl) {
-      if (nv[sl] <= 0) continue;
+    for (int sl = 0; sl < SL; ++sl) {
+      if (nv[sl] == 0) continue;
+      const uint8_t* vc =
+          stage + v_off + (sl >> 1) * code_hi + (sl & 1) * code_lo + g * BITS + t * ROW;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
         uint32_t pb[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float2 pr = vp[sl][r][gr];
-          const float w = BF16 ? pr.x : pr.x * vmul;
+          const float2 pr = param<BF16>(vpar[sl][r][gr]);
+          const float w = pr.x * vmul;
           omin[gr][0] = fmaf(s[sl][2 * r], pr.y, omin[gr][0]);
           omin[gr][1] = fmaf(s[sl][2 * r + 1], pr.y, omin[gr][1]);
-          pb[r] = movmatrix_trans(pack2_u32<BF16>(s[sl][2 * r] * w, s[sl][2 * r + 1] * w));
+          pb[r] = movmatrix_trans(pack2_u32<false>(s[sl][2 * r] * w, s[sl][2 * r + 1] * w));
         }
-        const uint8_t* vc = stage + v_off + sl * code_step + gr * 8 * BITS + g * BITS + t * ROW;
         if constexpr (BITS == 4) {
-          const uint32_t wa = *reinterpret_cast<const uint32_t*>(vc);
-          const uint32_t wb = *reinterpret_cast<const uint32_t*>(vc + 4 * ROW);
-          const uint32_t wc = *reinterpret_cast<const uint32_t*>(vc + 8 * ROW);
-          const uint32_t wd = *reinterpret_cast<const uint32_t*>(vc + 12 * ROW);
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(vc + gr * 32);
+          const uint32_t wb = *reinterpret_cast<const uint32_t*>(vc + gr * 32 + 4 * ROW);
+          const uint32_t wc = *reinterpret_cast<const uint32_t*>(vc + gr * 32 + 8 * ROW);
+          const uint32_t wd = *reinterpret_cast<const uint32_t*>(vc + gr * 32 + 12 * ROW);
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {  // channels 8g + 4*hf + 0..3
             uint32_t a[4], z[4];
-            unpack4<BF16>(__byte_perm(wa, wb, hf ? 0x7632 : 0x5410), a);
-            unpack4<BF16>(__byte_perm(wc, wd, hf ? 0x7632 : 0x5410), z);
-            mma16816<BF16>(o[gr][2 * hf], a[0], a[1], z[0], z[1], pb[0], pb[1]);
-            mma16816<BF16>(o[gr][2 * hf + 1], a[2], a[3], z[2], z[3], pb[0], pb[1]);
+            unpack4(__byte_perm(wa, wb, hf ? 0x7632 : 0x5410), a);
+            unpack4(__byte_perm(wc, wd, hf ? 0x7632 : 0x5410), z);
+            mma16816(o[gr][2 * hf], a[0], a[1], z[0], z[1], pb[0], pb[1]);
+            mma16816(o[gr][2 * hf + 1], a[2], a[3], z[2], z[3], pb[0], pb[1]);
           }
         } else {
-          const uint2 wa = *reinterpret_cast<const uint2*>(vc);
-          const uint2 wb = *reinterpret_cast<const uint2*>(vc + 4 * ROW);
-          const uint2 wc = *reinterpret_cast<const uint2*>(vc + 8 * ROW);
-          const uint2 wd = *reinterpret_cast<const uint2*>(vc + 12 * ROW);
+          const uint2 wa = *reinterpret_cast<const uint2*>(vc + gr * 64);
+          const uint2 wb = *reinterpret_cast<const uint2*>(vc + gr * 64 + 4 * ROW);
+          const uint2 wc = *reinterpret_cast<const uint2*>(vc + gr * 64 + 8 * ROW);
+          const uint2 wd = *reinterpret_cast<const uint2*>(vc + gr * 64 + 12 * ROW);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // channels 8g + 2k, 2k+1
             const uint32_t xa = k < 2 ? wa.x : wa.y, xb = k < 2 ? wb.x : wb.y;
             const uint32_t xc = k < 2 ? wc.x : wc.y, xd = k < 2 ? wd.x : wd.y;
             const uint32_t s0 = k & 1 ? 0x6622 : 0x4400, s1 = k & 1 ? 0x7733 : 0x5511;
-            mma16816<BF16>(o[gr][k], unpack8<BF16>(__byte_perm(xa, xb, s0)),
-                           unpack8<BF16>(__byte_perm(xa, xb, s1)),
-                           unpack8<BF16>(__byte_perm(xc, xd, s0)),
-                           unpack8<BF16>(__byte_perm(xc, xd, s1)), pb[0], pb[1]);
+            mma16816(o[gr][k], __byte_perm(xa, xb, s0) & 0x00ff00ffu,
+                     __byte_perm(xa, xb, s1) & 0x00ff00ffu, __byte_perm(xc, xd, s0) & 0x00ff00ffu,
+                     __byte_perm(xc, xd, s1) & 0x00ff00ffu, pb[0], pb[1]);
           }
         }
       }
     }
 
     __syncwarp();  // every lane has read the stage
-    if (i + S < n) issue(i + S, pageA, validA);
-    lookup(i + S + 1, pageA, validA);
+    if (i + S < n) issue(i + S, st);
+    if (++st == S) {
+      st = 0;
+      phase ^= 1u;
+    }
   }
   if (!ok) {
     // A copy never arrived.  Give the ones still in flight a bounded time to
@@ -665,12 +645,14 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
     }
     if (!ok) l[h] = 0.f;
   }
-  const float vscale = BF16 ? 1.f : __uint_as_float((uint32_t)vexp << 23);
+  const float vscale = pow2i(vexp - 127);
+  constexpr float kEven = 16777216.f;  // 2^24: the codes' factor
+  constexpr float kOdd = BITS == 4 ? 1048576.f : kEven;  // odd channels were 16 c
   __syncthreads();  // the rings are drained: their memory holds the merge now
-  constexpr int P = D + 4;  // padded against bank conflicts
-  float* mo = reinterpret_cast<float*>(smem);  // [4][8][P]
-  float* mm = mo + 4 * 8 * P;                  // [4][8] m, [4][8] l
-  float* ml = mm + 32;
+  constexpr int P = C::kPad;
+  float* mo = reinterpret_cast<float*>(smem);  // [W][8][P]
+  float* mm = mo + W * 8 * P;                  // [W][8] m, [W][8] l
+  float* ml = mm + W * 8;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float* dst = mo + (warp * 8 + 2 * t + h) * P + 8 * g;
@@ -679,26 +661,26 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         *reinterpret_cast<float2*>(dst + gr * 64 + 2 * k) =
-            make_float2(fmaf(o[gr][k][h], vscale, omin[gr][h]),
-                        fmaf(o[gr][k][2 + h], vscale, omin[gr][h]));
+            make_float2(fmaf(o[gr][k][h] * kEven, vscale, omin[gr][h]),
+                        fmaf(o[gr][k][2 + h] * kOdd, vscale, omin[gr][h]));
     if (g == 0) {
       mm[warp * 8 + 2 * t + h] = m[h];
       ml[warp * 8 + 2 * t + h] = l[h];
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < G * D; i += 128) {
+  for (int i = threadIdx.x; i < G * D; i += 32 * W) {
     const int h = i / D, d = i % D;
     float M = -INFINITY, L = 0.f, acc = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, mm[w * 8 + h]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, mm[w * 8 + h]);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float lw = ml[w * 8 + h];
       if (lw == 0.f) continue;  // no token
-      const float f = ex2_mufu(mm[w * 8 + h] - M);
-      L += lw * f;
-      acc += mo[(w * 8 + h) * P + d] * f;
+      const float x = ex2_mufu(mm[w * 8 + h] - M);
+      L += lw * x;
+      acc += mo[(w * 8 + h) * P + d] * x;
     }
     const float val = L == 0.f ? 0.f : acc / L;
     const float ll = L == 0.f ? -INFINITY : M * kLn2 + logf(L);
@@ -713,26 +695,77 @@ __global__ void __launch_bounds__(128, (BITS == 8 && D == 128) ? 3 : 4)
   }
 }
 
-// One CTA of D threads per (sequence, query head).  A split whose l is -inf has
-// no token and its o is not read; a NaN goes through to O and L.
-template <bool BF16>
-__global__ void combine_kernel(const float* __restrict__ o_part, const float* __restrict__ l_part,
-                               void* __restrict__ out, float* __restrict__ lse, int S, int D) {
+// One CTA of 4 warps per (sequence, query head).  A split whose l is -inf has
+// no token and its o is not read; a NaN goes through to O and L.  The splits'
+// weights are made first, one a thread; then each row of a split is read as
+// 16 bytes a lane, with eight rows in flight a warp, so that a load's latency
+// is paid a few times and not once per split.
+constexpr int kChunk = 512;  // weights held at a time
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128)
+    combine_kernel(const float* __restrict__ o_part, const float* __restrict__ l_part,
+                   void* __restrict__ out, float* __restrict__ lse, int S) {
+  constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
+  __shared__ float s_w[kChunk], s_red[2][4];
+  __shared__ float4 s_acc[4 * RPW][LPR];
   const size_t row = blockIdx.x;
-  const int d = threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* lp = l_part + row * S;
+  const float4* op = reinterpret_cast<const float4*>(o_part + row * S * D);
   float M = -INFINITY;
-  for (int s = 0; s < S; ++s) M = fmaxf(M, lp[s]);
-  float L = 0.f, acc = 0.f;
-  for (int s = 0; s < S; ++s) {
-    if (lp[s] == -INFINITY) continue;
-    const float w = expf(lp[s] - M);
-    L += w;
-    acc += w * o_part[(row * S + s) * D + d];
+  for (int s = threadIdx.x; s < S; s += 128) M = fmaxf(M, lp[s]);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  if (lane == 0) s_red[0][warp] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+  const int sub = warp * RPW + lane / LPR, c = lane % LPR;
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = 0; c0 < S; c0 += kChunk) {
+    const int cn = min(kChunk, S - c0);
+    __syncthreads();
+    for (int s = threadIdx.x; s < cn; s += 128) {
+      const float v = lp[c0 + s];
+      const float w = v == -INFINITY ? 0.f : expf(v - M);
+      s_w[s] = w;
+      L += w;
+    }
+    __syncthreads();
+    for (int s0 = sub; s0 < cn; s0 += 8 * 4 * RPW) {
+      float4 v[8];
+      float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int s = s0 + k * 4 * RPW;
+        w[k] = s < cn ? s_w[s] : 0.f;
+        // a weight of zero may stand for a row that was not written
+        v[k] = w[k] != 0.f ? op[(size_t)(c0 + s) * LPR + c] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        acc.x = fmaf(w[k], v[k].x, acc.x);
+        acc.y = fmaf(w[k], v[k].y, acc.y);
+        acc.z = fmaf(w[k], v[k].z, acc.z);
+        acc.w = fmaf(w[k], v[k].w, acc.w);
+      }
+    }
   }
-  static_cast<typename Elem<BF16>::T*>(out)[row * D + d] =
-      Elem<BF16>::from(L == 0.f ? 0.f : acc / L);
-  if (d == 0 && lse != nullptr) lse[row] = L == 0.f ? -INFINITY : M + logf(L);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  if (lane == 0) s_red[1][warp] = L;
+  s_acc[sub][c] = acc;
+  __syncthreads();
+  L = s_red[1][0] + s_red[1][1] + s_red[1][2] + s_red[1][3];
+  if (threadIdx.x < D) {
+    float a = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4 * RPW; ++k)
+      a += reinterpret_cast<const float*>(s_acc[k])[threadIdx.x];
+    static_cast<typename Elem<BF16>::T*>(out)[row * D + threadIdx.x] =
+        Elem<BF16>::from(L == 0.f ? 0.f : a / L);
+  }
+  if (threadIdx.x == 0 && lse != nullptr) lse[row] = L == 0.f ? -INFINITY : M + logf(L);
 }
 
 }  // namespace kvq
@@ -781,7 +814,7 @@ static int launch_kvq_decode(const void* q, int64_t q_b, int64_t q_h, const uint
                              cudaStream_t stream) {
   using namespace kvq;
   auto kern = decode_kernel<D, BITS, BF16>;
-  constexpr int smem = (int)DecCfg<D, BITS>::kSmem;
+  constexpr int smem = DecCfg<D, BITS>::kSmem;
   static bool attr_done[kMaxDevices] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
@@ -791,13 +824,14 @@ static int launch_kvq_decode(const void* q, int64_t q_b, int64_t q_h, const uint
     if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(quantised decode)");
     attr_done[dev] = true;
   }
-  kern<<<dim3((unsigned)splits, (unsigned)Hkv, (unsigned)B), 128, smem, stream>>>(
+  kern<<<dim3((unsigned)splits, (unsigned)Hkv, (unsigned)B), 32 * DecCfg<D, BITS>::kWarps, smem,
+         stream>>>(
       q, q_b, q_h, data, block_table, kv_lens, pages, n_list, o_part, l_part, o, lse, G, Hkv,
       splits, tps, page_shift, max_pages, num_pages, scale * kLog2e);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "quantised decode kernel launch");
   if (splits > 1) {
-    combine_kernel<BF16><<<B * G * Hkv, D, 0, stream>>>(o_part, l_part, o, lse, splits, D);
+    combine_kernel<D, BF16><<<B * G * Hkv, 128, 0, stream>>>(o_part, l_part, o, lse, splits);
     e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(e, "quantised decode combine launch");
   }
