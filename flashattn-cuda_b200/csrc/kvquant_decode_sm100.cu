@@ -5,6 +5,8 @@
 //   scores_kernel / select_kernel   the top_k pages of every (sequence, KV head)
 //   decode_kernel                   split-KV partials over all or the selected pages
 //   combine_kernel                  LSE-weighted merge of the splits
+#include <type_traits>
+
 #include "kvquant.cuh"
 #include "b2a_host.h"
 
@@ -222,15 +224,24 @@ struct DecCfg {
 // D[16x8] += A[16x16] B[16x8], fp16 operands, fp32 accumulators
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// D[16x8] = A[16x16] B[16x8]
+__device__ __forceinline__ void mma16816_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 // The four 4-bit codes at bits 4j of each 16-bit half of x as pairs of fp16
@@ -429,24 +440,17 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
   const uint32_t v_off = ROW << page_shift, vp_off = (NG * 4) << page_shift;
   const int tok = (g >> 1) + (g & 1) * 4;  // S row g is token `tok` of the slab, row g+8 8 later
 
-  bool ok = true;
-  int st = 0;
-  uint32_t phase = 0;
-  for (int i = 0; i < n; ++i) {
-    if (!mbar_wait(bar0 + 8 * st, phase, abort_flag)) {
-      ok = false;
-      break;
-    }
-    const uint8_t* stage = ring + st * C::kStage;
-    const int4 nv4 = *reinterpret_cast<const int4*>(s_valid + 4 * st);
-    const int nv[4] = {nv4.x, nv4.y, nv4.z, nv4.w};  // tokens of each slab
+  // One step; nv: tokens of each slab.  FULL: all of them, known by the caller,
+  // which leaves one run of straight code whose slabs overlap.
+  auto step = [&](auto full, const uint8_t* stage, const int (&nv)[4]) {
+    constexpr bool FULL = decltype(full)::value;
 
     // ---- S = K q^T
     float s[SL][4];
     uint32_t vpar[SL][2][NG];  // (scale, min) of V of rows g, g+8
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
-      if (nv[sl] == 0) {  // the same in every lane
+      if (!FULL && nv[sl] == 0) {  // the same in every lane
         s[sl][0] = s[sl][1] = s[sl][2] = s[sl][3] = -INFINITY;
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) vpar[sl][0][gr] = vpar[sl][1][gr] = 0u;
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
       s[sl][0] = s[sl][1] = s[sl][2] = s[sl][3] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        float acc[4];
         if constexpr (BITS == 4) {
           const uint2 x = *reinterpret_cast<const uint2*>(kc + gr * 32 + t * 8);
           const uint2 y = *reinterpret_cast<const uint2*>(kc + 8 * ROW + gr * 32 + t * 8);
@@ -479,7 +483,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
             uint32_t a[4], z[4];
             unpack4(w ? x.y : x.x, a);
             unpack4(w ? y.y : y.x, z);
-            mma16816(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2 * w][0], qb[gr * 4 + 2 * w][1]);
+            if (w == 0) mma16816_first(acc, a[0], z[0], a[1], z[1], qb[gr * 4][0], qb[gr * 4][1]);
+            else mma16816(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2][0], qb[gr * 4 + 2][1]);
             mma16816(acc, a[2], z[2], a[3], z[3], qb[gr * 4 + 2 * w + 1][0],
                      qb[gr * 4 + 2 * w + 1][1]);
           }
@@ -488,10 +493,12 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
           const uint4 y = *reinterpret_cast<const uint4*>(kc + 8 * ROW + gr * 64 + t * 16);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
-            mma16816(acc, __byte_perm(xs[w], 0, 0x4140), __byte_perm(ys[w], 0, 0x4140),
-                     __byte_perm(xs[w], 0, 0x4342), __byte_perm(ys[w], 0, 0x4342),
-                     qb[gr * 4 + w][0], qb[gr * 4 + w][1]);
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a0 = __byte_perm(xs[w], 0, 0x4140), a1 = __byte_perm(ys[w], 0, 0x4140);
+            const uint32_t a2 = __byte_perm(xs[w], 0, 0x4342), a3 = __byte_perm(ys[w], 0, 0x4342);
+            if (w == 0) mma16816_first(acc, a0, a1, a2, a3, qb[gr * 4][0], qb[gr * 4][1]);
+            else mma16816(acc, a0, a1, a2, a3, qb[gr * 4 + w][0], qb[gr * 4 + w][1]);
+          }
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
         }
       }
       // tokens past the end: whatever their slots hold is dropped here
-      if (nv[sl] < 16) {
+      if (!FULL && nv[sl] < 16) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
           if (tok + 8 * r >= nv[sl]) {
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
     // ---- O += V^T P
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
-      if (nv[sl] == 0) continue;
+      if (!FULL && nv[sl] == 0) continue;
       const uint8_t* vc =
           stage + v_off + (sl >> 1) * code_hi + (sl & 1) * code_lo + g * BITS + t * ROW;
 #pragma unroll
@@ -617,6 +624,21 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
       }
     }
 
+  };
+
+  bool ok = true;
+  int st = 0;
+  uint32_t phase = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!mbar_wait(bar0 + 8 * st, phase, abort_flag)) {
+      ok = false;
+      break;
+    }
+    const uint8_t* stage = ring + st * C::kStage;
+    const int4 nv4 = *reinterpret_cast<const int4*>(s_valid + 4 * st);
+    const int nv[4] = {nv4.x, nv4.y, nv4.z, nv4.w};
+    if (nv4.x + nv4.y + nv4.z + nv4.w == STEP) step(std::true_type{}, stage, nv);
+    else step(std::false_type{}, stage, nv);
     __syncwarp();  // every lane has read the stage
     if (i + S < n) issue(i + S, st);
     if (++st == S) {
