@@ -64,10 +64,11 @@ _SIGNATURES = {
     # q q_strides index index_scale bt lens keys pages
     # | B H Hkv D page max_pages num_pages top_k dtype | stream
     "b2a_kvq_select_pages": (_c_int, [_vp] * 8 + [_c_int] * 9 + [_vp]),
-    "b2a_kvq_decode_splits": (_c_int, [_c_int, _c_int, ctypes.c_int64]),
-    # q q_strides data bt lens pages | n_pages | o_part l_part o lse
-    # | B H Hkv D page max_pages num_pages splits bits dtype | scale stream
-    "b2a_kvq_decode_paged": (_c_int, [_vp] * 6 + [_c_int] + [_vp] * 4 + [_c_int] * 10
+    "b2a_kvq_decode_workers": (_c_int, [_c_int] * 4 + [ctypes.c_int64]),
+    "b2a_kvq_decode_workspace_floats": (ctypes.c_int64, [_c_int] * 5),
+    # q q_strides data bt lens pages | n_pages | workspace o lse
+    # | B H Hkv D page max_pages num_pages workers bits dtype | scale stream
+    "b2a_kvq_decode_paged": (_c_int, [_vp] * 6 + [_c_int] + [_vp] * 3 + [_c_int] * 10
                              + [_c_float, _vp]),
     "b2a_device_error": (_c_int, [ctypes.POINTER(ctypes.c_uint32)]),
     "b2a_selftest_wait_timeout": (_c_int, [_c_int, _vp]),

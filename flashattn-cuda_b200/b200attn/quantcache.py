@@ -254,7 +254,7 @@ def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Te
     """Decode attention over a quantised cache: [O, L] shaped like q ([B, H, D] or
     [B, H, 1, D]); kv_lens may hold zeros (O = 0, L = -inf).  `pages` int32 [B, Hkv, n]
     (from select_pages) restricts each KV head to those pages; negative entries are skipped.
-    `splits` overrides the number of pieces a sequence is cut into."""
+    `splits` overrides the number of warps that share the work, as a multiple of B * Hkv."""
     q3, had_len = _check_query(q, cache)
     B, H, D = q3.shape
     _check_table(cache, block_table, kv_lens, "kv_lens", B)
@@ -273,20 +273,20 @@ def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Te
         O = torch.empty((B, H, D), dtype=cache.dtype, device=dev)
         L = torch.empty((B, H), dtype=torch.float32, device=dev)
         if B > 0:
-            most = min(n_pages, block_table.shape[1]) if n_pages else block_table.shape[1]
-            S = (lib.b2a_kvq_decode_splits(B, Hkv, most * cache.page_size) if splits is None
-                 else int(splits))
-            part = (torch.empty(B * H * S * (D + 1), dtype=torch.float32, device=dev)
-                    if S > 1 else None)
-            po = _ptr(part)
+            if splits is None:
+                workers = lib.b2a_kvq_decode_workers(
+                    B, Hkv, D, cache.bits, (n_pages or block_table.shape[1]) * cache.page_size)
+            else:
+                workers = int(splits) * B * Hkv
+            ws = torch.empty(max(lib.b2a_kvq_decode_workspace_floats(B, H, Hkv, D, workers), 1),
+                             dtype=torch.float32, device=dev)
             qc, qs = _row_strides(q3, 2)
             _lib.check(lib.b2a_kvq_decode_paged(
                 qc.data_ptr(), qs, cache.data.data_ptr(), block_table.data_ptr(),
-                kv_lens.data_ptr(), _ptr(pages), n_pages, po,
-                None if po is None else po + 4 * B * H * S * D, O.data_ptr(), L.data_ptr(), B, H,
-                Hkv, D, cache.page_size, block_table.shape[1], cache.num_pages, S, cache.bits,
-                _DT[cache.dtype], float(D) ** -0.5 if scale is None else float(scale),
-                _stream(dev)))
+                kv_lens.data_ptr(), _ptr(pages), n_pages, ws.data_ptr(), O.data_ptr(),
+                L.data_ptr(), B, H, Hkv, D, cache.page_size, block_table.shape[1],
+                cache.num_pages, workers, cache.bits, _DT[cache.dtype],
+                float(D) ** -0.5 if scale is None else float(scale), _stream(dev)))
     if had_len:
         return [O.unsqueeze(2), L.unsqueeze(2)]
     return [O, L]

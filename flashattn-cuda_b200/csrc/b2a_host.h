@@ -100,12 +100,13 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
                         const int32_t* kv_lens, uint32_t* keys, int32_t* pages, int B, int H,
                         int Hkv, int D, int page_size, int max_pages, int num_pages, int top_k,
                         int dtype, cudaStream_t stream);
-int kvq_decode_splits(int B, int Hkv, long long max_tokens);
+int kvq_decode_workers(int B, int Hkv, int D, int bits, long long max_tokens);
+int64_t kvq_decode_workspace_floats(int B, int H, int Hkv, int D, int workers);
 int kvq_decode_dispatch(const void* q, int64_t q_b, int64_t q_h, const void* data,
                         const int32_t* block_table, const int32_t* kv_lens, const int32_t* pages,
-                        int n_list, float* o_part, float* l_part, void* o, float* lse, int B,
-                        int H, int Hkv, int D, int page_size, int max_pages, int num_pages,
-                        int splits, int bits, int dtype, float scale, cudaStream_t stream);
+                        int n_list, float* workspace, void* o, float* lse, int B, int H, int Hkv,
+                        int D, int page_size, int max_pages, int num_pages, int workers, int bits,
+                        int dtype, float scale, cudaStream_t stream);
 // combine_dispatch's dtype for an fp32 merged partial (o, lse) instead of O.
 constexpr int kCombineF32 = 100;
 // ranks > 1: partials of `ranks` ranks, rank r's o / l blocks `rank_stride`

@@ -568,24 +568,31 @@ int b2a_kvq_select_pages(const void* q, const int64_t* q_strides, const int8_t* 
                              top_k, dtype, static_cast<cudaStream_t>(stream));
 }
 
-int b2a_kvq_decode_splits(int B, int Hkv, int64_t max_tokens) {
+int b2a_kvq_decode_workers(int B, int Hkv, int D, int bits, int64_t max_tokens) {
   if (B <= 0 || Hkv <= 0 || max_tokens <= 0) return 1;
-  return kvq_decode_splits(B, Hkv, max_tokens);
+  return kvq_decode_workers(B, Hkv, D, bits, max_tokens);
+}
+
+int64_t b2a_kvq_decode_workspace_floats(int B, int H, int Hkv, int D, int workers) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || D <= 0 || workers <= 0) return 0;
+  return kvq_decode_workspace_floats(B, H, Hkv, D, workers);
 }
 
 int b2a_kvq_decode_paged(const void* q, const int64_t* q_strides, const void* data,
                          const int32_t* block_table, const int32_t* kv_lens, const int32_t* pages,
-                         int n_pages, float* o_part, float* l_part, void* o, float* lse, int B,
-                         int H, int Hkv, int D, int page_size, int max_pages, int num_pages,
-                         int splits, int bits, int dtype, float scale, void* stream) {
+                         int n_pages, float* workspace, void* o, float* lse, int B, int H, int Hkv,
+                         int D, int page_size, int max_pages, int num_pages, int workers, int bits,
+                         int dtype, float scale, void* stream) {
   t_last_error[0] = 0;
   B2A_TRY(kvq_checks(B, Hkv, D, page_size, max_pages, num_pages, bits, dtype));
   B2A_TRY(kvq_heads(H, Hkv));
-  if (splits <= 0 || splits > 65535)
-    return set_error(B2A_ERR_INVALID_ARG, "splits must be in 1 .. 65535");
+  if (workers <= 0 || workers > (1 << 20))
+    return set_error(B2A_ERR_INVALID_ARG, "workers (splits) must be in 1 .. 2^20");
   if (pages != nullptr && (n_pages <= 0 || (int64_t)n_pages * page_size > 0x7fff0000))
     return set_error(B2A_ERR_INVALID_ARG, "n_pages must be > 0 and n_pages * page_size < 2^31");
-  if ((int64_t)B * H > 0x7fffffff) return set_error(B2A_ERR_INVALID_ARG, "B*H too large");
+  if ((int64_t)B * H > 0x7fffffff / 2) return set_error(B2A_ERR_INVALID_ARG, "B*H too large");
+  if ((int64_t)num_pages * Hkv > 0x7fffffff)
+    return set_error(B2A_ERR_INVALID_ARG, "num_pages * Hkv too large");
   if (!(scale > 0.f)) return set_error(B2A_ERR_INVALID_ARG, "scale must be > 0");
   B2A_TRY(kvq_strides(q_strides, 2, "q"));
   B2A_TRY(check_device_ptr(q, "q"));
@@ -593,15 +600,12 @@ int b2a_kvq_decode_paged(const void* q, const int64_t* q_strides, const void* da
   B2A_TRY(check_ptr_align(block_table, "block_table", 4));
   B2A_TRY(check_ptr_align(kv_lens, "kv_lens", 4));
   if (pages != nullptr) B2A_TRY(check_ptr_align(pages, "pages", 4));
-  if (splits > 1) {
-    B2A_TRY(check_device_ptr(o_part, "o_part"));
-    B2A_TRY(check_ptr_align(l_part, "l_part", 4));
-  }
+  B2A_TRY(check_device_ptr(workspace, "workspace"));
   B2A_TRY(check_device_ptr(o, "O"));
   if (lse != nullptr) B2A_TRY(check_ptr_align(lse, "L", 4));
   return kvq_decode_dispatch(q, q_strides[0], q_strides[1], data, block_table, kv_lens, pages,
-                             n_pages, o_part, l_part, o, lse, B, H, Hkv, D, page_size, max_pages,
-                             num_pages, splits, bits, dtype, scale,
+                             n_pages, workspace, o, lse, B, H, Hkv, D, page_size, max_pages,
+                             num_pages, workers, bits, dtype, scale,
                              static_cast<cudaStream_t>(stream));
 }
 

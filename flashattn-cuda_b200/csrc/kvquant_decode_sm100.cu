@@ -3,8 +3,8 @@
 // by a cheap score.
 //
 //   scores_kernel / select_kernel   the top_k pages of every (sequence, KV head)
-//   decode_kernel                   split-KV partials over all or the selected pages
-//   combine_kernel                  LSE-weighted merge of the splits
+//   decode_kernel                   attention over all or the selected pages
+//   combine_kernel                  LSE-weighted merge of what several warps shared
 #include <type_traits>
 
 #include "kvquant.cuh"
@@ -178,11 +178,13 @@ __global__ void __launch_bounds__(kSelThreads)
 }
 
 // ------------------------------------------------------------------- attention
-// One CTA per (split, KV head, sequence).  Its warps take the split's 64-token
-// steps in turn and work alone: each has its own ring of stages that its lanes
-// fill with bulk copies (one copy a page: a block is contiguous), its own
-// online softmax and its own accumulators, so the loop has no barrier between
-// warps; they merge once at the end.
+// The work is a list of 64-token steps: all steps of KV head 0 of sequence 0,
+// of its head 1, ..., of sequence 1, ...  Every warp takes an equal run of it,
+// whatever the lengths, and works alone: it fills its own ring of stages with
+// bulk copies (one a page: a block is contiguous), keeps its own online softmax
+// and never waits for another warp.  A (sequence, KV head) that lies in one
+// run is finished by its warp; the partials of one that is cut are merged by
+// combine_kernel.
 //
 // Both products run on the tensor cores on the raw codes, and the (scale, min)
 // pairs are applied outside them in fp32:
@@ -203,6 +205,11 @@ __global__ void __launch_bounds__(kSelThreads)
 // transpose (movmatrix) between them.  Contraction and output channels are
 // dealt to lanes so that a lane's operand is a run of codes as they lie in
 // memory.
+//   HALF (groups of up to 4 heads): the four spare columns hold the same heads
+// again, with the second half of the contraction in S and of the tokens in O.
+// A lane then keeps one token row instead of two, and the scores, exponentials
+// and products with the scales are done once each instead of half of them for
+// columns that nobody reads.
 template <int D, int BITS>
 struct DecCfg {
   static constexpr int kStep = 64;  // tokens per step
@@ -212,13 +219,11 @@ struct DecCfg {
   // Two stages of 9 or 17 KB a warp; three CTAs of 74 or 70 KB fit an SM.
   static constexpr int kWarps = (D == 128 && BITS == 8) ? 2 : 4;
   static constexpr int kStages = 2;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kPad = D + 4;  // merge row, padded against bank conflicts
-  static constexpr int kMerge = kWarps * (8 * kPad + 16) * 4;
-  static constexpr int kOffBar = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kOffValid = kOffBar + kWarps * kStages * 8;  // [warp][stage] int4
-  static constexpr int kOffAbort = kOffValid + kWarps * kStages * 16;
-  static constexpr int kSmem = kOffAbort + 16;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kOffBar = kWarps * kRing;
+  static constexpr int kOffValid = kOffBar + kWarps * kStages * 8;    // [warp][stage] int4
+  static constexpr int kOffAbort = kOffValid + kWarps * kStages * 16;  // [warp] int
+  static constexpr int kSmem = kOffAbort + kWarps * 4;
 };
 
 // D[16x8] += A[16x16] B[16x8], fp16 operands, fp32 accumulators
@@ -258,116 +263,180 @@ __device__ __forceinline__ float pow2i(int e) {
   return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
 }
 
-template <int D, int BITS, bool BF16>
+// The steps of sequence b.
+__device__ __forceinline__ int seq_steps(int len, int n_list, int page_shift) {
+  if (len == 0) return 0;
+  const long long tokens = n_list > 0 ? (long long)n_list << page_shift : len;
+  return (int)((tokens + 63) >> 6);
+}
+
+template <int D, int BITS, bool BF16, bool HALF>
 __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
     decode_kernel(const void* __restrict__ q, long long q_b, long long q_h,
                   const uint8_t* __restrict__ data, const int32_t* __restrict__ block_table,
                   const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ pages,
                   int n_list, float* __restrict__ o_part, float* __restrict__ l_part,
-                  void* __restrict__ out, float* __restrict__ lse, int G, int Hkv, int splits,
-                  int tps, int page_shift, int max_pages, int num_pages, float scale_log2) {
+                  int* __restrict__ meta, void* __restrict__ out, float* __restrict__ lse, int B,
+                  int G, int Hkv, int workers, int page_shift, int max_pages, int num_pages,
+                  float scale_log2) {
   using C = DecCfg<D, BITS>;
   using T1 = typename Elem<BF16>::T;
   using T2 = typename Elem<BF16>::T2;
-  constexpr int ROW = C::kRow, NG = C::kNG, S = C::kStages, STEP = C::kStep, W = C::kWarps;
-  constexpr int SL = STEP / 16;  // 16-token slabs per step
+  constexpr int ROW = C::kRow, NG = C::kNG, S = C::kStages, STEP = C::kStep;
+  constexpr int SL = STEP / 16;         // 16-token slabs per step
+  constexpr int R = HALF ? 1 : 2;       // token rows of a slab per lane
+  constexpr int KG = HALF ? 1 : NG;     // channel groups whose scores a lane sums itself
   extern __shared__ __align__(128) uint8_t smem[];
-  const int split = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int H = Hkv * G;
+  const int worker = blockIdx.x * C::kWarps + warp;
+  if (worker >= workers) return;
   const int page_size = 1 << page_shift;
-  const int len = table_len(kv_lens, b, page_size, max_pages,
-                            split == 0 && hkv == 0 && threadIdx.x == 0);
-  const int span = pages != nullptr ? n_list << page_shift : len;
-  const int t_begin = split * tps, t_end = min(span, t_begin + tps);
-  const size_t row0 = (size_t)b * H + hkv * G;  // first query head
-  if (t_begin >= t_end) {  // no token: an empty partial, or the whole answer
-    for (int i = threadIdx.x; i < G; i += 32 * W) {
-      if (splits > 1) l_part[(row0 + i) * splits + split] = -INFINITY;
-      else if (lse != nullptr) lse[row0 + i] = -INFINITY;
+  auto length = [&](int b, bool flag) {
+    return table_len(kv_lens, b, page_size, max_pages, flag);
+  };
+
+  // ------------------------------------------------------------ this warp's run
+  long long total = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int s = b0 + lane < B ? seq_steps(length(b0 + lane, worker == 0), n_list, page_shift) : 0;
+    total += __reduce_add_sync(0xffffffffu, (unsigned)s);
+  }
+  total *= Hkv;
+  const long long per = (total + workers - 1) / workers;
+  const long long u0 = worker * per;
+  const int n = (int)max(0ll, min(per, total - u0));  // steps
+  if (n == 0) return;
+  // its first (sequence, head, step)
+  int b = 0, hkv = 0, i = 0, nst = 1;
+  {
+    long long base = 0;  // steps of a head of the sequences before b0
+    for (int b0 = 0; b0 < B; b0 += 32) {
+      const int s = b0 + lane < B ? seq_steps(length(b0 + lane, false), n_list, page_shift) : 0;
+      int inc = s;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, x);
+        if (lane >= x) inc += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, (base + inc) * Hkv > u0);
+      if (hit != 0) {
+        const int src = __ffs(hit) - 1;
+        nst = __shfl_sync(0xffffffffu, s, src);
+        base += __shfl_sync(0xffffffffu, inc, src) - nst;
+        const long long rem = u0 - base * Hkv;
+        b = b0 + src;
+        hkv = (int)(rem / nst);
+        i = (int)(rem % nst);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (splits == 1)
-      for (int i = threadIdx.x; i < G * D; i += 32 * W)
-        static_cast<T1*>(out)[row0 * D + i] = Elem<BF16>::from(0.f);
-    return;
   }
 
   // ---------------------------------------------------------------- the ring
   const int np_shift = 6 - page_shift;  // log2 of the blocks per stage: 1, 2 or 4
   const uint32_t blk = (uint32_t)block_bytes(D, 1, BITS) << page_shift;
-  uint8_t* ring = smem + warp * S * C::kStage;
+  uint8_t* ring = smem + warp * C::kRing;
   const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(smem + C::kOffBar) + warp * S * 8;
   int* s_valid = reinterpret_cast<int*>(smem + C::kOffValid) + warp * S * 4;  // tokens per slab
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffAbort);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffAbort) + warp;
   if (lane < S) mbar_init(bar0 + 8 * lane, 1u);
-  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) *abort_flag = 0;
   fence_mbar_init();
-  __syncthreads();
-  const int steps = (t_end - t_begin + STEP - 1) / STEP;
-  const int n = (steps - warp + W - 1) / W;  // this warp's steps
-  const int32_t* list = pages == nullptr ? nullptr : pages + ((size_t)b * Hkv + hkv) * n_list;
-  const int32_t* table = block_table + (size_t)b * max_pages;
+  __syncwarp();
 
   // Page numbers are looked up 32 blocks at a time, one a lane, and one window
-  // ahead, so that the two dependent loads are off the loop's path.
-  auto lookup = [&](int k, int& page, int& valid) {  // this warp's block k
-    page = -1;
+  // ahead, so that the dependent loads are off the loop's path.  (cb, ch) is the
+  // (sequence, head) of the window's first step, cf its first step counted in
+  // this run, cn its number of steps.
+  int cb = b, ch = hkv, cf = -i, cn = nst;
+  auto lookup = [&](int k, int& row, int& valid) {  // this run's block k
+    row = 0;
     valid = 0;
-    const int i = k >> np_shift;
-    if (i >= n) return;
-    const int pos = t_begin + (warp + W * i) * STEP + ((k & ((1 << np_shift) - 1)) << page_shift);
-    if (pos >= t_end) return;
-    int lp = pos >> page_shift;
-    if (list != nullptr) lp = list[lp];
-    if (lp < 0 || lp >= max_pages) return;
-    valid = min(max(len - (lp << page_shift), 0), page_size);
-    if (valid == 0) return;
-    page = table[lp];
-    if (page < 0 || page >= num_pages) {
-      atomicOr(&g_error_flags, 2u);  // page number out of range: read page 0 instead
-      page = 0;
+    const int j = k >> np_shift;
+    int lb = cb, lh = ch, lf = cf, ln = cn;
+    if (j < n) {
+      while (j - lf >= ln) {  // it ends: j < n lies in some sequence
+        lf += ln;
+        if (++lh == Hkv) {
+          lh = 0;
+          do ln = seq_steps(length(++lb, false), n_list, page_shift);
+          while (ln == 0);
+        }
+      }
+      int lp = ((j - lf) << np_shift) + (k & ((1 << np_shift) - 1));
+      if (n_list > 0)
+        lp = lp < n_list ? pages[((size_t)lb * Hkv + lh) * n_list + lp] : -1;
+      if (lp >= 0 && lp < max_pages) {
+        valid = min(max(length(lb, false) - (lp << page_shift), 0), page_size);
+        if (valid > 0) {
+          int page = block_table[(size_t)lb * max_pages + lp];
+          if (page < 0 || page >= num_pages) {
+            atomicOr(&g_error_flags, 2u);  // page number out of range: read page 0 instead
+            page = 0;
+          }
+          row = page * Hkv + lh;
+        }
+      }
     }
+    __syncwarp();
+    // where the next window starts from (unused if the run ends before)
+    cb = __shfl_sync(0xffffffffu, lb, 31);
+    ch = __shfl_sync(0xffffffffu, lh, 31);
+    cf = __shfl_sync(0xffffffffu, lf, 31);
+    cn = __shfl_sync(0xffffffffu, ln, 31);
   };
-  int page0, valid0, page1, valid1;
-  lookup(lane, page0, valid0);
-  lookup(32 + lane, page1, valid1);
-  auto issue = [&](int i, int st) {  // copy step i's blocks into stage st
-    const int k = i << np_shift;
+  int row0, valid0, row1 = 0, valid1 = 0;
+  lookup(lane, row0, valid0);
+  if ((n << np_shift) > 32) lookup(32 + lane, row1, valid1);
+  unsigned full = 0;  // bit st: every token of stage st is valid
+  auto issue = [&](int j, int st) {  // copy step j's blocks into stage st
+    const int k = j << np_shift;
     if ((k & 31) == 0 && k > 0) {
-      page0 = page1;
+      row0 = row1;
       valid0 = valid1;
-      lookup(k + 32 + lane, page1, valid1);
+      if ((n << np_shift) > k + 32) lookup(k + 32 + lane, row1, valid1);
     }
-    const int page = __shfl_sync(0xffffffffu, page0, (k + lane) & 31);
+    const int row = __shfl_sync(0xffffffffu, row0, (k + lane) & 31);
     const int valid = __shfl_sync(0xffffffffu, valid0, (k + lane) & 31);
-    // slab `lane` (< 4) lies in block lane / (page / 16)
-    const int slab = __shfl_sync(0xffffffffu, valid0, (k + (lane >> (page_shift - 4))) & 31) -
-                     16 * (lane & ((1 << (page_shift - 4)) - 1));
-    const bool copy = lane < (1 << np_shift) && valid > 0;
+    const bool mine = lane < (1 << np_shift);
+    const bool copy = mine && valid > 0;
     const int some = __popc(__ballot_sync(0xffffffffu, copy));
-    if (lane < 4) s_valid[4 * st + lane] = min(max(slab, 0), 16);
+    if (__all_sync(0xffffffffu, !mine || valid == page_size)) {
+      full |= 1u << st;
+    } else {
+      full &= ~(1u << st);
+      // slab `lane` (< 4) lies in block lane / (page / 16)
+      const int slab = __shfl_sync(0xffffffffu, valid0, (k + (lane >> (page_shift - 4))) & 31) -
+                       16 * (lane & ((1 << (page_shift - 4)) - 1));
+      if (lane < 4) s_valid[4 * st + lane] = min(max(slab, 0), 16);
+    }
     const uint32_t bar = bar0 + 8 * st;
     if (lane == 0) mbar_arrive_expect_tx(bar, some * blk);
     __syncwarp();
     if (copy)
-      bulk_load(ring0 + st * C::kStage + lane * blk, data + ((size_t)page * Hkv + hkv) * blk, blk,
-                bar);
+      bulk_load(ring0 + st * C::kStage + lane * blk, data + (size_t)(uint32_t)row * blk, blk, bar);
   };
-  for (int i = 0; i < min(n, S); ++i) issue(i, i);
+  for (int j = 0; j < min(n, S); ++j) issue(j, j);
 
   // ------------------------------------------------------------------ queries
-  // B fragments of S: lane (g, t) holds head g's channels 64*grp + 16 t + 0..15
-  // in the order in which a K row's codes unpack, over 16 where those are 16 c.
+  // B fragments of S: lane (g, t) holds its head's channels 64*grp + 16 t +
+  // 0..15 in the order in which a K row's codes unpack, over 16 where those are
+  // 16 c.  Column g is head g; in HALF, head g & 3 with the contraction's half
+  // g >> 2 (group g >> 2, or the g >> 2'th 8 of the 16 channels).
+  const int half = t >> 1;                      // HALF: this lane's token row and half of S
+  const int head0 = HALF ? 2 * (t & 1) : 2 * t;  // its heads: head0, head0 + 1
   uint32_t qb[NG * 4][2];
-  float qsum[NG][2], sl2[2];  // of heads 2t, 2t+1
-  {
-    const T1* qp = static_cast<const T1*>(q) + b * q_b + (long long)(hkv * G + g) * q_h + 16 * t;
+  float qsum[KG][2], sl2[2];
+  auto load_q = [&]() {
+    const int hq = HALF ? g & 3 : g;
+    const T1* qp = static_cast<const T1*>(q) + b * q_b + (long long)(hkv * G + hq) * q_h + 16 * t;
     float f[NG][16], top = 0.f;
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
       uint32_t u[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-      if (g < G) {
+      if (hq < G) {
         *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(qp + gr * 64);
         *reinterpret_cast<uint4*>(u + 4) = *reinterpret_cast<const uint4*>(qp + gr * 64 + 8);
       }
@@ -383,19 +452,16 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int shift = 139 - (int)(__float_as_uint(top) >> 23);  // to [2^12, 2^13)
     const float mul = pow2i(shift);
+    float sum[NG][2];
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
-      float sum = 0.f;
+      sum[gr][0] = sum[gr][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         f[gr][j] *= mul;
-        sum += f[gr][j];
+        if (HALF && (NG == 2 ? gr : j / 8) != (g >> 2)) f[gr][j] = 0.f;
+        sum[gr][0] += f[gr][j];
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= pow2i(-24);  // the codes' factor
-      qsum[gr][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-      qsum[gr][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (BITS == 4) {
@@ -409,28 +475,44 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
         }
       }
     }
-    const int e = 24 - min(max(shift, -126), 127);
-    const float s2 = scale_log2 * pow2i(e);  // what a score in these units is in log2
-    sl2[0] = __shfl_sync(0xffffffffu, s2, 8 * t);
+    // sums of the codes' factors over each column's channels
+#pragma unroll
+    for (int gr = 0; gr < KG; ++gr) {
+      float x = sum[gr][0];
+      if constexpr (HALF && NG == 2) x += sum[1][0];  // the other group's are zeros
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      x *= pow2i(-24);
+      qsum[gr][0] = __shfl_sync(0xffffffffu, x, 8 * t);  // columns 2t, 2t + 1
+      qsum[gr][1] = __shfl_sync(0xffffffffu, x, 8 * t + 4);
+    }
+    const float s2 = scale_log2 * pow2i(24 - min(max(shift, -126), 127));
+    sl2[0] = __shfl_sync(0xffffffffu, s2, 8 * t);  // what a score in these units is in log2
     sl2[1] = __shfl_sync(0xffffffffu, s2, 8 * t + 4);
-  }
+  };
 
-  // --------------------------------------------------------------------- loop
-  float o[NG][4][4];  // [group][tile][(d even, head 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
+  // --------------------------------------------------------------------- state
+  float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
   float omin[NG][2];  // sum of p * vmin over this lane's tokens
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2], l[2];
   // value scales are multiplied by vmul = 2^(127 - vexp), vexp the biased
   // exponent of the largest so far
-  int vexp = 1;
-  float vmul = pow2i(126);
+  int vexp;
+  float vmul;
+  auto reset = [&]() {
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+    vexp = 1;
+    vmul = pow2i(126);
 #pragma unroll
-  for (int gr = 0; gr < NG; ++gr) {
-    omin[gr][0] = omin[gr][1] = 0.f;
+    for (int gr = 0; gr < NG; ++gr) {
+      omin[gr][0] = omin[gr][1] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[gr][i][e] = 0.f;
-  }
+        for (int e = 0; e < 4; ++e) o[gr][k][e] = 0.f;
+    }
+  };
   // Slab s of a stage: codes at (s >> 1) * code_hi + (s & 1) * code_lo, params
   // likewise; 16-token pages put each slab in a block of its own.
   const uint32_t code_lo = page_shift == 4 ? blk : 16 * ROW;
@@ -439,42 +521,50 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
   const uint32_t par_hi = page_shift == 6 ? 32 * NG * 4 : page_shift == 5 ? blk : 2 * blk;
   const uint32_t v_off = ROW << page_shift, vp_off = (NG * 4) << page_shift;
   const int tok = (g >> 1) + (g & 1) * 4;  // S row g is token `tok` of the slab, row g+8 8 later
+  const int vtok = HALF ? tok + 8 * half : tok;  // the first token whose p this lane holds
 
   // One step; nv: tokens of each slab.  FULL: all of them, known by the caller,
   // which leaves one run of straight code whose slabs overlap.
-  auto step = [&](auto full, const uint8_t* stage, const int (&nv)[4]) {
-    constexpr bool FULL = decltype(full)::value;
+  auto step = [&](auto all, const uint8_t* stage, const int (&nv)[4]) {
+    constexpr bool FULL = decltype(all)::value;
 
     // ---- S = K q^T
-    float s[SL][4];
-    uint32_t vpar[SL][2][NG];  // (scale, min) of V of rows g, g+8
+    float s[SL][R][2];
+    uint32_t vpar[SL][R][NG];  // (scale, min) of V of this lane's rows
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
       if (!FULL && nv[sl] == 0) {  // the same in every lane
-        s[sl][0] = s[sl][1] = s[sl][2] = s[sl][3] = -INFINITY;
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) vpar[sl][0][gr] = vpar[sl][1][gr] = 0u;
+        for (int r = 0; r < R; ++r) {
+          s[sl][r][0] = s[sl][r][1] = -INFINITY;
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) vpar[sl][r][gr] = 0u;
+        }
         continue;
       }
       const uint8_t* kc = stage + (sl >> 1) * code_hi + (sl & 1) * code_lo + tok * ROW;
-      const uint8_t* kp =
-          stage + 2 * v_off + (sl >> 1) * par_hi + (sl & 1) * par_lo + tok * NG * 4;
-      uint32_t kpar[2][NG];
+      const uint8_t* pp = stage + 2 * v_off + (sl >> 1) * par_hi + (sl & 1) * par_lo;
+      uint32_t kpar[2][KG];  // of rows g, g+8
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        if constexpr (NG == 2) {
-          *reinterpret_cast<uint2*>(kpar[r]) = *reinterpret_cast<const uint2*>(kp + r * 8 * NG * 4);
-          *reinterpret_cast<uint2*>(vpar[sl][r]) =
-              *reinterpret_cast<const uint2*>(kp + vp_off + r * 8 * NG * 4);
-        } else {
-          kpar[r][0] = *reinterpret_cast<const uint32_t*>(kp + r * 8 * NG * 4);
-          vpar[sl][r][0] = *reinterpret_cast<const uint32_t*>(kp + vp_off + r * 8 * NG * 4);
-        }
+        const uint8_t* kp = pp + (tok + 8 * r) * NG * 4;
+        if constexpr (KG == 2)
+          *reinterpret_cast<uint2*>(kpar[r]) = *reinterpret_cast<const uint2*>(kp);
+        else
+          kpar[r][0] = *reinterpret_cast<const uint32_t*>(kp + (HALF && NG == 2 ? 4 * half : 0));
       }
-      s[sl][0] = s[sl][1] = s[sl][2] = s[sl][3] = 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint8_t* vp = pp + vp_off + (vtok + 8 * r) * NG * 4;
+        if constexpr (NG == 2)
+          *reinterpret_cast<uint2*>(vpar[sl][r]) = *reinterpret_cast<const uint2*>(vp);
+        else
+          vpar[sl][r][0] = *reinterpret_cast<const uint32_t*>(vp);
+      }
+      float part[2][2];  // rows g, g+8
+      float acc[4];
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        float acc[4];
         if constexpr (BITS == 4) {
           const uint2 x = *reinterpret_cast<const uint2*>(kc + gr * 32 + t * 8);
           const uint2 y = *reinterpret_cast<const uint2*>(kc + 8 * ROW + gr * 32 + t * 8);
@@ -483,8 +573,10 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
             uint32_t a[4], z[4];
             unpack4(w ? x.y : x.x, a);
             unpack4(w ? y.y : y.x, z);
-            if (w == 0) mma16816_first(acc, a[0], z[0], a[1], z[1], qb[gr * 4][0], qb[gr * 4][1]);
-            else mma16816(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2][0], qb[gr * 4 + 2][1]);
+            if (w == 0 && (gr == 0 || !HALF))
+              mma16816_first(acc, a[0], z[0], a[1], z[1], qb[gr * 4][0], qb[gr * 4][1]);
+            else
+              mma16816(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2 * w][0], qb[gr * 4 + 2 * w][1]);
             mma16816(acc, a[2], z[2], a[3], z[3], qb[gr * 4 + 2 * w + 1][0],
                      qb[gr * 4 + 2 * w + 1][1]);
           }
@@ -496,41 +588,58 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
           for (int w = 0; w < 4; ++w) {
             const uint32_t a0 = __byte_perm(xs[w], 0, 0x4140), a1 = __byte_perm(ys[w], 0, 0x4140);
             const uint32_t a2 = __byte_perm(xs[w], 0, 0x4342), a3 = __byte_perm(ys[w], 0, 0x4342);
-            if (w == 0) mma16816_first(acc, a0, a1, a2, a3, qb[gr * 4][0], qb[gr * 4][1]);
-            else mma16816(acc, a0, a1, a2, a3, qb[gr * 4 + w][0], qb[gr * 4 + w][1]);
+            if (w == 0 && (gr == 0 || !HALF))
+              mma16816_first(acc, a0, a1, a2, a3, qb[gr * 4][0], qb[gr * 4][1]);
+            else
+              mma16816(acc, a0, a1, a2, a3, qb[gr * 4 + w][0], qb[gr * 4 + w][1]);
           }
         }
+        if (!HALF || gr == NG - 1) {
+          constexpr int last = KG - 1;
+          const int kg = HALF ? 0 : min(gr, last);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float2 pr = param<BF16>(kpar[r][gr]);
+          for (int r = 0; r < 2; ++r) {
+            const float2 pr = param<BF16>(kpar[r][kg]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            s[sl][2 * r + h] =
-                fmaf(pr.x, acc[2 * r + h], fmaf(pr.y, qsum[gr][h], s[sl][2 * r + h]));
+            for (int h = 0; h < 2; ++h) {
+              const float bias = pr.y * qsum[kg][h];
+              part[r][h] = fmaf(pr.x, acc[2 * r + h], HALF || gr == 0 ? bias : part[r][h] + bias);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (HALF) {  // the other half of this lane's row, for this half of the other
+          const float got = __shfl_xor_sync(0xffffffffu, half ? part[0][h] : part[1][h], 2);
+          s[sl][0][h] = (half ? part[1][h] : part[0][h]) + got;
+        } else {
+          s[sl][0][h] = part[0][h];
+          s[sl][R - 1][h] = part[1][h];
         }
       }
       // tokens past the end: whatever their slots hold is dropped here
       if (!FULL && nv[sl] < 16) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (tok + 8 * r >= nv[sl]) {
-            s[sl][2 * r] = s[sl][2 * r + 1] = -INFINITY;
+        for (int r = 0; r < R; ++r)
+          if (vtok + 8 * r >= nv[sl]) {
+            s[sl][r][0] = s[sl][r][1] = -INFINITY;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) vpar[sl][r][gr] = 0u;
           }
       }
     }
 
-    // ---- online softmax, per head over the step's tokens (rows: lanes of one t)
+    // ---- online softmax, per head over the step's tokens
     float alpha[2];
     bool moved = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float mx = fmaxf(s[0][h], s[0][h + 2]);
+      float mx = s[0][0][h];
 #pragma unroll
-      for (int sl = 1; sl < SL; ++sl) mx = fmax3(mx, s[sl][h], s[sl][h + 2]);
+      for (int k = 1; k < SL * R; ++k) mx = fmaxf(mx, s[k / R][k % R][h]);
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      for (int x = HALF ? 2 : 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       const float mn = fmaxf(m[h], mx * sl2[h]);
       const float mu = mn == -INFINITY ? 0.f : mn;
       alpha[h] = ex2_mufu(m[h] - mu);
@@ -538,22 +647,17 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
       m[h] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int sl = 0; sl < SL; ++sl)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float p = ex2_mufu(fmaf(s[sl][2 * r + h], sl2[h], -mu));
-          s[sl][2 * r + h] = p;
-          sum += p;
-        }
+      for (int k = 0; k < SL * R; ++k) {
+        const float p = ex2_mufu(fmaf(s[k / R][k % R][h], sl2[h], -mu));
+        s[k / R][k % R][h] = p;
+        sum += p;
+      }
       l[h] = l[h] * alpha[h] + sum;
     }
     T2 big = *reinterpret_cast<T2*>(&vpar[0][0][0]);  // largest value scale, in .x
 #pragma unroll
-    for (int sl = 0; sl < SL; ++sl)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) big = __hmax2(big, *reinterpret_cast<T2*>(&vpar[sl][r][gr]));
+    for (int k = 1; k < SL * R * NG; ++k)
+      big = __hmax2(big, *reinterpret_cast<T2*>(&vpar[k / (R * NG)][k / NG % R][k % NG]));
     const float vbig = Elem<BF16>::unpack(big).x;
     float f = 1.f;
     if (__any_sync(0xffffffffu, vbig * vmul >= 2.f)) {
@@ -586,12 +690,16 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
       for (int gr = 0; gr < NG; ++gr) {
         uint32_t pb[2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < R; ++r) {
           const float2 pr = param<BF16>(vpar[sl][r][gr]);
           const float w = pr.x * vmul;
-          omin[gr][0] = fmaf(s[sl][2 * r], pr.y, omin[gr][0]);
-          omin[gr][1] = fmaf(s[sl][2 * r + 1], pr.y, omin[gr][1]);
-          pb[r] = movmatrix_trans(pack2_u32<false>(s[sl][2 * r] * w, s[sl][2 * r + 1] * w));
+          omin[gr][0] = fmaf(s[sl][r][0], pr.y, omin[gr][0]);
+          omin[gr][1] = fmaf(s[sl][r][1], pr.y, omin[gr][1]);
+          pb[r] = movmatrix_trans(pack2_u32<false>(s[sl][r][0] * w, s[sl][r][1] * w));
+        }
+        if constexpr (HALF) {  // columns 0-3: tokens 0-7 of the slab, columns 4-7: tokens 8-15
+          pb[1] = g >= 4 ? pb[0] : 0u;
+          pb[0] = g >= 4 ? 0u : pb[0];
         }
         if constexpr (BITS == 4) {
           const uint32_t wa = *reinterpret_cast<const uint32_t*>(vc + gr * 32);
@@ -623,27 +731,99 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
         }
       }
     }
-
   };
 
+  // Write out what was gathered for (b, hkv): the answer where this warp had all
+  // of it, else a partial (o normalised, natural log l).
+  auto flush = [&](bool first, bool last) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int x = HALF ? 2 : 4; x < 32; x <<= 1) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+          omin[gr][h] += __shfl_xor_sync(0xffffffffu, omin[gr][h], x);
+      }
+    }
+    const float vscale = pow2i(vexp - 127);
+    constexpr float kEven = 16777216.f;  // 2^24: the codes' factor
+    constexpr float kOdd = BITS == 4 ? 1048576.f : kEven;  // odd channels were 16 c
+    const bool whole = first && last;
+    const int tile = b * Hkv + hkv;
+    const size_t seg = (size_t)worker + tile;  // either grows along the list: no two alike
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int head = head0 + h;
+      const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+      const float ll = l[h] == 0.f ? -INFINITY : m[h] * kLn2 + logf(l[h]);
+      const size_t orow = whole ? (size_t)b * Hkv * G + hkv * G + head : seg * G + head;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float x = o[gr][k][h], y = o[gr][k][2 + h];
+          if constexpr (HALF) {  // the other tokens' half
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            y += __shfl_xor_sync(0xffffffffu, y, 2);
+          }
+          x = fmaf(x * kEven, vscale, omin[gr][h]) * inv;
+          y = fmaf(y * kOdd, vscale, omin[gr][h]) * inv;
+          const size_t at = orow * D + gr * 64 + 8 * g + 2 * k;
+          if (head < G && (!HALF || (k >> 1) == half)) {
+            if (whole) *reinterpret_cast<uint32_t*>(static_cast<T1*>(out) + at) = pack2_u32<BF16>(x, y);
+            else *reinterpret_cast<float2*>(o_part + at) = make_float2(x, y);
+          }
+        }
+      if (g == 0 && head < G && (!HALF || half == 0)) {
+        if (!whole) l_part[orow] = ll;
+        else if (lse != nullptr) lse[orow] = ll;
+      }
+    }
+    if (lane == 0) {  // which workers hold partials of this (sequence, KV head)
+      if (first) meta[2 * tile] = whole ? -1 : worker;
+      if (last) meta[2 * tile + 1] = worker;
+    }
+  };
+
+  // ---------------------------------------------------------------------- loop
+  load_q();
+  reset();
+  int i0 = i;  // the step at which this warp entered (b, hkv)
   bool ok = true;
   int st = 0;
   uint32_t phase = 0;
-  for (int i = 0; i < n; ++i) {
-    if (!mbar_wait(bar0 + 8 * st, phase, abort_flag)) {
-      ok = false;
-      break;
+  for (int j = 0; j < n; ++j) {
+    ok = ok && mbar_wait(bar0 + 8 * st, phase, abort_flag);
+    if (ok) {
+      const uint8_t* stage = ring + st * C::kStage;
+      if (full >> st & 1u) {
+        const int nv[4] = {16, 16, 16, 16};
+        step(std::true_type{}, stage, nv);
+      } else {
+        const int4 v = *reinterpret_cast<const int4*>(s_valid + 4 * st);
+        const int nv[4] = {v.x, v.y, v.z, v.w};
+        step(std::false_type{}, stage, nv);
+      }
+      __syncwarp();  // every lane has read the stage
+      if (j + S < n) issue(j + S, st);
+      if (++st == S) {
+        st = 0;
+        phase ^= 1u;
+      }
     }
-    const uint8_t* stage = ring + st * C::kStage;
-    const int4 nv4 = *reinterpret_cast<const int4*>(s_valid + 4 * st);
-    const int nv[4] = {nv4.x, nv4.y, nv4.z, nv4.w};
-    if (nv4.x + nv4.y + nv4.z + nv4.w == STEP) step(std::true_type{}, stage, nv);
-    else step(std::false_type{}, stage, nv);
-    __syncwarp();  // every lane has read the stage
-    if (i + S < n) issue(i + S, st);
-    if (++st == S) {
-      st = 0;
-      phase ^= 1u;
+    if (++i == nst || j == n - 1) {
+      flush(i0 == 0, i == nst);
+      if (j < n - 1) {  // the next (sequence, KV head) with a step
+        i = i0 = 0;
+        if (++hkv == Hkv) {
+          hkv = 0;
+          do nst = seq_steps(length(++b, false), n_list, page_shift);
+          while (nst == 0);
+        }
+        load_q();
+        reset();
+      }
     }
   }
   if (!ok) {
@@ -655,87 +835,40 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
       mbar_wait_limit(bar0 + 8 * k, 1, &never, kDrainNs);
     }
   }
-
-  // ---------------------------------------------------------------- merge warps
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr) omin[gr][h] += __shfl_xor_sync(0xffffffffu, omin[gr][h], x);
-    }
-    if (!ok) l[h] = 0.f;
-  }
-  const float vscale = pow2i(vexp - 127);
-  constexpr float kEven = 16777216.f;  // 2^24: the codes' factor
-  constexpr float kOdd = BITS == 4 ? 1048576.f : kEven;  // odd channels were 16 c
-  __syncthreads();  // the rings are drained: their memory holds the merge now
-  constexpr int P = C::kPad;
-  float* mo = reinterpret_cast<float*>(smem);  // [W][8][P]
-  float* mm = mo + W * 8 * P;                  // [W][8] m, [W][8] l
-  float* ml = mm + W * 8;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float* dst = mo + (warp * 8 + 2 * t + h) * P + 8 * g;
-#pragma unroll
-    for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<float2*>(dst + gr * 64 + 2 * k) =
-            make_float2(fmaf(o[gr][k][h] * kEven, vscale, omin[gr][h]),
-                        fmaf(o[gr][k][2 + h] * kOdd, vscale, omin[gr][h]));
-    if (g == 0) {
-      mm[warp * 8 + 2 * t + h] = m[h];
-      ml[warp * 8 + 2 * t + h] = l[h];
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < G * D; i += 32 * W) {
-    const int h = i / D, d = i % D;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, mm[w * 8 + h]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float lw = ml[w * 8 + h];
-      if (lw == 0.f) continue;  // no token
-      const float x = ex2_mufu(mm[w * 8 + h] - M);
-      L += lw * x;
-      acc += mo[(w * 8 + h) * P + d] * x;
-    }
-    const float val = L == 0.f ? 0.f : acc / L;
-    const float ll = L == 0.f ? -INFINITY : M * kLn2 + logf(L);
-    const size_t row = row0 + h;
-    if (splits > 1) {
-      o_part[(row * splits + split) * D + d] = val;
-      if (d == 0) l_part[row * splits + split] = ll;
-    } else {
-      static_cast<T1*>(out)[row * D + d] = Elem<BF16>::from(val);
-      if (d == 0 && lse != nullptr) lse[row] = ll;
-    }
-  }
 }
 
-// One CTA of 4 warps per (sequence, query head).  A split whose l is -inf has
-// no token and its o is not read; a NaN goes through to O and L.  The splits'
-// weights are made first, one a thread; then each row of a split is read as
-// 16 bytes a lane, with eight rows in flight a warp, so that a load's latency
-// is paid a few times and not once per split.
+// One CTA of 4 warps per (sequence, query head), for those whose KV head was
+// cut; it also writes the answer of empty sequences.  A partial whose l is -inf
+// has no token; a NaN goes through to O and L.  The partials' weights are made
+// first, one a thread; then each row is read as 16 bytes a lane, with eight
+// rows in flight a warp, so that a load's latency is paid a few times and not
+// once per partial.
 constexpr int kChunk = 512;  // weights held at a time
 template <int D, bool BF16>
 __global__ void __launch_bounds__(128)
     combine_kernel(const float* __restrict__ o_part, const float* __restrict__ l_part,
-                   void* __restrict__ out, float* __restrict__ lse, int S) {
+                   const int* __restrict__ meta, const int32_t* __restrict__ kv_lens,
+                   void* __restrict__ out, float* __restrict__ lse, int G, int Hkv) {
+  using T1 = typename Elem<BF16>::T;
   constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
   __shared__ float s_w[kChunk], s_red[2][4];
   __shared__ float4 s_acc[4 * RPW][LPR];
   const size_t row = blockIdx.x;
+  const int tile = blockIdx.x / G, h = blockIdx.x % G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float* lp = l_part + row * S;
-  const float4* op = reinterpret_cast<const float4*>(o_part + row * S * D);
+  if (kv_lens[tile / Hkv] <= 0) {
+    if (threadIdx.x < D) static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(0.f);
+    if (threadIdx.x == 0 && lse != nullptr) lse[row] = -INFINITY;
+    return;
+  }
+  const int first = meta[2 * tile];
+  if (first < 0) return;  // one warp had all of it
+  const int S = meta[2 * tile + 1] - first + 1;
+  const size_t seg0 = (size_t)first + tile;
+  const float* lp = l_part + seg0 * G + h;  // partial s at s * G
+  const float4* op = reinterpret_cast<const float4*>(o_part + (seg0 * G + h) * D);
   float M = -INFINITY;
-  for (int s = threadIdx.x; s < S; s += 128) M = fmaxf(M, lp[s]);
+  for (int s = threadIdx.x; s < S; s += 128) M = fmaxf(M, lp[(size_t)s * G]);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
   if (lane == 0) s_red[0][warp] = M;
@@ -748,7 +881,7 @@ __global__ void __launch_bounds__(128)
     const int cn = min(kChunk, S - c0);
     __syncthreads();
     for (int s = threadIdx.x; s < cn; s += 128) {
-      const float v = lp[c0 + s];
+      const float v = lp[(size_t)(c0 + s) * G];
       const float w = v == -INFINITY ? 0.f : expf(v - M);
       s_w[s] = w;
       L += w;
@@ -761,8 +894,7 @@ __global__ void __launch_bounds__(128)
       for (int k = 0; k < 8; ++k) {
         const int s = s0 + k * 4 * RPW;
         w[k] = s < cn ? s_w[s] : 0.f;
-        // a weight of zero may stand for a row that was not written
-        v[k] = w[k] != 0.f ? op[(size_t)(c0 + s) * LPR + c] : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[k] = s < cn ? op[(size_t)(c0 + s) * G * LPR + c] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -784,8 +916,7 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
     for (int k = 0; k < 4 * RPW; ++k)
       a += reinterpret_cast<const float*>(s_acc[k])[threadIdx.x];
-    static_cast<typename Elem<BF16>::T*>(out)[row * D + threadIdx.x] =
-        Elem<BF16>::from(L == 0.f ? 0.f : a / L);
+    static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(L == 0.f ? 0.f : a / L);
   }
   if (threadIdx.x == 0 && lse != nullptr) lse[row] = L == 0.f ? -INFINITY : M + logf(L);
 }
@@ -817,70 +948,79 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
   return B2A_OK;
 }
 
-int kvq_decode_splits(int B, int Hkv, long long max_tokens) {
-  const long long want = 148 * 4;
-  long long s = (want + (long long)B * Hkv - 1) / ((long long)B * Hkv);
-  const long long most = (max_tokens + 255) / 256;
-  s = s < most ? s : most;
-  const long long least = (max_tokens + 4095) / 4096;
-  s = s > least ? s : least;
-  return (int)(s < 1 ? 1 : s > 65535 ? 65535 : s);
+// Warps that the GPU runs at a time; no more than there can be steps.
+int kvq_decode_workers(int B, int Hkv, int D, int bits, long long max_tokens) {
+  const long long resident = 148ll * 3 * (D == 128 && bits == 8 ? 2 : 4);
+  const long long steps = (long long)B * Hkv * ((max_tokens + 63) / 64);
+  return (int)(steps < resident ? steps : resident);
 }
 
-template <int D, int BITS, bool BF16>
+// Partials: a worker's share of a (sequence, KV head) has number worker + tile.
+// [worker + tile][G][D] o, [worker + tile][G] l, [tile][2] first and last worker.
+int64_t kvq_decode_workspace_floats(int B, int H, int Hkv, int D, int workers) {
+  const int64_t tiles = (int64_t)B * Hkv;
+  return (workers + tiles) * (H / Hkv) * (D + 1) + 2 * tiles;
+}
+
+template <int D, int BITS, bool BF16, bool HALF>
 static int launch_kvq_decode(const void* q, int64_t q_b, int64_t q_h, const uint8_t* data,
                              const int32_t* block_table, const int32_t* kv_lens,
-                             const int32_t* pages, int n_list, float* o_part, float* l_part,
-                             void* o, float* lse, int B, int G, int Hkv, int splits, int tps,
-                             int page_shift, int max_pages, int num_pages, float scale,
-                             cudaStream_t stream) {
+                             const int32_t* pages, int n_list, float* ws, void* o, float* lse,
+                             int B, int G, int Hkv, int workers, int page_shift, int max_pages,
+                             int num_pages, float scale, cudaStream_t stream) {
   using namespace kvq;
-  auto kern = decode_kernel<D, BITS, BF16>;
-  constexpr int smem = DecCfg<D, BITS>::kSmem;
+  using C = DecCfg<D, BITS>;
+  auto kern = decode_kernel<D, BITS, BF16, HALF>;
   static bool attr_done[kMaxDevices] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
     return set_error(B2A_ERR_CUDA, "cudaGetDevice failed");
   if (!attr_done[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(quantised decode)");
     attr_done[dev] = true;
   }
-  kern<<<dim3((unsigned)splits, (unsigned)Hkv, (unsigned)B), 32 * DecCfg<D, BITS>::kWarps, smem,
-         stream>>>(
-      q, q_b, q_h, data, block_table, kv_lens, pages, n_list, o_part, l_part, o, lse, G, Hkv,
-      splits, tps, page_shift, max_pages, num_pages, scale * kLog2e);
+  const int64_t segs = (int64_t)workers + (int64_t)B * Hkv;
+  float* l_part = ws + segs * G * D;
+  int* meta = reinterpret_cast<int*>(l_part + segs * G);
+  kern<<<(workers + C::kWarps - 1) / C::kWarps, 32 * C::kWarps, C::kSmem, stream>>>(
+      q, q_b, q_h, data, block_table, kv_lens, pages, n_list, ws, l_part, meta, o, lse, B, G, Hkv,
+      workers, page_shift, max_pages, num_pages, scale * kLog2e);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "quantised decode kernel launch");
-  if (splits > 1) {
-    combine_kernel<D, BF16><<<B * G * Hkv, 128, 0, stream>>>(o_part, l_part, o, lse, splits);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return set_cuda_error(e, "quantised decode combine launch");
-  }
+  combine_kernel<D, BF16><<<B * G * Hkv, 128, 0, stream>>>(ws, l_part, meta, kv_lens, o, lse, G,
+                                                          Hkv);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error(e, "quantised decode combine launch");
   return B2A_OK;
 }
 
 int kvq_decode_dispatch(const void* q, int64_t q_b, int64_t q_h, const void* data,
                         const int32_t* block_table, const int32_t* kv_lens, const int32_t* pages,
-                        int n_list, float* o_part, float* l_part, void* o, float* lse, int B,
-                        int H, int Hkv, int D, int page_size, int max_pages, int num_pages,
-                        int splits, int bits, int dtype, float scale, cudaStream_t stream) {
-  const long long span = (long long)(pages != nullptr ? n_list : max_pages) * page_size;
-  // whole pages and whole 64-token pieces, so that no step straddles a split
-  const int tps = (int)(((span + splits - 1) / splits + 63) / 64 * 64);
+                        int n_list, float* workspace, void* o, float* lse, int B, int H, int Hkv,
+                        int D, int page_size, int max_pages, int num_pages, int workers, int bits,
+                        int dtype, float scale, cudaStream_t stream) {
   const int shift = page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
+  const int G = H / Hkv;
   auto go = [&](auto fn) {
-    return fn(q, q_b, q_h, static_cast<const uint8_t*>(data), block_table, kv_lens, pages, n_list,
-              o_part, l_part, o, lse, B, H / Hkv, Hkv, splits, tps, shift, max_pages, num_pages,
-              scale, stream);
+    return fn(q, q_b, q_h, static_cast<const uint8_t*>(data), block_table, kv_lens, pages,
+              pages != nullptr ? n_list : 0, workspace, o, lse, B, G, Hkv, workers, shift,
+              max_pages, num_pages, scale, stream);
   };
   const bool bf = dtype == B2A_BF16;
-  if (D == 64 && bits == 4)
-    return bf ? go(launch_kvq_decode<64, 4, true>) : go(launch_kvq_decode<64, 4, false>);
-  if (D == 64) return bf ? go(launch_kvq_decode<64, 8, true>) : go(launch_kvq_decode<64, 8, false>);
-  if (bits == 4)
-    return bf ? go(launch_kvq_decode<128, 4, true>) : go(launch_kvq_decode<128, 4, false>);
-  return bf ? go(launch_kvq_decode<128, 8, true>) : go(launch_kvq_decode<128, 8, false>);
+#define B2A_KVQ(DD, BB)                                                                      \
+  if (D == DD && bits == BB)                                                                 \
+    return G <= 4 ? (bf ? go(launch_kvq_decode<DD, BB, true, true>)                          \
+                        : go(launch_kvq_decode<DD, BB, false, true>))                        \
+                  : (bf ? go(launch_kvq_decode<DD, BB, true, false>)                         \
+                        : go(launch_kvq_decode<DD, BB, false, false>));
+  B2A_KVQ(64, 4)
+  B2A_KVQ(64, 8)
+  B2A_KVQ(128, 4)
+  B2A_KVQ(128, 8)
+#undef B2A_KVQ
+  return set_error(B2A_ERR_UNSUPPORTED, "quantised decode: unsupported (D, bits)");
 }
 
 }  // namespace b2a

@@ -330,26 +330,28 @@ int b2a_kvq_select_pages(const void* q, const int64_t* q_strides,
                          int top_k, int dtype, void* stream);
 
 /*
- * Decode attention (query length 1) over the quantised cache, split over the
- * tokens: O [B,H,D] (dtype) and lse [B,H] (may be NULL) as b2a_decode_paged.
- * kv_lens[b] may be 0 (O = 0, lse = -inf).  pages == NULL attends to the whole
- * cache; else to the n_pages logical pages that pages [B, Hkv, n_pages] lists
- * for each KV head (entries that are negative or lie behind the sequence's end
- * are skipped; a page listed twice counts twice).  splits > 1 needs the fp32
- * scratch o_part [B,H,splits,D] and l_part [B,H,splits];
- * b2a_kvq_decode_splits gives the number that suits B, Hkv and the most tokens
- * one sequence attends to.  A bad block-table entry sets bit 1 of the device
- * error word and reads page 0 instead.  H/Hkv <= 8.
+ * Decode attention (query length 1) over the quantised cache: O [B,H,D]
+ * (dtype) and lse [B,H] (may be NULL) as b2a_decode_paged.  kv_lens[b] may be 0
+ * (O = 0, lse = -inf).  pages == NULL attends to the whole cache; else to the
+ * n_pages logical pages that pages [B, Hkv, n_pages] lists for each KV head
+ * (entries that are negative or lie behind the sequence's end are skipped; a
+ * page listed twice counts twice).  The tokens of all sequences are divided
+ * evenly among `workers` warps whatever the lengths; b2a_kvq_decode_workers
+ * gives the number that fills the GPU, max_tokens being the most that one
+ * sequence can attend to, and b2a_kvq_decode_workspace_floats the scratch that
+ * a call needs.  A bad block-table entry sets bit 1 of the device error word
+ * and reads page 0 instead.  H/Hkv <= 8.
  */
-int b2a_kvq_decode_splits(int B, int Hkv, int64_t max_tokens);
+int b2a_kvq_decode_workers(int B, int Hkv, int D, int bits, int64_t max_tokens);
+int64_t b2a_kvq_decode_workspace_floats(int B, int H, int Hkv, int D,
+                                        int workers);
 int b2a_kvq_decode_paged(const void* q, const int64_t* q_strides,
                          const void* data, const int32_t* block_table,
                          const int32_t* kv_lens, const int32_t* pages,
-                         int n_pages, float* o_part, float* l_part, void* o,
-                         float* lse, int B, int H, int Hkv, int D,
-                         int page_size, int max_pages, int num_pages,
-                         int splits, int bits, int dtype, float scale,
-                         void* stream);
+                         int n_pages, float* workspace, void* o, float* lse,
+                         int B, int H, int Hkv, int D, int page_size,
+                         int max_pages, int num_pages, int workers, int bits,
+                         int dtype, float scale, void* stream);
 
 /*
  * Device error word written by the kernels (bit 0: a bounded pipeline wait
