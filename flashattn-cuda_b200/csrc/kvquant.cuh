@@ -24,6 +24,32 @@ __host__ __device__ constexpr int block_bytes(int D, int page, int bits) {
   return 2 * page * (row_bytes(D, bits) + D / kGroup * 4);
 }
 
+// Programmatic dependent launch: a kernel lets the next one on its stream start
+// as soon as all its own blocks run (pdl_trigger), and a kernel that was started
+// so waits for the one before it, and its memory, before it touches any
+// (pdl_wait).  Only the launch itself overlaps; after a foreign kernel both do
+// nothing.
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+inline cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem,
+                              cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
 // 8 consecutive values of a row as four packed pairs.
 template <bool BF16>
 struct Vec8 {

@@ -41,28 +41,42 @@ __device__ __forceinline__ uint32_t order_key(float s) {
 // dot = sum_d max(q8 * min8, q8 * max8): an upper bound of q.k over the page's
 // keys, up to the roundings to 8 bits.  dot is a whole number below 2^24 and
 // the two products are rounded one by one, so the scores are the same to the
-// bit however the work is split.  8 lanes hold a page's bounds, 4 pages a warp.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(128)
+// bit however the work is split.
+//   8 lanes hold a page's bounds with 16 bytes each (8 at D = 64), and every
+// lane the same channels of up to GP query heads in registers.  The GP sums over
+// 8 lanes are reduced together, halving the heads a lane carries at each step.
+constexpr int kScoreWarps = 8;
+constexpr int kScorePages = 32 * kScoreWarps;  // pages per CTA, 32 a warp
+template <int D, int GP, bool BF16>
+__global__ void __launch_bounds__(32 * kScoreWarps)
     scores_kernel(const void* __restrict__ q, long long q_b, long long q_h,
                   const int8_t* __restrict__ index, const float* __restrict__ index_scale,
                   const int32_t* __restrict__ block_table, const int32_t* __restrict__ kv_lens,
                   uint32_t* __restrict__ keys, int G, int Hkv, int page_size, int max_pages,
                   int num_pages) {
   using T1 = typename Elem<BF16>::T;
-  __shared__ __align__(16) int8_t s_pos[kMaxG][D];  // max(q8, 0)
-  __shared__ __align__(16) int8_t s_neg[kMaxG][D];  // min(q8, 0)
-  __shared__ float s_scale[kMaxG];
+  constexpr int W = D / 32;  // words of 4 channels per lane
+  __shared__ __align__(16) int s_q[2][GP][D / 4];  // max(q8, 0), min(q8, 0)
+  __shared__ float s_scale[GP];
   const int b = blockIdx.z, hkv = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
   const int len = table_len(kv_lens, b, page_size, max_pages,
                             blockIdx.x == 0 && hkv == 0 && threadIdx.x == 0);
   const int count = (int)(((long long)len + page_size - 1) / page_size);
-  if ((int)(blockIdx.x * 128) >= count) return;
-  for (int g = warp; g < G; g += 4) {
-    const T1* qp = static_cast<const T1*>(q) + b * q_b + (hkv * G + g) * q_h;
+  const int p0 = blockIdx.x * kScorePages + warp * 32;  // this warp's first page
+  if ((int)(blockIdx.x * kScorePages) >= count) return;
+  int mine = p0 + lane < count ? block_table[(size_t)b * max_pages + p0 + lane] : 0;
+  if (mine < 0 || mine >= num_pages) {
+    atomicOr(&g_error_flags, 2u);  // page number out of range: page 0's bounds instead
+    mine = 0;
+  }
+  if (warp < GP) {  // a warp a head; heads past the group's are zeros
+    const int g = warp;
     float v[D / 32], top = 0.f;
     bool ok = true;
+    const T1* qp = static_cast<const T1*>(q) + b * q_b + (long long)(hkv * G + min(g, G - 1)) * q_h;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       v[i] = (float)qp[lane + 32 * i];
@@ -75,103 +89,204 @@ __global__ void __launch_bounds__(128)
     const float inv = __frcp_rn(scale);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      const int c = code127(v[i], scale, inv);
-      s_pos[g][lane + 32 * i] = (int8_t)max(c, 0);
-      s_neg[g][lane + 32 * i] = (int8_t)min(c, 0);
+      const int c = g < G ? code127(v[i], scale, inv) : 0;
+      reinterpret_cast<int8_t*>(s_q[0][g])[lane + 32 * i] = (int8_t)max(c, 0);
+      reinterpret_cast<int8_t*>(s_q[1][g])[lane + 32 * i] = (int8_t)min(c, 0);
     }
     if (lane == 0) s_scale[g] = scale;
   }
   __syncthreads();
-  constexpr int W = D / 32;  // 4-byte words per lane of a row's D bytes
   const int sub = lane & 7;
-  // 128 pages per CTA
-  for (int p = blockIdx.x * 128 + warp * 4 + (lane >> 3); p < min(count, (int)(blockIdx.x + 1) * 128);
-       p += 16) {
-    const unsigned mask = 0xffu << (lane & 24);  // the page's 8 lanes
-    int page = block_table[(size_t)b * max_pages + p];
-    if (page < 0 || page >= num_pages) {
-      if (sub == 0) atomicOr(&g_error_flags, 2u);
-      page = 0;
+  int qp[GP][W], qn[GP][W];
+#pragma unroll
+  for (int g = 0; g < GP; ++g)
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      qp[g][i] = s_q[0][g][sub * W + i];
+      qn[g][i] = s_q[1][g][sub * W + i];
     }
+  // after the reduction lane `sub` holds head sub % GP (heads past G: -inf)
+  const int head = sub & (GP - 1);
+  const float qs = s_scale[head];
+  const bool real = head < G;
+#pragma unroll 4
+  for (int it = 0; it < 8; ++it) {
+    const int p = p0 + 4 * it + (lane >> 3);
+    const int page = __shfl_sync(0xffffffffu, mine, 4 * it + (lane >> 3));
     const size_t row = (size_t)page * Hkv + hkv;
-    const int* lo = reinterpret_cast<const int*>(index + row * 2 * D) + sub * W;
-    const int* hi = reinterpret_cast<const int*>(index + row * 2 * D + D) + sub * W;
     const float ps = index_scale[row];
-    float best = -INFINITY;
-    for (int g = 0; g < G; ++g) {
-      int dot = 0;
+    int lo[W], hi[W];
+    if constexpr (W == 4) {
+      *reinterpret_cast<int4*>(lo) = reinterpret_cast<const int4*>(index + row * 2 * D)[sub];
+      *reinterpret_cast<int4*>(hi) = reinterpret_cast<const int4*>(index + row * 2 * D + D)[sub];
+    } else {
+      *reinterpret_cast<int2*>(lo) = reinterpret_cast<const int2*>(index + row * 2 * D)[sub];
+      *reinterpret_cast<int2*>(hi) = reinterpret_cast<const int2*>(index + row * 2 * D + D)[sub];
+    }
+    int dot[GP];
+#pragma unroll
+    for (int g = 0; g < GP; ++g) {
+      dot[g] = 0;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        dot = __dp4a(hi[i], reinterpret_cast<const int*>(s_pos[g])[sub * W + i], dot);
-        dot = __dp4a(lo[i], reinterpret_cast<const int*>(s_neg[g])[sub * W + i], dot);
+        dot[g] = __dp4a(hi[i], qp[g][i], dot[g]);
+        dot[g] = __dp4a(lo[i], qn[g][i], dot[g]);
       }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) dot += __shfl_xor_sync(mask, dot, o);
-      float s = __fmul_rn(__fmul_rn((float)dot, s_scale[g]), ps);
-      if (isnan(s)) s = INFINITY;  // a page or query that is not finite is not hidden
-      best = fmaxf(best, s);
     }
+    // lanes that differ in bit x keep the heads whose number agrees with theirs
+#pragma unroll
+    for (int x = 4, h = GP; x > 0; x >>= 1) {
+      if (h > x) {  // h == 2 x: hand over half the heads
+#pragma unroll
+        for (int g = 0; g < GP / 2; ++g)
+          if (g < h / 2) {
+            const int keep = sub & x ? dot[g + h / 2] : dot[g];
+            const int give = sub & x ? dot[g] : dot[g + h / 2];
+            dot[g] = keep + __shfl_xor_sync(0xffffffffu, give, x);
+          }
+        h /= 2;
+      } else {  // fewer heads than lanes: a plain sum
+#pragma unroll
+        for (int g = 0; g < GP; ++g)
+          if (g < h) dot[g] += __shfl_xor_sync(0xffffffffu, dot[g], x);
+      }
+    }
+    float best = real ? __fmul_rn(__fmul_rn((float)dot[0], qs), ps) : -INFINITY;
+    if (isnan(best)) best = INFINITY;  // a page or query that is not finite is not hidden
+#pragma unroll
+    for (int x = 1; x < GP; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
     if (p == count - 1) best = INFINITY;  // the page being filled
-    if (sub == 0) keys[((size_t)b * Hkv + hkv) * max_pages + p] = order_key(best);
+    if (sub == 0 && p < count) keys[((size_t)b * Hkv + hkv) * max_pages + p] = order_key(best);
   }
 }
 
-// The top_k of `count` keys, ties to the lowest page, in ascending order.
-constexpr int kSelThreads = 256;
-__global__ void __launch_bounds__(kSelThreads)
+// The top_k of `count` keys, ties to the lowest page, in ascending order.  One
+// CTA per (sequence, KV head); up to KPT keys a thread stay in registers, more
+// are read again at each pass.  The top_k-th largest key is found two bits at a
+// time from the top: a pass counts the keys at or above three candidates.
+template <int THREADS, int KPT>
+__global__ void __launch_bounds__(THREADS)
     select_kernel(const uint32_t* __restrict__ keys, const int32_t* __restrict__ kv_lens,
                   int32_t* __restrict__ pages, int Hkv, int page_size, int max_pages, int top_k) {
-  __shared__ int s_cnt[kSelThreads / 32][2];
+  constexpr int NW = THREADS / 32;
+  __shared__ int2 s_cnt[2][NW];
+  __shared__ uint32_t s_at[KPT][NW];
   const int hkv = blockIdx.x, b = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
   const int len = table_len(kv_lens, b, page_size, max_pages, false);
   const int count = (int)(((long long)len + page_size - 1) / page_size);
   const uint32_t* kp = keys + ((size_t)b * Hkv + hkv) * max_pages;
   int32_t* out = pages + ((size_t)b * Hkv + hkv) * top_k;
   if (count <= top_k) {
-    for (int i = threadIdx.x; i < top_k; i += kSelThreads) out[i] = i < count ? i : -1;
+    for (int i = threadIdx.x; i < top_k; i += THREADS) out[i] = i < count ? i : -1;
     return;
   }
-  auto total = [&](int n) {  // sum over the block
-    n = __reduce_add_sync(0xffffffffu, n);
-    __syncthreads();
-    if (lane == 0) s_cnt[warp][0] = n;
-    __syncthreads();
-    int t = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) t += s_cnt[w][0];
-    return t;
-  };
-  // the top_k-th largest key, bit by bit: the largest t with top_k keys >= t
-  uint32_t t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = t | (1u << bit);
-    int n = 0;
-    for (int i = threadIdx.x; i < count; i += kSelThreads) n += kp[i] >= cand;
-    if (total(n) >= top_k) t = cand;
+  const bool held = count <= KPT * THREADS;
+  uint32_t key[KPT];  // 0 (below every real key) behind the last
+  if (held) {
+#pragma unroll
+    for (int c = 0; c < KPT; ++c) {
+      const int i = c * THREADS + threadIdx.x;
+      key[c] = i < count ? kp[i] : 0u;
+    }
   }
-  int n = 0;
-  for (int i = threadIdx.x; i < count; i += kSelThreads) n += kp[i] > t;
-  int ties = top_k - total(n);  // how many keys equal to t are taken, lowest pages first
-  int base = 0, seen = 0;       // written, and equal keys met, so far
-  for (int i0 = 0; i0 < count; i0 += kSelThreads) {
+  int pass = 0;
+  // how many keys are >= x, >= y (both in one word) and >= z over the block
+  auto count3 = [&](uint32_t x, uint32_t y, uint32_t z) {
+    int nx = 0, ny = 0, nz = 0;
+    if (held) {
+#pragma unroll
+      for (int c = 0; c < KPT; ++c) {
+        nx += key[c] >= x;
+        ny += key[c] >= y;
+        nz += key[c] >= z;
+      }
+    } else {
+      for (int i = threadIdx.x; i < count; i += THREADS) {
+        const uint32_t k = kp[i];
+        nx += k >= x;
+        ny += k >= y;
+        nz += k >= z;
+      }
+    }
+    nx = __reduce_add_sync(0xffffffffu, nx);
+    ny = __reduce_add_sync(0xffffffffu, ny);
+    nz = __reduce_add_sync(0xffffffffu, nz);
+    __shared__ int s_z[2][NW];
+    if (lane == 0) {
+      s_cnt[pass & 1][warp] = make_int2(nx, ny);
+      s_z[pass & 1][warp] = nz;
+    }
+    __syncthreads();
+    const int2 v = lane < NW ? s_cnt[pass & 1][lane] : make_int2(0, 0);
+    const int w = lane < NW ? s_z[pass & 1][lane] : 0;
+    ++pass;  // the other buffer next: one barrier a pass is enough
+    return make_int3(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y),
+                     __reduce_add_sync(0xffffffffu, w));
+  };
+  uint32_t t = 0;  // the largest t with top_k keys >= t
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    const int3 n = count3(t | 1u << bit, t | 2u << bit, t | 3u << bit);
+    t |= (uint32_t)((n.x >= top_k) + (n.y >= top_k) + (n.z >= top_k)) << bit;
+  }
+  // keys above t are all taken, of those equal to t the lowest pages
+  const int ties = top_k - (t == 0xffffffffu ? 0 : count3(t + 1, t + 1, t + 1).x);
+  if (held) {
+    // above (low 16 bits) and equal of each warp's 32 pages, in page order
+#pragma unroll
+    for (int c = 0; c < KPT; ++c) {
+      const bool in = c * THREADS + (int)threadIdx.x < count;
+      const int gt = __popc(__ballot_sync(0xffffffffu, in && key[c] > t));
+      const int eq = __popc(__ballot_sync(0xffffffffu, in && key[c] == t));
+      if (lane == 0) s_at[c][warp] = gt | eq << 16;
+    }
+    __syncthreads();
+    if (warp == 0) {  // their exclusive prefix sums
+      uint32_t base = 0;
+      uint32_t* at = &s_at[0][0];
+      for (int k = 0; k < KPT * NW; k += 32) {
+        const uint32_t v = k + lane < KPT * NW ? at[k + lane] : 0u;
+        uint32_t inc = v;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const uint32_t y = __shfl_up_sync(0xffffffffu, inc, x);
+          if (lane >= x) inc += y;
+        }
+        if (k + lane < KPT * NW) at[k + lane] = base + inc - v;
+        base += __shfl_sync(0xffffffffu, inc, 31);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < KPT; ++c) {
+      const int i = c * THREADS + threadIdx.x;
+      const bool gt = i < count && key[c] > t, eq = i < count && key[c] == t;
+      const unsigned below = (1u << lane) - 1;
+      const int gt_at = __popc(__ballot_sync(0xffffffffu, gt) & below) + (s_at[c][warp] & 0xffffu);
+      const int eq_at = __popc(__ballot_sync(0xffffffffu, eq) & below) + (s_at[c][warp] >> 16);
+      if (gt || (eq && eq_at < ties)) out[gt_at + min(eq_at, ties)] = i;
+    }
+    return;
+  }
+  int base = 0, seen = 0;  // written, and equal keys met, so far
+  for (int i0 = 0; i0 < count; i0 += THREADS) {
     const int i = i0 + threadIdx.x;
     const uint32_t k = i < count ? kp[i] : 0u;
     const bool eq = i < count && k == t, gt = i < count && k > t;
     const unsigned meq = __ballot_sync(0xffffffffu, eq), mgt = __ballot_sync(0xffffffffu, gt);
+    const unsigned below = (1u << lane) - 1;
     __syncthreads();
-    if (lane == 0) {
-      s_cnt[warp][0] = __popc(mgt);
-      s_cnt[warp][1] = __popc(meq);
-    }
+    if (lane == 0) s_cnt[0][warp] = make_int2(__popc(mgt), __popc(meq));
     __syncthreads();
-    int gt_before = __popc(mgt & ((1u << lane) - 1)), eq_before = __popc(meq & ((1u << lane) - 1));
-    int gt_all = 0, eq_all = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) gt_before += s_cnt[w][0], eq_before += s_cnt[w][1];
-      gt_all += s_cnt[w][0], eq_all += s_cnt[w][1];
+    int gt_at = __popc(mgt & below), eq_at = __popc(meq & below), gt_all = 0, eq_all = 0;
+    for (int w = 0; w < NW; ++w) {
+      const int2 v = s_cnt[0][w];
+      if (w < warp) gt_at += v.x, eq_at += v.y;
+      gt_all += v.x, eq_all += v.y;
     }
-    if (gt || (eq && seen + eq_before < ties))
-      out[base + gt_before + min(eq_before, ties - seen)] = i;
+    if (gt || (eq && seen + eq_at < ties)) out[base + gt_at + min(eq_at, ties - seen)] = i;
     base += gt_all + min(eq_all, ties - seen);
     seen = min(seen + eq_all, ties);
   }
@@ -290,7 +405,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int worker = blockIdx.x * C::kWarps + warp;
+  pdl_trigger();
   if (worker >= workers) return;
+  pdl_wait();
   const int page_size = 1 << page_shift;
   auto length = [&](int b, bool flag) {
     return table_len(kv_lens, b, page_size, max_pages, flag);
@@ -391,7 +508,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
   lookup(lane, row0, valid0);
   if ((n << np_shift) > 32) lookup(32 + lane, row1, valid1);
   unsigned full = 0;  // bit st: every token of stage st is valid
-  auto issue = [&](int j, int st) {  // copy step j's blocks into stage st
+  auto issue = [&](int j, int st) {  // copy step j's blocks into stage st, one a lane
     const int k = j << np_shift;
     if ((k & 31) == 0 && k > 0) {
       row0 = row1;
@@ -400,20 +517,21 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
     }
     const int row = __shfl_sync(0xffffffffu, row0, (k + lane) & 31);
     const int valid = __shfl_sync(0xffffffffu, valid0, (k + lane) & 31);
-    const bool mine = lane < (1 << np_shift);
+    const bool mine = (lane >> np_shift) == 0;
     const bool copy = mine && valid > 0;
-    const int some = __popc(__ballot_sync(0xffffffffu, copy));
+    uint32_t bytes = C::kStage;
     if (__all_sync(0xffffffffu, !mine || valid == page_size)) {
       full |= 1u << st;
     } else {
       full &= ~(1u << st);
+      bytes = __popc(__ballot_sync(0xffffffffu, copy)) * blk;
       // slab `lane` (< 4) lies in block lane / (page / 16)
       const int slab = __shfl_sync(0xffffffffu, valid0, (k + (lane >> (page_shift - 4))) & 31) -
                        16 * (lane & ((1 << (page_shift - 4)) - 1));
       if (lane < 4) s_valid[4 * st + lane] = min(max(slab, 0), 16);
     }
     const uint32_t bar = bar0 + 8 * st;
-    if (lane == 0) mbar_arrive_expect_tx(bar, some * blk);
+    if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
     __syncwarp();
     if (copy)
       bulk_load(ring0 + st * C::kStage + lane * blk, data + (size_t)(uint32_t)row * blk, blk, bar);
@@ -837,25 +955,27 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
   }
 }
 
-// One CTA of 4 warps per (sequence, query head), for those whose KV head was
+// One CTA of NW warps per (sequence, query head), for those whose KV head was
 // cut; it also writes the answer of empty sequences.  A partial whose l is -inf
 // has no token; a NaN goes through to O and L.  The partials' weights are made
 // first, one a thread; then each row is read as 16 bytes a lane, with eight
 // rows in flight a warp, so that a load's latency is paid a few times and not
 // once per partial.
 constexpr int kChunk = 512;  // weights held at a time
-template <int D, bool BF16>
-__global__ void __launch_bounds__(128)
+template <int D, int NW, bool BF16>
+__global__ void __launch_bounds__(32 * NW)
     combine_kernel(const float* __restrict__ o_part, const float* __restrict__ l_part,
                    const int* __restrict__ meta, const int32_t* __restrict__ kv_lens,
                    void* __restrict__ out, float* __restrict__ lse, int G, int Hkv) {
   using T1 = typename Elem<BF16>::T;
   constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
-  __shared__ float s_w[kChunk], s_red[2][4];
-  __shared__ float4 s_acc[4 * RPW][LPR];
+  __shared__ float s_w[kChunk], s_red[2][NW];
+  __shared__ float4 s_acc[NW * RPW][LPR];
   const size_t row = blockIdx.x;
   const int tile = blockIdx.x / G, h = blockIdx.x % G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
   if (kv_lens[tile / Hkv] <= 0) {
     if (threadIdx.x < D) static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(0.f);
     if (threadIdx.x == 0 && lse != nullptr) lse[row] = -INFINITY;
@@ -868,31 +988,33 @@ __global__ void __launch_bounds__(128)
   const float* lp = l_part + seg0 * G + h;  // partial s at s * G
   const float4* op = reinterpret_cast<const float4*>(o_part + (seg0 * G + h) * D);
   float M = -INFINITY;
-  for (int s = threadIdx.x; s < S; s += 128) M = fmaxf(M, lp[(size_t)s * G]);
+  for (int s = threadIdx.x; s < S; s += 32 * NW) M = fmaxf(M, lp[(size_t)s * G]);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
   if (lane == 0) s_red[0][warp] = M;
   __syncthreads();
-  M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+  M = s_red[0][0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) M = fmaxf(M, s_red[0][w]);
   const int sub = warp * RPW + lane / LPR, c = lane % LPR;
   float L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c0 = 0; c0 < S; c0 += kChunk) {
     const int cn = min(kChunk, S - c0);
     __syncthreads();
-    for (int s = threadIdx.x; s < cn; s += 128) {
+    for (int s = threadIdx.x; s < cn; s += 32 * NW) {
       const float v = lp[(size_t)(c0 + s) * G];
       const float w = v == -INFINITY ? 0.f : expf(v - M);
       s_w[s] = w;
       L += w;
     }
     __syncthreads();
-    for (int s0 = sub; s0 < cn; s0 += 8 * 4 * RPW) {
+    for (int s0 = sub; s0 < cn; s0 += 8 * NW * RPW) {
       float4 v[8];
       float w[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int s = s0 + k * 4 * RPW;
+        const int s = s0 + k * NW * RPW;
         w[k] = s < cn ? s_w[s] : 0.f;
         v[k] = s < cn ? op[(size_t)(c0 + s) * G * LPR + c] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -910,11 +1032,13 @@ __global__ void __launch_bounds__(128)
   if (lane == 0) s_red[1][warp] = L;
   s_acc[sub][c] = acc;
   __syncthreads();
-  L = s_red[1][0] + s_red[1][1] + s_red[1][2] + s_red[1][3];
+  L = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) L += s_red[1][w];
   if (threadIdx.x < D) {
     float a = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4 * RPW; ++k)
+    for (int k = 0; k < NW * RPW; ++k)
       a += reinterpret_cast<const float*>(s_acc[k])[threadIdx.x];
     static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(L == 0.f ? 0.f : a / L);
   }
@@ -931,19 +1055,28 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
                         int Hkv, int D, int page_size, int max_pages, int num_pages, int top_k,
                         int dtype, cudaStream_t stream) {
   using namespace kvq;
-  dim3 grid((unsigned)((max_pages + 127) / 128), (unsigned)Hkv, (unsigned)B);
+  const dim3 grid((unsigned)((max_pages + kScorePages - 1) / kScorePages), (unsigned)Hkv,
+                  (unsigned)B);
+  const int G = H / Hkv;
   auto go = [&](auto kern) {
-    kern<<<grid, 128, 0, stream>>>(q, q_b, q_h, index, index_scale, block_table, kv_lens, keys,
-                                   H / Hkv, Hkv, page_size, max_pages, num_pages);
+    return launch_pdl(kern, grid, 32 * kScoreWarps, 0, stream, q, q_b, q_h, index, index_scale,
+                      block_table, kv_lens, keys, G, Hkv, page_size, max_pages, num_pages);
   };
   const bool bf = dtype == B2A_BF16;
-  if (D == 64) bf ? go(scores_kernel<64, true>) : go(scores_kernel<64, false>);
-  else bf ? go(scores_kernel<128, true>) : go(scores_kernel<128, false>);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (D == 64 && G <= 4) e = bf ? go(scores_kernel<64, 4, true>) : go(scores_kernel<64, 4, false>);
+  else if (D == 64) e = bf ? go(scores_kernel<64, 8, true>) : go(scores_kernel<64, 8, false>);
+  else if (G <= 4) e = bf ? go(scores_kernel<128, 4, true>) : go(scores_kernel<128, 4, false>);
+  else e = bf ? go(scores_kernel<128, 8, true>) : go(scores_kernel<128, 8, false>);
   if (e != cudaSuccess) return set_cuda_error(e, "page score kernel launch");
-  select_kernel<<<dim3((unsigned)Hkv, (unsigned)B), kSelThreads, 0, stream>>>(
-      keys, kv_lens, pages, Hkv, page_size, max_pages, top_k);
-  e = cudaGetLastError();
+  const dim3 tiles((unsigned)Hkv, (unsigned)B);
+  // 8 keys a thread with 256 threads; longer tables take 1024 threads
+  if (max_pages <= 2048)
+    e = launch_pdl(select_kernel<256, 8>, tiles, 256, 0, stream, keys, kv_lens, pages, Hkv,
+                   page_size, max_pages, top_k);
+  else
+    e = launch_pdl(select_kernel<1024, 16>, tiles, 1024, 0, stream, keys, kv_lens, pages, Hkv,
+                   page_size, max_pages, top_k);
   if (e != cudaSuccess) return set_cuda_error(e, "page selection kernel launch");
   return B2A_OK;
 }
@@ -984,14 +1117,19 @@ static int launch_kvq_decode(const void* q, int64_t q_b, int64_t q_h, const uint
   const int64_t segs = (int64_t)workers + (int64_t)B * Hkv;
   float* l_part = ws + segs * G * D;
   int* meta = reinterpret_cast<int*>(l_part + segs * G);
-  kern<<<(workers + C::kWarps - 1) / C::kWarps, 32 * C::kWarps, C::kSmem, stream>>>(
-      q, q_b, q_h, data, block_table, kv_lens, pages, n_list, ws, l_part, meta, o, lse, B, G, Hkv,
-      workers, page_shift, max_pages, num_pages, scale * kLog2e);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_pdl(kern, dim3((workers + C::kWarps - 1) / C::kWarps), 32 * C::kWarps,
+                             C::kSmem, stream, q, q_b, q_h, data, block_table, kv_lens, pages,
+                             n_list, ws, l_part, meta, o, lse, B, G, Hkv, workers, page_shift,
+                             max_pages, num_pages, scale * kLog2e);
   if (e != cudaSuccess) return set_cuda_error(e, "quantised decode kernel launch");
-  combine_kernel<D, BF16><<<B * G * Hkv, 128, 0, stream>>>(ws, l_part, meta, kv_lens, o, lse, G,
-                                                          Hkv);
-  e = cudaGetLastError();
+  // Few (sequence, KV head)s have many partials each: more warps for each.
+  // One sequence of 131072 tokens, 222 partials: 9 us with 4 warps.
+  if (workers > 32ll * B * Hkv)
+    e = launch_pdl(combine_kernel<D, 16, BF16>, dim3(B * G * Hkv), 512, 0, stream, ws, l_part,
+                   meta, kv_lens, o, lse, G, Hkv);
+  else
+    e = launch_pdl(combine_kernel<D, 4, BF16>, dim3(B * G * Hkv), 128, 0, stream, ws, l_part,
+                   meta, kv_lens, o, lse, G, Hkv);
   if (e != cudaSuccess) return set_cuda_error(e, "quantised decode combine launch");
   return B2A_OK;
 }
