@@ -155,15 +155,18 @@ __global__ void __launch_bounds__(32 * kScoreWarps)
     if (isnan(best)) best = INFINITY;  // a page or query that is not finite is not hidden
 #pragma unroll
     for (int x = 1; x < GP; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
-    if (p == count - 1) best = INFINITY;  // the page being filled
     if (sub == 0 && p < count) keys[((size_t)b * Hkv + hkv) * max_pages + p] = order_key(best);
   }
 }
 
-// The top_k of `count` keys, ties to the lowest page, in ascending order.  One
-// CTA per (sequence, KV head); up to KPT keys a thread stay in registers, more
-// are read again at each pass.  The top_k-th largest key is found two bits at a
-// time from the top: a pass counts the keys at or above three candidates.
+// The top_k pages, ties to the lowest page, in ascending order.  The last page
+// counts as +infinity: it and the top_k - 1 best of the others, unless top_k of
+// those are infinite themselves.  One CTA per (sequence, KV head); up to KPT
+// keys a thread stay in registers, more are read again at each pass.  The
+// smallest key that is taken is found bit by bit below the bits that all keys
+// share: a pass counts the keys at or above one candidate, which for keys in
+// registers costs a compare and an add each (three candidates and half the
+// passes cost more: 27 us against 8192 keys on one SM).
 template <int THREADS, int KPT>
 __global__ void __launch_bounds__(THREADS)
     select_kernel(const uint32_t* __restrict__ keys, const int32_t* __restrict__ kv_lens,
@@ -176,63 +179,72 @@ __global__ void __launch_bounds__(THREADS)
   pdl_trigger();
   pdl_wait();
   const int len = table_len(kv_lens, b, page_size, max_pages, false);
-  const int count = (int)(((long long)len + page_size - 1) / page_size);
+  const int all = (int)(((long long)len + page_size - 1) / page_size);
   const uint32_t* kp = keys + ((size_t)b * Hkv + hkv) * max_pages;
   int32_t* out = pages + ((size_t)b * Hkv + hkv) * top_k;
-  if (count <= top_k) {
-    for (int i = threadIdx.x; i < top_k; i += THREADS) out[i] = i < count ? i : -1;
+  if (all <= top_k) {
+    for (int i = threadIdx.x; i < top_k; i += THREADS) out[i] = i < all ? i : -1;
     return;
   }
+  const int count = all - 1;  // without the last page
+  int want = top_k - 1;
   const bool held = count <= KPT * THREADS;
+  const int rounds = held ? (count + THREADS - 1) / THREADS : 0;  // keys a thread holds
   uint32_t key[KPT];  // 0 (below every real key) behind the last
+  uint32_t top = 0, low = 0xffffffffu;
   if (held) {
 #pragma unroll
     for (int c = 0; c < KPT; ++c) {
       const int i = c * THREADS + threadIdx.x;
       key[c] = i < count ? kp[i] : 0u;
+      top = max(top, key[c]);
+      if (i < count) low = min(low, key[c]);
+    }
+  } else {
+    for (int i = threadIdx.x; i < count; i += THREADS) {
+      top = max(top, kp[i]);
+      low = min(low, kp[i]);
     }
   }
   int pass = 0;
-  // how many keys are >= x, >= y (both in one word) and >= z over the block
-  auto count3 = [&](uint32_t x, uint32_t y, uint32_t z) {
-    int nx = 0, ny = 0, nz = 0;
+  auto buffer = [&]() { return pass++ & 1; };  // in turn: one barrier a pass is enough
+  {
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    const int p = buffer();
+    if (lane == 0) s_cnt[p][warp] = make_int2((int)top, (int)low);
+    __syncthreads();
+    const int2 v = s_cnt[p][lane < NW ? lane : 0];
+    top = __reduce_max_sync(0xffffffffu, (uint32_t)v.x);
+    low = __reduce_min_sync(0xffffffffu, (uint32_t)v.y);
+  }
+  auto at_least = [&](uint32_t x) {  // how many keys are >= x
+    int n = 0;
     if (held) {
 #pragma unroll
-      for (int c = 0; c < KPT; ++c) {
-        nx += key[c] >= x;
-        ny += key[c] >= y;
-        nz += key[c] >= z;
-      }
+      for (int c = 0; c < KPT; ++c)
+        if (c < rounds) n += key[c] >= x;
     } else {
-      for (int i = threadIdx.x; i < count; i += THREADS) {
-        const uint32_t k = kp[i];
-        nx += k >= x;
-        ny += k >= y;
-        nz += k >= z;
-      }
+      for (int i = threadIdx.x; i < count; i += THREADS) n += kp[i] >= x;
     }
-    nx = __reduce_add_sync(0xffffffffu, nx);
-    ny = __reduce_add_sync(0xffffffffu, ny);
-    nz = __reduce_add_sync(0xffffffffu, nz);
-    __shared__ int s_z[2][NW];
-    if (lane == 0) {
-      s_cnt[pass & 1][warp] = make_int2(nx, ny);
-      s_z[pass & 1][warp] = nz;
-    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    const int p = buffer();
+    if (lane == 0) s_cnt[p][warp].x = n;
     __syncthreads();
-    const int2 v = lane < NW ? s_cnt[pass & 1][lane] : make_int2(0, 0);
-    const int w = lane < NW ? s_z[pass & 1][lane] : 0;
-    ++pass;  // the other buffer next: one barrier a pass is enough
-    return make_int3(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y),
-                     __reduce_add_sync(0xffffffffu, w));
+    return __reduce_add_sync(0xffffffffu, lane < NW ? s_cnt[p][lane].x : 0);
   };
-  uint32_t t = 0;  // the largest t with top_k keys >= t
-  for (int bit = 30; bit >= 0; bit -= 2) {
-    const int3 n = count3(t | 1u << bit, t | 2u << bit, t | 3u << bit);
-    t |= (uint32_t)((n.x >= top_k) + (n.y >= top_k) + (n.z >= top_k)) << bit;
-  }
+  const uint32_t infinite = order_key(INFINITY);
+  const int inf_keys = top >= infinite ? at_least(infinite) : 0;
+  if (inf_keys >= top_k) want = top_k;
+  else if (threadIdx.x == 0) out[want] = count;
+  if (want == 0) return;
+  // t: the largest value that `want` keys reach
+  const int differ = 32 - __clz(top ^ low);  // bits below the shared ones
+  uint32_t t = differ == 32 ? 0u : top >> differ << differ;
+  for (int bit = differ - 1; bit >= 0; --bit)
+    if (at_least(t | 1u << bit) >= want) t |= 1u << bit;
   // keys above t are all taken, of those equal to t the lowest pages
-  const int ties = top_k - (t == 0xffffffffu ? 0 : count3(t + 1, t + 1, t + 1).x);
+  const int ties = want - (t == 0xffffffffu ? 0 : at_least(t + 1));
   if (held) {
     // above (low 16 bits) and equal of each warp's 32 pages, in page order
 #pragma unroll
@@ -331,9 +343,11 @@ struct DecCfg {
   static constexpr int kRow = row_bytes(D, BITS);
   static constexpr int kNG = D / kGroup;
   static constexpr int kStage = kStep * (2 * kRow + 2 * kNG * 4);
-  // Two stages of 9 or 17 KB a warp; three CTAs of 74 or 70 KB fit an SM.
+  // Two stages of 4.6 to 17 KB a warp: three CTAs of 74 or 70 KB fit an SM, four
+  // of 37.
   static constexpr int kWarps = (D == 128 && BITS == 8) ? 2 : 4;
   static constexpr int kStages = 2;
+  static constexpr int kCtas = (D == 64 && BITS == 4) ? 4 : 3;  // per SM
   static constexpr int kRing = kStages * kStage;
   static constexpr int kOffBar = kWarps * kRing;
   static constexpr int kOffValid = kOffBar + kWarps * kStages * 8;    // [warp][stage] int4
@@ -386,7 +400,7 @@ __device__ __forceinline__ int seq_steps(int len, int n_list, int page_shift) {
 }
 
 template <int D, int BITS, bool BF16, bool HALF>
-__global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, 3)
+__global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>::kCtas)
     decode_kernel(const void* __restrict__ q, long long q_b, long long q_h,
                   const uint8_t* __restrict__ data, const int32_t* __restrict__ block_table,
                   const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ pages,
@@ -1070,7 +1084,7 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
   else e = bf ? go(scores_kernel<128, 8, true>) : go(scores_kernel<128, 8, false>);
   if (e != cudaSuccess) return set_cuda_error(e, "page score kernel launch");
   const dim3 tiles((unsigned)Hkv, (unsigned)B);
-  // 8 keys a thread with 256 threads; longer tables take 1024 threads
+  // at most 8 keys a thread with 256 threads; longer tables take 1024 threads
   if (max_pages <= 2048)
     e = launch_pdl(select_kernel<256, 8>, tiles, 256, 0, stream, keys, kv_lens, pages, Hkv,
                    page_size, max_pages, top_k);
@@ -1083,7 +1097,8 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
 
 // Warps that the GPU runs at a time; no more than there can be steps.
 int kvq_decode_workers(int B, int Hkv, int D, int bits, long long max_tokens) {
-  const long long resident = 148ll * 3 * (D == 128 && bits == 8 ? 2 : 4);
+  const long long resident =
+      148ll * (D == 128 && bits == 8 ? 3 * 2 : D == 64 && bits == 4 ? 4 * 4 : 3 * 4);
   const long long steps = (long long)B * Hkv * ((max_tokens + 63) / 64);
   return (int)(steps < resident ? steps : resident);
 }
