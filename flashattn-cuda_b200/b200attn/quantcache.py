@@ -24,23 +24,52 @@ reference has no KV cache; the decode math is its online softmax
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import List, Optional
 
 import torch
 
 from . import _lib
-from .attention import _DT, _decode_q, _on_device, _ptr, _stream
+from .attention import _DT, _decode_q, _fastcall, _on_device, _ptr, _stream
 from .kvcache import PagePool
 
 GROUP = 64  # channels that share one (scale, min)
 
 
+_BLOCK_BYTES = {}
+
+
 def block_bytes(head_dim: int, page_size: int, bits: int) -> int:
     """Bytes of one (page, KV head) block."""
-    n = _lib.load().b2a_kvq_block_bytes(head_dim, page_size, bits)
-    if n == 0:
-        raise RuntimeError("head_dim must be 64 or 128, page_size 16, 32 or 64 and bits 4 or 8")
+    n = _BLOCK_BYTES.get((head_dim, page_size, bits))
+    if n is None:
+        n = _lib.load().b2a_kvq_block_bytes(head_dim, page_size, bits)
+        if n == 0:
+            raise RuntimeError("head_dim must be 64 or 128, page_size 16, 32 or 64 and bits 4 or 8")
+        _BLOCK_BYTES[head_dim, page_size, bits] = n
     return n
+
+
+if hasattr(_fastcall, "kvq_append"):  # the CPython binding: the same calls, cheaper to make
+    _append, _read = _fastcall.kvq_append, _fastcall.kvq_read
+    _select, _decode = _fastcall.kvq_select, _fastcall.kvq_decode
+else:
+    def _strides(*s):
+        return (ctypes.c_int64 * len(s))(*s)
+
+    def _append(k, v, data, index, index_scale, *rest):
+        return _lib.load().b2a_kvq_append_paged(k, v, _strides(*rest[13:16]), _strides(*rest[16:]),
+                                                data, index, index_scale, *rest[:13])
+
+    def _read(*args):
+        return _lib.load().b2a_kvq_read_paged(*args)
+
+    def _select(q, *rest):
+        return _lib.load().b2a_kvq_select_pages(q, _strides(*rest[16:]), *rest[:16])
+
+    def _decode(q, *rest):
+        return _lib.load().b2a_kvq_decode_paged(q, _strides(*rest[19:21]), *rest[:18], rest[21],
+                                                rest[18])
 
 
 class QuantCache:
@@ -125,14 +154,16 @@ def _check_table(cache: QuantCache, block_table: torch.Tensor, rows: torch.Tenso
         raise RuntimeError(f"{what} must be contiguous int32 [{n}] on the cache's device")
 
 
-def _row_strides(t: torch.Tensor, n: int):
-    """(t, element strides of its first n dims) with t copied where its rows are not contiguous
-    or not 16-byte aligned; a dim of size 1 has stride 0."""
-    shape, st = t.shape, t.stride()
-    if st[-1] != 1 or t.data_ptr() & 15 or any(s & 7 for i, s in enumerate(st[:n]) if shape[i] > 1):
-        t = t.clone(memory_format=torch.contiguous_format)
-        st = t.stride()
-    return t, (ctypes.c_int64 * n)(*(st[i] if shape[i] > 1 else 0 for i in range(n)))
+def _rows_of(t: torch.Tensor, n: int):
+    """t, or a copy where its rows are not contiguous or not 16-byte aligned, and the element
+    strides of its first n dims; a dim of size 1 has stride 0."""
+    st = t.stride()
+    if st[-1] == 1 and not t.data_ptr() & 15:
+        st = [0 if k == 1 else s for k, s in zip(t.shape, st[:n])]
+        if not any(s & 7 for s in st):
+            return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, [0 if k == 1 else s for k, s in zip(t.shape, t.stride()[:n])]
 
 
 def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCache,
@@ -157,15 +188,14 @@ def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCac
         raise RuntimeError("block_table must have one row per sequence")
     if B == 0 or T == 0:
         return
-    lib = _lib.load()
     with _on_device(dev):
-        kn, ks = _row_strides(k_new, 3)
-        vn, vs = _row_strides(v_new, 3)
-        _lib.check(lib.b2a_kvq_append_paged(
-            kn.data_ptr(), vn.data_ptr(), ks, vs, cache.data.data_ptr(), _ptr(cache.index),
+        kn, ks = _rows_of(k_new, 3)
+        vn, vs = _rows_of(v_new, 3)
+        _lib.check(_append(
+            kn.data_ptr(), vn.data_ptr(), cache.data.data_ptr(), _ptr(cache.index),
             _ptr(cache.index_scale), block_table.data_ptr(), kv_lens.data_ptr(), B, Hkv, T, D,
             cache.page_size, block_table.shape[1], cache.num_pages, cache.bits,
-            _DT[cache.dtype], int(bool(advance)), _stream(dev)))
+            _DT[cache.dtype], int(bool(advance)), _stream(dev), *ks, *vs))
 
 
 def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -196,7 +226,7 @@ def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: t
             K = torch.empty(shape, dtype=cache.dtype, device=dev)
             V = torch.empty(shape, dtype=cache.dtype, device=dev)
         if B > 0 and total > 0 and max_len > 0:
-            _lib.check(_lib.load().b2a_kvq_read_paged(
+            _lib.check(_read(
                 cache.data.data_ptr(), block_table.data_ptr(), _ptr(start),
                 cu_seqlens.data_ptr(), K.data_ptr(), V.data_ptr(), B, shape[1], shape[2],
                 cache.page_size, block_table.shape[1], cache.num_pages, shape[0], int(max_len),
@@ -238,13 +268,22 @@ def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
         if B == 0:
             return pages
         keys = torch.empty(B * Hkv * max_pages, dtype=torch.int32, device=dev)
-        qc, qs = _row_strides(q3, 2)
-        _lib.check(_lib.load().b2a_kvq_select_pages(
-            qc.data_ptr(), qs, cache.index.data_ptr(), cache.index_scale.data_ptr(),
+        qc, qs = _rows_of(q3, 2)
+        _lib.check(_select(
+            qc.data_ptr(), cache.index.data_ptr(), cache.index_scale.data_ptr(),
             block_table.data_ptr(), kv_lens.data_ptr(), keys.data_ptr(), pages.data_ptr(), B, H,
             Hkv, D, cache.page_size, max_pages, cache.num_pages, int(top_k), _DT[cache.dtype],
-            _stream(dev)))
+            _stream(dev), *qs))
     return pages
+
+
+@functools.lru_cache(maxsize=256)
+def _plan(B: int, H: int, Hkv: int, D: int, bits: int, max_tokens: int, splits):
+    """(warps that share a decode, floats of its workspace): functions of the sizes alone."""
+    lib = _lib.load()
+    workers = (lib.b2a_kvq_decode_workers(B, Hkv, D, bits, max_tokens) if splits is None
+               else int(splits) * B * Hkv)
+    return workers, max(lib.b2a_kvq_decode_workspace_floats(B, H, Hkv, D, workers), 1)
 
 
 def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
@@ -268,25 +307,21 @@ def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Te
                 or pages.device != dev):
             raise RuntimeError("pages must be contiguous int32 [B, Hkv, n] on the cache's device")
         n_pages = pages.shape[2]
-    lib = _lib.load()
+    max_pages = block_table.shape[1]
     with _on_device(dev):
         O = torch.empty((B, H, D), dtype=cache.dtype, device=dev)
         L = torch.empty((B, H), dtype=torch.float32, device=dev)
         if B > 0:
-            if splits is None:
-                workers = lib.b2a_kvq_decode_workers(
-                    B, Hkv, D, cache.bits, (n_pages or block_table.shape[1]) * cache.page_size)
-            else:
-                workers = int(splits) * B * Hkv
-            ws = torch.empty(max(lib.b2a_kvq_decode_workspace_floats(B, H, Hkv, D, workers), 1),
-                             dtype=torch.float32, device=dev)
-            qc, qs = _row_strides(q3, 2)
-            _lib.check(lib.b2a_kvq_decode_paged(
-                qc.data_ptr(), qs, cache.data.data_ptr(), block_table.data_ptr(),
-                kv_lens.data_ptr(), _ptr(pages), n_pages, ws.data_ptr(), O.data_ptr(),
-                L.data_ptr(), B, H, Hkv, D, cache.page_size, block_table.shape[1],
-                cache.num_pages, workers, cache.bits, _DT[cache.dtype],
-                float(D) ** -0.5 if scale is None else float(scale), _stream(dev)))
+            workers, floats = _plan(B, H, Hkv, D, cache.bits,
+                                    (n_pages or max_pages) * cache.page_size, splits)
+            ws = torch.empty(floats, dtype=torch.float32, device=dev)
+            qc, qs = _rows_of(q3, 2)
+            _lib.check(_decode(
+                qc.data_ptr(), cache.data.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(),
+                _ptr(pages), n_pages, ws.data_ptr(), O.data_ptr(), L.data_ptr(), B, H, Hkv, D,
+                cache.page_size, max_pages, cache.num_pages, workers, cache.bits,
+                _DT[cache.dtype], _stream(dev), *qs,
+                float(D) ** -0.5 if scale is None else float(scale)))
     if had_len:
         return [O.unsqueeze(2), L.unsqueeze(2)]
     return [O, L]
