@@ -100,52 +100,61 @@ __device__ __forceinline__ float group_step(float lo, float hi) {
   return s < kTinyStep ? 0.f : s;
 }
 
-// Round to nearest even of 0 <= x <= 255 as an integer in the low mantissa bits.
-__device__ __forceinline__ uint32_t small_rint(float x) {
-  return __float_as_uint(__fadd_rn(x, 8388608.f)) & 0xffu;
+// Reciprocal of half a step (0 for a step of 0 or NaN: codes 0).
+__device__ __forceinline__ float step_inverse(float step) {
+  return step > 0.f ? __frcp_rn(0.5f * step) : 0.f;
 }
 
-// Codes of 8 values of a group (lo, step): one word at 4 bits, two at 8.
+// Codes of 8 finite values of a group, min(rint((x/2 - lo/2) * inv), n): one
+// word at 4 bits, two at 8.  Adding 2^23 leaves the value, rounded to nearest
+// even, in the low mantissa bits.
 template <bool BF16, int BITS>
-__device__ __forceinline__ uint2 encode8(const Vec8<BF16>& x, float lo, float step) {
+__device__ __forceinline__ uint2 encode8(const Vec8<BF16>& x, float lo, float inv) {
   constexpr float n = (float)((1 << BITS) - 1);
-  uint2 w = make_uint2(0u, 0u);
-  if (step > 0.f) {  // also false for a NaN step: codes 0
-    const float inv = __frcp_rn(0.5f * step), lo2 = 0.5f * lo;
+  const float lo2 = 0.5f * lo;
+  uint32_t c[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Elem<BF16>::unpack(x.v[i]);
-      const uint32_t c0 = small_rint(fminf(__fmul_rn(__fsub_rn(0.5f * f.x, lo2), inv), n));
-      const uint32_t c1 = small_rint(fminf(__fmul_rn(__fsub_rn(0.5f * f.y, lo2), inv), n));
-      if constexpr (BITS == 4) {
-        w.x |= (c0 | (c1 << 4)) << (8 * i);
-      } else {
-        const uint32_t p = c0 | (c1 << 8);
-        if (i < 2) w.x |= p << (16 * i);
-        else w.y |= p << (16 * (i - 2));
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Elem<BF16>::unpack(x.v[i]);
+    // x/2 is exact, so the fused form rounds once as the difference does
+    c[2 * i] = __float_as_uint(
+        __fadd_rn(fminf(__fmul_rn(__fmaf_rn(f.x, 0.5f, -lo2), inv), n), 8388608.f));
+    c[2 * i + 1] = __float_as_uint(
+        __fadd_rn(fminf(__fmul_rn(__fmaf_rn(f.y, 0.5f, -lo2), inv), n), 8388608.f));
+  }
+  uint2 w = make_uint2(0u, 0u);
+  if constexpr (BITS == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = c[2 * i] + (c[2 * i + 1] << 4);  // a byte, rest unused
+    w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  } else {
+    w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
   }
   return w;
 }
 
 // The values that 8 codes stand for: one fused multiply-add in fp32, rounded
-// once to dtype.
+// once to dtype.  A code becomes a float by placing its byte in 2^23 (int to
+// float conversions run at a quarter of the rate).
 template <bool BF16, int BITS>
 __device__ __forceinline__ Vec8<BF16> decode8(uint2 w, float step, float lo) {
   Vec8<BF16> r;
+  const uint32_t even = w.x & 0x0f0f0f0fu, odd = (w.x >> 4) & 0x0f0f0f0fu;  // 4 bits
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t c0, c1;
     if constexpr (BITS == 4) {
-      c0 = (w.x >> (8 * i)) & 15u;
-      c1 = (w.x >> (8 * i + 4)) & 15u;
+      c0 = __byte_perm(even, 0x4b000000u, 0x7550 + i);
+      c1 = __byte_perm(odd, 0x4b000000u, 0x7550 + i);
     } else {
-      const uint32_t p = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
-      c0 = p & 255u;
-      c1 = (p >> 8) & 255u;
+      const uint32_t x = i < 2 ? w.x : w.y;
+      c0 = __byte_perm(x, 0x4b000000u, i & 1 ? 0x7552 : 0x7550);
+      c1 = __byte_perm(x, 0x4b000000u, i & 1 ? 0x7553 : 0x7551);
     }
-    r.v[i] = Elem<BF16>::pack(__fmaf_rn((float)c0, step, lo), __fmaf_rn((float)c1, step, lo));
+    r.v[i] = Elem<BF16>::pack(
+        __fmaf_rn(__fadd_rn(__uint_as_float(c0), -8388608.f), step, lo),
+        __fmaf_rn(__fadd_rn(__uint_as_float(c1), -8388608.f), step, lo));
   }
   return r;
 }
