@@ -69,21 +69,20 @@ __device__ __forceinline__ typename Elem<BF16>::T2 max2_nan(typename Elem<BF16>:
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// fp32 -> dtype with directed rounding (x >= 0), back in fp32
+// fp32 x >= 0 -> dtype with directed rounding, back in fp32
 template <bool BF16>
 __device__ __forceinline__ float round_up(float x) {
-  if constexpr (BF16) return __bfloat162float(__float2bfloat16_ru(x));
-  else return __half2float(__float2half_ru(x));
+  if constexpr (BF16) {
+    const uint32_t u = __float_as_uint(x);
+    return __uint_as_float((u + 0xffffu) & 0xffff0000u);
+  } else {
+    return __half2float(__float2half_ru(x));
+  }
 }
 template <bool BF16>
 __device__ __forceinline__ float round_down(float x) {
-  if constexpr (BF16) return __bfloat162float(__float2bfloat16_rd(x));
+  if constexpr (BF16) return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
   else return __half2float(__float2half_rd(x));
-}
-template <bool BF16>
-__device__ __forceinline__ float round_near(float x) {
-  const float2 r = Elem<BF16>::unpack(Elem<BF16>::pack(x, 0.f));
-  return r.x;
 }
 
 // The step of a group with extremes lo, hi (both finite) and n = 2^bits - 1:
@@ -95,8 +94,10 @@ template <bool BF16, int BITS>
 __device__ __forceinline__ float group_step(float lo, float hi) {
   constexpr float n = (float)((1 << BITS) - 1);
   const float want = __fmul_rn(__fsub_rn(0.5f * hi, 0.5f * lo), 2.0f / n);
+  // the least fp32 that rounds to infinity: max + half a last place
+  constexpr float kPast = BF16 ? 3.3961775292304601e38f : 65520.f;
   float s = round_up<BF16>(want);
-  if (!finite(round_near<BF16>(__fmaf_rn(n, s, lo)))) s = round_down<BF16>(want);
+  if (__fmaf_rn(n, s, lo) >= kPast) s = round_down<BF16>(want);
   return s < kTinyStep ? 0.f : s;
 }
 

@@ -104,17 +104,28 @@ __global__ void append_kernel(const void* __restrict__ k_new, const void* __rest
     return m;
   };
   uint32_t* params = reinterpret_cast<uint32_t*>(blk + 2 * page_size * ROW);
-  auto load = [&](int s, Vec8<BF16>& k, Vec8<BF16>& v) {
-    const long long t = t0 + (s < s1 ? s : s0);  // idle rows repeat a live one: shuffles stay whole
-    *reinterpret_cast<uint4*>(&k) = *reinterpret_cast<const uint4*>(kp + t * ks.t);
-    *reinterpret_cast<uint4*>(&v) = *reinterpret_cast<const uint4*>(vp + t * vs.t);
-  };
+  // This lane's row of the next iteration; one behind the last keeps its values,
+  // so that the shuffles stay whole.
   Vec8<BF16> next[2];
-  load(s0 + r, next[0], next[1]);
+  {
+    const long long t = t0 + (s0 + r < s1 ? s0 + r : s0);
+    kp += t * ks.t;
+    vp += t * vs.t;
+    *reinterpret_cast<uint4*>(&next[0]) = *reinterpret_cast<const uint4*>(kp);
+    *reinterpret_cast<uint4*>(&next[1]) = *reinterpret_cast<const uint4*>(vp);
+  }
+  const long long k_step = RPI * ks.t, v_step = RPI * vs.t;
+  uint8_t* row = blk + (s0 + r) * ROW + c * (ROW / LPR);
+  uint32_t* par = params + ((c & 4 ? page_size : 0) + s0 + r) * NG + grp;
   for (int s = s0 + r; s - r < s1; s += RPI) {
     const bool live = s < s1;
     const Vec8<BF16> x[2] = {next[0], next[1]};
-    if (s - r + RPI < s1) load(s + RPI, next[0], next[1]);  // ahead of this row's arithmetic
+    kp += k_step;
+    vp += v_step;
+    if (s + RPI < s1) {  // ahead of this row's arithmetic
+      *reinterpret_cast<uint4*>(&next[0]) = *reinterpret_cast<const uint4*>(kp);
+      *reinterpret_cast<uint4*>(&next[1]) = *reinterpret_cast<const uint4*>(vp);
+    }
     // The steps of K and V are worked out side by side: K's by the lower four
     // lanes of a group, V's by the upper four.
     T2 ext[2] = {extremes(x[0]), extremes(x[1])};
@@ -128,8 +139,7 @@ __global__ void append_kernel(const void* __restrict__ k_new, const void* __rest
     const float other_step = __shfl_xor_sync(0xffffffffu, step, 4);
     const float other_inv = __shfl_xor_sync(0xffffffffu, inv, 4);
     // lane 0 of a group writes K's pair, lane 4 V's
-    if (live && (c & 3) == 0)
-      params[((upper ? page_size : 0) + s) * NG + grp] = pack2_u32<BF16>(step, low);
+    if (live && (c & 3) == 0) *par = pack2_u32<BF16>(step, low);
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       const bool own = upper == (side == 1);
@@ -137,22 +147,24 @@ __global__ void append_kernel(const void* __restrict__ k_new, const void* __rest
       uint2 w = encode8<BF16, BITS>(x[side], lo, own ? inv : other_inv);
       if (isnan(lo)) w = make_uint2(0u, 0u);
       if (live) {
-        uint8_t* row = blk + (size_t)(side * page_size + s) * ROW;
-        if constexpr (BITS == 4) reinterpret_cast<uint32_t*>(row)[c] = w.x;
-        else reinterpret_cast<uint2*>(row)[c] = w;
+        uint8_t* dst = row + (side ? page_size * ROW : 0);
+        if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(dst) = w.x;
+        else *reinterpret_cast<uint2*>(dst) = w;
       }
       if (side == 0 && index != nullptr)
         bound(decode8<BF16, BITS>(w, own ? step : other_step, lo));
     }
+    row += RPI * ROW;
+    par += RPI * NG;
   }
   if (index == nullptr) return;
   // the keys already in the page
   for (int s = 0; s < s0; s += RPI) {
     const int slot = min(s + r, s0 - 1);
-    const uint8_t* row = blk + (size_t)slot * ROW;
+    const uint8_t* old = blk + (size_t)slot * ROW;
     uint2 w = make_uint2(0u, 0u);
-    if constexpr (BITS == 4) w.x = reinterpret_cast<const uint32_t*>(row)[c];
-    else w = reinterpret_cast<const uint2*>(row)[c];
+    if constexpr (BITS == 4) w.x = reinterpret_cast<const uint32_t*>(old)[c];
+    else w = reinterpret_cast<const uint2*>(old)[c];
     const float2 p = param<BF16>(
         reinterpret_cast<const uint32_t*>(blk + 2 * page_size * ROW)[slot * NG + grp]);
     bound(decode8<BF16, BITS>(w, p.x, p.y));
