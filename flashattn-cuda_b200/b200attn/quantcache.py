@@ -80,24 +80,28 @@ class QuantCache:
     dtype is that of the keys and values written and read (float16 or bfloat16).
     """
 
-    __slots__ = ("data", "index", "index_scale", "page_size", "head_dim", "bits", "dtype")
+    __slots__ = ("data", "index", "index_scale", "page_size", "head_dim", "bits", "dtype",
+                 "device", "num_pages", "num_kv_heads")
 
     def __init__(self, data: torch.Tensor, *, page_size: int, head_dim: int, bits: int,
                  dtype: torch.dtype, index: Optional[torch.Tensor] = None,
                  index_scale: Optional[torch.Tensor] = None):
         if dtype not in _DT:
             raise RuntimeError("dtype must be torch.float16 or torch.bfloat16")
-        if (data.dim() != 3 or data.dtype != torch.uint8 or not data.is_contiguous()
-                or data.shape[2] != block_bytes(head_dim, page_size, bits)):
+        shape = data.shape
+        if (len(shape) != 3 or data.dtype is not torch.uint8 or not data.is_contiguous()
+                or shape[2] != block_bytes(head_dim, page_size, bits)):
             raise RuntimeError("data must be contiguous uint8 [P, Hkv, block_bytes]")
+        self.num_pages, self.num_kv_heads, _ = shape
+        self.device = data.device
         if (index is None) != (index_scale is None):
             raise RuntimeError("index and index_scale must be given together")
         if index is not None:
-            P, Hkv, _ = data.shape
-            if (index.shape != (P, Hkv, 2, head_dim) or index.dtype != torch.int8
-                    or index_scale.shape != (P, Hkv) or index_scale.dtype != torch.float32
+            P, Hkv, _ = shape
+            if (index.shape != (P, Hkv, 2, head_dim) or index.dtype is not torch.int8
+                    or index_scale.shape != (P, Hkv) or index_scale.dtype is not torch.float32
                     or not (index.is_contiguous() and index_scale.is_contiguous())
-                    or index.device != data.device or index_scale.device != data.device):
+                    or index.device != self.device or index_scale.device != self.device):
                 raise RuntimeError("index must be contiguous int8 [P, Hkv, 2, D] and index_scale "
                                    "fp32 [P, Hkv] on data's device")
         self.data, self.index, self.index_scale = data, index, index_scale
@@ -118,14 +122,6 @@ class QuantCache:
         return cls(data, page_size=page_size, head_dim=head_dim, bits=bits, dtype=dtype,
                    index=idx, index_scale=sc)
 
-    @property
-    def num_pages(self) -> int:
-        return self.data.shape[0]
-
-    @property
-    def num_kv_heads(self) -> int:
-        return self.data.shape[1]
-
     def codes(self, side: int) -> torch.Tensor:
         """View of the K (0) or V (1) codes: uint8 [P, Hkv, page_size, D*bits/8]."""
         row = self.head_dim * self.bits // 8
@@ -141,17 +137,21 @@ class QuantCache:
 
 
 def _check_table(cache: QuantCache, block_table: torch.Tensor, rows: torch.Tensor, what: str,
-                 n: int) -> None:
-    """block_table int32 [B, max_pages] and `rows` int32 [n], contiguous, on the cache's device."""
-    dev = cache.data.device
-    if not cache.data.is_cuda:
+                 extra: int = 0):
+    """(B, max_pages) of block_table int32 [B, max_pages], with `rows` int32 [B + extra], both
+    contiguous and on the cache's device."""
+    dev = cache.device
+    if dev.type != "cuda":
         raise RuntimeError("the cache must be on a CUDA device")
-    if (block_table.dim() != 2 or block_table.dtype != torch.int32
+    shape = block_table.shape
+    if (len(shape) != 2 or block_table.dtype is not torch.int32
             or not block_table.is_contiguous() or block_table.device != dev):
         raise RuntimeError("block_table must be contiguous int32 [B, max_pages] on the cache's device")
-    if (rows.shape != (n,) or rows.dtype != torch.int32 or not rows.is_contiguous()
-            or rows.device != dev):
-        raise RuntimeError(f"{what} must be contiguous int32 [{n}] on the cache's device")
+    if (rows.dim() != 1 or rows.shape[0] != shape[0] + extra or rows.dtype is not torch.int32
+            or not rows.is_contiguous() or rows.device != dev):
+        raise RuntimeError(f"{what} must be contiguous int32 [{shape[0] + extra}] on the cache's "
+                           "device (block_table has one row per sequence)")
+    return shape
 
 
 def _rows_of(t: torch.Tensor, n: int):
@@ -173,18 +173,19 @@ def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCac
     positions kv_lens[b] + t of the sequences in block_table (b2a_kvq_append_paged); with
     `advance`, kv_lens += T on the device.  Updates the index of a cache that has one.
     No page may be owned by two of the sequences that write to it."""
-    if k_new.dim() != 4 or k_new.shape != v_new.shape:
+    shape = k_new.shape
+    if len(shape) != 4 or shape != v_new.shape:
         raise RuntimeError("k_new and v_new must both be [B, Hkv, T, D]")
-    B, Hkv, T, D = k_new.shape
+    B, Hkv, T, D = shape
     if Hkv != cache.num_kv_heads or D != cache.head_dim:
         raise RuntimeError("k_new must match the cache's KV heads and head dim")
-    if k_new.dtype != cache.dtype or v_new.dtype != cache.dtype:
+    if k_new.dtype is not cache.dtype or v_new.dtype is not cache.dtype:
         raise RuntimeError("k_new and v_new must have the cache's dtype")
-    _check_table(cache, block_table, kv_lens, "kv_lens", B)
-    dev = cache.data.device
+    rows, max_pages = _check_table(cache, block_table, kv_lens, "kv_lens")
+    dev = cache.device
     if k_new.device != dev or v_new.device != dev:
         raise RuntimeError("k_new and v_new must be on the cache's device")
-    if block_table.shape[0] != B:
+    if rows != B:
         raise RuntimeError("block_table must have one row per sequence")
     if B == 0 or T == 0:
         return
@@ -194,8 +195,8 @@ def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCac
         _lib.check(_append(
             kn.data_ptr(), vn.data_ptr(), cache.data.data_ptr(), _ptr(cache.index),
             _ptr(cache.index_scale), block_table.data_ptr(), kv_lens.data_ptr(), B, Hkv, T, D,
-            cache.page_size, block_table.shape[1], cache.num_pages, cache.bits,
-            _DT[cache.dtype], int(bool(advance)), _stream(dev), *ks, *vs))
+            cache.page_size, max_pages, cache.num_pages, cache.bits, _DT[cache.dtype],
+            int(bool(advance)), _stream(dev), *ks, *vs))
 
 
 def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -206,11 +207,10 @@ def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: t
     cu_seqlens[b+1] - cu_seqlens[b] (int32 [B+1], device), go to rows cu_seqlens[b] .. ;
     total = cu_seqlens[B] and max_len, a bound of every length, are host numbers.
     `out` = (K, V) to write into; rows that no sequence owns are left as they were."""
-    B = block_table.shape[0]
-    _check_table(cache, block_table, cu_seqlens, "cu_seqlens", B + 1)
+    B, max_pages = _check_table(cache, block_table, cu_seqlens, "cu_seqlens", 1)
     if start is not None:
-        _check_table(cache, block_table, start, "start", B)
-    dev = cache.data.device
+        _check_table(cache, block_table, start, "start")
+    dev = cache.device
     shape = (int(total), cache.num_kv_heads, cache.head_dim)
     if shape[0] < 0 or max_len < 0:
         raise RuntimeError("total and max_len must be >= 0")
@@ -229,21 +229,22 @@ def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: t
             _lib.check(_read(
                 cache.data.data_ptr(), block_table.data_ptr(), _ptr(start),
                 cu_seqlens.data_ptr(), K.data_ptr(), V.data_ptr(), B, shape[1], shape[2],
-                cache.page_size, block_table.shape[1], cache.num_pages, shape[0], int(max_len),
+                cache.page_size, max_pages, cache.num_pages, shape[0], int(max_len),
                 cache.bits, _DT[cache.dtype], _stream(dev)))
     return [K, V]
 
 
 def _check_query(q: torch.Tensor, cache: QuantCache):
+    """(q as [B, H, D], whether it had a length dim, B, H, D)."""
     q3, had_len = _decode_q(q)
-    if not q3.is_cuda or q3.device != cache.data.device:
+    if not q3.is_cuda or q3.device != cache.device:
         raise RuntimeError("q must be a CUDA tensor on the cache's device")
-    if q3.dtype != cache.dtype:
+    if q3.dtype is not cache.dtype:
         raise RuntimeError("q must have the cache's dtype")
-    H, Hkv = q3.shape[1], cache.num_kv_heads
-    if q3.shape[2] != cache.head_dim or H == 0 or H % Hkv != 0:
+    B, H, D = q3.shape
+    if D != cache.head_dim or H == 0 or H % cache.num_kv_heads != 0:
         raise RuntimeError("q must be [B, H, D] with the cache's head dim and H a multiple of Hkv")
-    return q3, had_len
+    return q3, had_len, B, H, D
 
 
 def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
@@ -252,26 +253,25 @@ def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
     [B, H, 1, D]): int32 [B, Hkv, top_k], logical page numbers, ascending, -1 behind the
     last.  A page's score is an upper bound, from the cache's index, of its keys' products
     with the group's query heads, in 8 bits (b2a_kvq_select_pages)."""
-    q3, _ = _check_query(q, cache)
+    q3, _, B, H, D = _check_query(q, cache)
     if cache.index is None:
         raise RuntimeError("select_pages needs a cache with an index")
     if top_k <= 0:
         raise RuntimeError("top_k must be > 0")
-    B, H, D = q3.shape
-    _check_table(cache, block_table, kv_lens, "kv_lens", B)
-    if block_table.shape[0] != B:
+    rows, max_pages = _check_table(cache, block_table, kv_lens, "kv_lens")
+    if rows != B:
         raise RuntimeError("block_table must have one row per sequence")
-    dev = cache.data.device
-    Hkv, max_pages = cache.num_kv_heads, block_table.shape[1]
+    dev, Hkv = cache.device, cache.num_kv_heads
     with _on_device(dev):
         pages = torch.empty((B, Hkv, int(top_k)), dtype=torch.int32, device=dev)
         if B == 0:
             return pages
-        keys = torch.empty(B * Hkv * max_pages, dtype=torch.int32, device=dev)
+        keys = (torch.empty(B * Hkv * max_pages, dtype=torch.int32, device=dev)
+                if max_pages > 2048 else None)
         qc, qs = _rows_of(q3, 2)
         _lib.check(_select(
             qc.data_ptr(), cache.index.data_ptr(), cache.index_scale.data_ptr(),
-            block_table.data_ptr(), kv_lens.data_ptr(), keys.data_ptr(), pages.data_ptr(), B, H,
+            block_table.data_ptr(), kv_lens.data_ptr(), _ptr(keys), pages.data_ptr(), B, H,
             Hkv, D, cache.page_size, max_pages, cache.num_pages, int(top_k), _DT[cache.dtype],
             _stream(dev), *qs))
     return pages
@@ -294,27 +294,26 @@ def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Te
     [B, H, 1, D]); kv_lens may hold zeros (O = 0, L = -inf).  `pages` int32 [B, Hkv, n]
     (from select_pages) restricts each KV head to those pages; negative entries are skipped.
     `splits` overrides the number of warps that share the work, as a multiple of B * Hkv."""
-    q3, had_len = _check_query(q, cache)
-    B, H, D = q3.shape
-    _check_table(cache, block_table, kv_lens, "kv_lens", B)
-    if block_table.shape[0] != B:
+    q3, had_len, B, H, D = _check_query(q, cache)
+    rows, max_pages = _check_table(cache, block_table, kv_lens, "kv_lens")
+    if rows != B:
         raise RuntimeError("block_table must have one row per sequence")
-    dev, Hkv = cache.data.device, cache.num_kv_heads
+    dev, Hkv = cache.device, cache.num_kv_heads
     n_pages = 0
     if pages is not None:
-        if (pages.dim() != 3 or pages.shape[:2] != (B, Hkv) or pages.shape[2] == 0
-                or pages.dtype != torch.int32 or not pages.is_contiguous()
+        shape = pages.shape
+        if (len(shape) != 3 or shape[0] != B or shape[1] != Hkv or shape[2] == 0
+                or pages.dtype is not torch.int32 or not pages.is_contiguous()
                 or pages.device != dev):
             raise RuntimeError("pages must be contiguous int32 [B, Hkv, n] on the cache's device")
-        n_pages = pages.shape[2]
-    max_pages = block_table.shape[1]
+        n_pages = shape[2]
     with _on_device(dev):
-        O = torch.empty((B, H, D), dtype=cache.dtype, device=dev)
-        L = torch.empty((B, H), dtype=torch.float32, device=dev)
+        O = q3.new_empty((B, H, D))
+        L = q3.new_empty((B, H), dtype=torch.float32)
         if B > 0:
             workers, floats = _plan(B, H, Hkv, D, cache.bits,
                                     (n_pages or max_pages) * cache.page_size, splits)
-            ws = torch.empty(floats, dtype=torch.float32, device=dev)
+            ws = L.new_empty(floats)
             qc, qs = _rows_of(q3, 2)
             _lib.check(_decode(
                 qc.data_ptr(), cache.data.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(),

@@ -2,7 +2,8 @@
 // quantised paged KV cache (format: kvquant.cuh), and the selection of pages
 // by a cheap score.
 //
-//   scores_kernel / select_kernel   the top_k pages of every (sequence, KV head)
+//   score_select_kernel             the top_k pages of every (sequence, KV head);
+//   scores_kernel, select_kernel    the same in two steps for long tables
 //   decode_kernel                   attention over all or the selected pages
 //   combine_kernel                  LSE-weighted merge of what several warps shared
 #include <type_traits>
@@ -46,37 +47,44 @@ __device__ __forceinline__ uint32_t order_key(float s) {
 // lane the same channels of up to GP query heads in registers.  The GP sums over
 // 8 lanes are reduced together, halving the heads a lane carries at each step.
 constexpr int kScoreWarps = 8;
-constexpr int kScorePages = 32 * kScoreWarps;  // pages per CTA, 32 a warp
+constexpr int kScorePages = 32 * kScoreWarps;  // pages per round of a CTA, 32 a warp
+struct ScoreArgs {
+  const void* q;
+  long long q_b, q_h;  // element strides
+  const int8_t* index;
+  const float* index_scale;
+  const int32_t* block_table;
+  const int32_t* kv_lens;
+  int G, Hkv, page_size, max_pages, num_pages;
+};
+
+// The keys of pages [first, last) of (b, hkv), by a CTA of kScoreWarps warps; page
+// p's goes to keys[p].
 template <int D, int GP, bool BF16>
-__global__ void __launch_bounds__(32 * kScoreWarps)
-    scores_kernel(const void* __restrict__ q, long long q_b, long long q_h,
-                  const int8_t* __restrict__ index, const float* __restrict__ index_scale,
-                  const int32_t* __restrict__ block_table, const int32_t* __restrict__ kv_lens,
-                  uint32_t* __restrict__ keys, int G, int Hkv, int page_size, int max_pages,
-                  int num_pages) {
+__device__ __forceinline__ void score_pages(const ScoreArgs& a, int b, int hkv, int first,
+                                            int last, uint32_t* keys) {
   using T1 = typename Elem<BF16>::T;
   constexpr int W = D / 32;  // words of 4 channels per lane
   __shared__ __align__(16) int s_q[2][GP][D / 4];  // max(q8, 0), min(q8, 0)
   __shared__ float s_scale[GP];
-  const int b = blockIdx.z, hkv = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
-  pdl_wait();
-  const int len = table_len(kv_lens, b, page_size, max_pages,
-                            blockIdx.x == 0 && hkv == 0 && threadIdx.x == 0);
-  const int count = (int)(((long long)len + page_size - 1) / page_size);
-  const int p0 = blockIdx.x * kScorePages + warp * 32;  // this warp's first page
-  if ((int)(blockIdx.x * kScorePages) >= count) return;
-  int mine = p0 + lane < count ? block_table[(size_t)b * max_pages + p0 + lane] : 0;
-  if (mine < 0 || mine >= num_pages) {
-    atomicOr(&g_error_flags, 2u);  // page number out of range: page 0's bounds instead
-    mine = 0;
-  }
+  const int G = a.G;
+  // this warp's next 32 pages, one a lane
+  auto lookup = [&](int p0) {
+    int page = p0 + lane < last ? a.block_table[(size_t)b * a.max_pages + p0 + lane] : 0;
+    if (page < 0 || page >= a.num_pages) {
+      atomicOr(&g_error_flags, 2u);  // page number out of range: page 0's bounds instead
+      page = 0;
+    }
+    return page;
+  };
+  int mine = lookup(first + warp * 32);
   if (warp < GP) {  // a warp a head; heads past the group's are zeros
     const int g = warp;
     float v[D / 32], top = 0.f;
     bool ok = true;
-    const T1* qp = static_cast<const T1*>(q) + b * q_b + (long long)(hkv * G + min(g, G - 1)) * q_h;
+    const T1* qp =
+        static_cast<const T1*>(a.q) + b * a.q_b + (long long)(hkv * G + min(g, G - 1)) * a.q_h;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       v[i] = (float)qp[lane + 32 * i];
@@ -109,54 +117,73 @@ __global__ void __launch_bounds__(32 * kScoreWarps)
   const int head = sub & (GP - 1);
   const float qs = s_scale[head];
   const bool real = head < G;
+  for (int p0 = first + warp * 32; p0 < last; p0 += kScorePages) {
+    const int next = p0 + kScorePages < last ? lookup(p0 + kScorePages) : 0;
 #pragma unroll 4
-  for (int it = 0; it < 8; ++it) {
-    const int p = p0 + 4 * it + (lane >> 3);
-    const int page = __shfl_sync(0xffffffffu, mine, 4 * it + (lane >> 3));
-    const size_t row = (size_t)page * Hkv + hkv;
-    const float ps = index_scale[row];
-    int lo[W], hi[W];
-    if constexpr (W == 4) {
-      *reinterpret_cast<int4*>(lo) = reinterpret_cast<const int4*>(index + row * 2 * D)[sub];
-      *reinterpret_cast<int4*>(hi) = reinterpret_cast<const int4*>(index + row * 2 * D + D)[sub];
-    } else {
-      *reinterpret_cast<int2*>(lo) = reinterpret_cast<const int2*>(index + row * 2 * D)[sub];
-      *reinterpret_cast<int2*>(hi) = reinterpret_cast<const int2*>(index + row * 2 * D + D)[sub];
-    }
-    int dot[GP];
-#pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      dot[g] = 0;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        dot[g] = __dp4a(hi[i], qp[g][i], dot[g]);
-        dot[g] = __dp4a(lo[i], qn[g][i], dot[g]);
+    for (int it = 0; it < 8; ++it) {
+      const int p = p0 + 4 * it + (lane >> 3);
+      const int page = __shfl_sync(0xffffffffu, mine, 4 * it + (lane >> 3));
+      const size_t row = (size_t)page * a.Hkv + hkv;
+      const float ps = a.index_scale[row];
+      int lo[W], hi[W];
+      if constexpr (W == 4) {
+        *reinterpret_cast<int4*>(lo) = reinterpret_cast<const int4*>(a.index + row * 2 * D)[sub];
+        *reinterpret_cast<int4*>(hi) = reinterpret_cast<const int4*>(a.index + row * 2 * D + D)[sub];
+      } else {
+        *reinterpret_cast<int2*>(lo) = reinterpret_cast<const int2*>(a.index + row * 2 * D)[sub];
+        *reinterpret_cast<int2*>(hi) = reinterpret_cast<const int2*>(a.index + row * 2 * D + D)[sub];
       }
-    }
-    // lanes that differ in bit x keep the heads whose number agrees with theirs
+      int dot[GP];
 #pragma unroll
-    for (int x = 4, h = GP; x > 0; x >>= 1) {
-      if (h > x) {  // h == 2 x: hand over half the heads
+      for (int g = 0; g < GP; ++g) {
+        dot[g] = 0;
 #pragma unroll
-        for (int g = 0; g < GP / 2; ++g)
-          if (g < h / 2) {
-            const int keep = sub & x ? dot[g + h / 2] : dot[g];
-            const int give = sub & x ? dot[g] : dot[g + h / 2];
-            dot[g] = keep + __shfl_xor_sync(0xffffffffu, give, x);
-          }
-        h /= 2;
-      } else {  // fewer heads than lanes: a plain sum
-#pragma unroll
-        for (int g = 0; g < GP; ++g)
-          if (g < h) dot[g] += __shfl_xor_sync(0xffffffffu, dot[g], x);
+        for (int i = 0; i < W; ++i) {
+          dot[g] = __dp4a(hi[i], qp[g][i], dot[g]);
+          dot[g] = __dp4a(lo[i], qn[g][i], dot[g]);
+        }
       }
-    }
-    float best = real ? __fmul_rn(__fmul_rn((float)dot[0], qs), ps) : -INFINITY;
-    if (isnan(best)) best = INFINITY;  // a page or query that is not finite is not hidden
+      // lanes that differ in bit x keep the heads whose number agrees with theirs
 #pragma unroll
-    for (int x = 1; x < GP; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
-    if (sub == 0 && p < count) keys[((size_t)b * Hkv + hkv) * max_pages + p] = order_key(best);
+      for (int x = 4, h = GP; x > 0; x >>= 1) {
+        if (h > x) {  // h == 2 x: hand over half the heads
+#pragma unroll
+          for (int g = 0; g < GP / 2; ++g)
+            if (g < h / 2) {
+              const int keep = sub & x ? dot[g + h / 2] : dot[g];
+              const int give = sub & x ? dot[g] : dot[g + h / 2];
+              dot[g] = keep + __shfl_xor_sync(0xffffffffu, give, x);
+            }
+          h /= 2;
+        } else {  // fewer heads than lanes: a plain sum
+#pragma unroll
+          for (int g = 0; g < GP; ++g)
+            if (g < h) dot[g] += __shfl_xor_sync(0xffffffffu, dot[g], x);
+        }
+      }
+      float best = real ? __fmul_rn(__fmul_rn((float)dot[0], qs), ps) : -INFINITY;
+      if (isnan(best)) best = INFINITY;  // a page or query that is not finite is not hidden
+#pragma unroll
+      for (int x = 1; x < GP; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
+      if (sub == 0 && p < last) keys[p] = order_key(best);
+    }
+    mine = next;
   }
+}
+
+template <int D, int GP, bool BF16>
+__global__ void __launch_bounds__(32 * kScoreWarps)
+    scores_kernel(ScoreArgs a, uint32_t* __restrict__ keys, int top_k) {
+  const int b = blockIdx.z, hkv = blockIdx.y;
+  pdl_trigger();
+  pdl_wait();
+  const int len = table_len(a.kv_lens, b, a.page_size, a.max_pages,
+                            blockIdx.x == 0 && hkv == 0 && threadIdx.x == 0);
+  const int count = (int)(((long long)len + a.page_size - 1) / a.page_size);
+  const int first = blockIdx.x * kScorePages;
+  if (first >= count || count <= top_k) return;  // all pages are taken: no score needed
+  score_pages<D, GP, BF16>(a, b, hkv, first, min(count, first + kScorePages),
+                           keys + ((size_t)b * a.Hkv + hkv) * a.max_pages);
 }
 
 // The top_k pages, ties to the lowest page, in ascending order.  The last page
@@ -168,20 +195,11 @@ __global__ void __launch_bounds__(32 * kScoreWarps)
 // registers costs a compare and an add each (three candidates and half the
 // passes cost more: 27 us against 8192 keys on one SM).
 template <int THREADS, int KPT>
-__global__ void __launch_bounds__(THREADS)
-    select_kernel(const uint32_t* __restrict__ keys, const int32_t* __restrict__ kv_lens,
-                  int32_t* __restrict__ pages, int Hkv, int page_size, int max_pages, int top_k) {
+__device__ __forceinline__ void select_top(const uint32_t* kp, int all, int32_t* out, int top_k) {
   constexpr int NW = THREADS / 32;
   __shared__ int2 s_cnt[2][NW];
   __shared__ uint32_t s_at[KPT][NW];
-  const int hkv = blockIdx.x, b = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
-  pdl_wait();
-  const int len = table_len(kv_lens, b, page_size, max_pages, false);
-  const int all = (int)(((long long)len + page_size - 1) / page_size);
-  const uint32_t* kp = keys + ((size_t)b * Hkv + hkv) * max_pages;
-  int32_t* out = pages + ((size_t)b * Hkv + hkv) * top_k;
   if (all <= top_k) {
     for (int i = threadIdx.x; i < top_k; i += THREADS) out[i] = i < all ? i : -1;
     return;
@@ -302,6 +320,40 @@ __global__ void __launch_bounds__(THREADS)
     base += gt_all + min(eq_all, ties - seen);
     seen = min(seen + eq_all, ties);
   }
+}
+
+template <int THREADS, int KPT>
+__global__ void __launch_bounds__(THREADS)
+    select_kernel(const uint32_t* __restrict__ keys, const int32_t* __restrict__ kv_lens,
+                  int32_t* __restrict__ pages, int Hkv, int page_size, int max_pages, int top_k) {
+  const int hkv = blockIdx.x, b = blockIdx.y;
+  pdl_trigger();
+  pdl_wait();
+  const int len = table_len(kv_lens, b, page_size, max_pages, false);
+  const size_t tile = (size_t)b * Hkv + hkv;
+  select_top<THREADS, KPT>(keys + tile * max_pages,
+                           (int)(((long long)len + page_size - 1) / page_size),
+                           pages + tile * top_k, top_k);
+}
+
+// Scores and selection of tables of up to kFusedPages pages in one CTA, the keys
+// in shared memory: one launch and no trip through memory.
+constexpr int kFusedPages = 2048;
+template <int D, int GP, bool BF16>
+__global__ void __launch_bounds__(32 * kScoreWarps)
+    score_select_kernel(ScoreArgs a, int32_t* __restrict__ pages, int top_k) {
+  __shared__ uint32_t s_keys[kFusedPages];
+  const int hkv = blockIdx.x, b = blockIdx.y;
+  pdl_trigger();
+  pdl_wait();
+  const int len = table_len(a.kv_lens, b, a.page_size, a.max_pages, hkv == 0 && threadIdx.x == 0);
+  const int count = (int)(((long long)len + a.page_size - 1) / a.page_size);
+  if (count > top_k) {
+    score_pages<D, GP, BF16>(a, b, hkv, 0, count, s_keys);
+    __syncthreads();
+  }
+  select_top<32 * kScoreWarps, kFusedPages / (32 * kScoreWarps)>(
+      s_keys, count, pages + ((size_t)b * a.Hkv + hkv) * top_k, top_k);
 }
 
 // ------------------------------------------------------------------- attention
@@ -1069,28 +1121,35 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
                         int Hkv, int D, int page_size, int max_pages, int num_pages, int top_k,
                         int dtype, cudaStream_t stream) {
   using namespace kvq;
+  const int G = H / Hkv;
+  const ScoreArgs a{q,       q_b, q_h, index,     index_scale, block_table,
+                    kv_lens, G,   Hkv, page_size, max_pages,   num_pages};
+  const bool bf = dtype == B2A_BF16;
+  const dim3 tiles((unsigned)Hkv, (unsigned)B);
+  cudaError_t e;
+#define B2A_KVQ_SCORES(KERNEL, GO)                                                      \
+  if (D == 64 && G <= 4) e = bf ? GO((KERNEL<64, 4, true>)) : GO((KERNEL<64, 4, false>)); \
+  else if (D == 64) e = bf ? GO((KERNEL<64, 8, true>)) : GO((KERNEL<64, 8, false>));      \
+  else if (G <= 4) e = bf ? GO((KERNEL<128, 4, true>)) : GO((KERNEL<128, 4, false>));     \
+  else e = bf ? GO((KERNEL<128, 8, true>)) : GO((KERNEL<128, 8, false>));
+  if (max_pages <= kFusedPages) {
+    auto go = [&](auto kern) {
+      return launch_pdl(kern, tiles, 32 * kScoreWarps, 0, stream, a, pages, top_k);
+    };
+    B2A_KVQ_SCORES(score_select_kernel, go)
+    if (e != cudaSuccess) return set_cuda_error(e, "page selection kernel launch");
+    return B2A_OK;
+  }
   const dim3 grid((unsigned)((max_pages + kScorePages - 1) / kScorePages), (unsigned)Hkv,
                   (unsigned)B);
-  const int G = H / Hkv;
   auto go = [&](auto kern) {
-    return launch_pdl(kern, grid, 32 * kScoreWarps, 0, stream, q, q_b, q_h, index, index_scale,
-                      block_table, kv_lens, keys, G, Hkv, page_size, max_pages, num_pages);
+    return launch_pdl(kern, grid, 32 * kScoreWarps, 0, stream, a, keys, top_k);
   };
-  const bool bf = dtype == B2A_BF16;
-  cudaError_t e;
-  if (D == 64 && G <= 4) e = bf ? go(scores_kernel<64, 4, true>) : go(scores_kernel<64, 4, false>);
-  else if (D == 64) e = bf ? go(scores_kernel<64, 8, true>) : go(scores_kernel<64, 8, false>);
-  else if (G <= 4) e = bf ? go(scores_kernel<128, 4, true>) : go(scores_kernel<128, 4, false>);
-  else e = bf ? go(scores_kernel<128, 8, true>) : go(scores_kernel<128, 8, false>);
+  B2A_KVQ_SCORES(scores_kernel, go)
+#undef B2A_KVQ_SCORES
   if (e != cudaSuccess) return set_cuda_error(e, "page score kernel launch");
-  const dim3 tiles((unsigned)Hkv, (unsigned)B);
-  // at most 8 keys a thread with 256 threads; longer tables take 1024 threads
-  if (max_pages <= 2048)
-    e = launch_pdl(select_kernel<256, 8>, tiles, 256, 0, stream, keys, kv_lens, pages, Hkv,
-                   page_size, max_pages, top_k);
-  else
-    e = launch_pdl(select_kernel<1024, 16>, tiles, 1024, 0, stream, keys, kv_lens, pages, Hkv,
-                   page_size, max_pages, top_k);
+  e = launch_pdl(select_kernel<1024, 16>, tiles, 1024, 0, stream, keys, kv_lens, pages, Hkv,
+                 page_size, max_pages, top_k);
   if (e != cudaSuccess) return set_cuda_error(e, "page selection kernel launch");
   return B2A_OK;
 }
