@@ -190,15 +190,17 @@ __global__ void __launch_bounds__(32 * kScoreWarps)
 // counts as +infinity: it and the top_k - 1 best of the others, unless top_k of
 // those are infinite themselves.  One CTA per (sequence, KV head); up to KPT
 // keys a thread stay in registers, more are read again at each pass.  The
-// smallest key that is taken is found bit by bit below the bits that all keys
-// share: a pass counts the keys at or above one candidate, which for keys in
-// registers costs a compare and an add each (three candidates and half the
-// passes cost more: 27 us against 8192 keys on one SM).
+// smallest key that is taken is found 8 bits at a time below the bits that all
+// keys share: a pass counts the keys that agree so far by their next 8 bits, in
+// shared memory, and one warp finds the digit.  (One bit a pass, by compares and
+// a block-wide sum: 32 us with the scores for 8192 pages.)
 template <int THREADS, int KPT>
 __device__ __forceinline__ void select_top(const uint32_t* kp, int all, int32_t* out, int top_k) {
   constexpr int NW = THREADS / 32;
-  __shared__ int2 s_cnt[2][NW];
+  __shared__ int2 s_cnt[NW];
   __shared__ uint32_t s_at[KPT][NW];
+  __shared__ __align__(16) int s_hist[256];
+  __shared__ int2 s_digit;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (all <= top_k) {
     for (int i = threadIdx.x; i < top_k; i += THREADS) out[i] = i < all ? i : -1;
@@ -207,62 +209,89 @@ __device__ __forceinline__ void select_top(const uint32_t* kp, int all, int32_t*
   const int count = all - 1;  // without the last page
   int want = top_k - 1;
   const bool held = count <= KPT * THREADS;
-  const int rounds = held ? (count + THREADS - 1) / THREADS : 0;  // keys a thread holds
-  uint32_t key[KPT];  // 0 (below every real key) behind the last
+  uint32_t key[KPT];
   uint32_t top = 0, low = 0xffffffffu;
+  auto each = [&](auto f) {  // every key of this thread
+    if (held) {
+#pragma unroll
+      for (int c = 0; c < KPT; ++c)
+        if (c * THREADS + (int)threadIdx.x < count) f(key[c]);
+    } else {
+      for (int i = threadIdx.x; i < count; i += THREADS) f(kp[i]);
+    }
+  };
   if (held) {
 #pragma unroll
     for (int c = 0; c < KPT; ++c) {
       const int i = c * THREADS + threadIdx.x;
       key[c] = i < count ? kp[i] : 0u;
-      top = max(top, key[c]);
-      if (i < count) low = min(low, key[c]);
-    }
-  } else {
-    for (int i = threadIdx.x; i < count; i += THREADS) {
-      top = max(top, kp[i]);
-      low = min(low, kp[i]);
     }
   }
-  int pass = 0;
-  auto buffer = [&]() { return pass++ & 1; };  // in turn: one barrier a pass is enough
+  each([&](uint32_t k) {
+    top = max(top, k);
+    low = min(low, k);
+  });
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  if (lane == 0) s_cnt[warp] = make_int2((int)top, (int)low);
+  __syncthreads();
   {
-    top = __reduce_max_sync(0xffffffffu, top);
-    low = __reduce_min_sync(0xffffffffu, low);
-    const int p = buffer();
-    if (lane == 0) s_cnt[p][warp] = make_int2((int)top, (int)low);
-    __syncthreads();
-    const int2 v = s_cnt[p][lane < NW ? lane : 0];
+    const int2 v = s_cnt[lane < NW ? lane : 0];
     top = __reduce_max_sync(0xffffffffu, (uint32_t)v.x);
     low = __reduce_min_sync(0xffffffffu, (uint32_t)v.y);
   }
-  auto at_least = [&](uint32_t x) {  // how many keys are >= x
-    int n = 0;
-    if (held) {
-#pragma unroll
-      for (int c = 0; c < KPT; ++c)
-        if (c < rounds) n += key[c] >= x;
-    } else {
-      for (int i = threadIdx.x; i < count; i += THREADS) n += kp[i] >= x;
-    }
-    n = __reduce_add_sync(0xffffffffu, n);
-    const int p = buffer();
-    if (lane == 0) s_cnt[p][warp].x = n;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, lane < NW ? s_cnt[p][lane].x : 0);
-  };
   const uint32_t infinite = order_key(INFINITY);
-  const int inf_keys = top >= infinite ? at_least(infinite) : 0;
+  int inf_keys = 0;
+  if (top >= infinite) {  // the same in every thread
+    each([&](uint32_t k) { inf_keys += k >= infinite; });
+    inf_keys = __reduce_add_sync(0xffffffffu, inf_keys);
+    __syncthreads();
+    if (lane == 0) s_cnt[warp].x = inf_keys;
+    __syncthreads();
+    inf_keys = __reduce_add_sync(0xffffffffu, lane < NW ? s_cnt[lane].x : 0);
+  }
   if (inf_keys >= top_k) want = top_k;
   else if (threadIdx.x == 0) out[want] = count;
   if (want == 0) return;
-  // t: the largest value that `want` keys reach
-  const int differ = 32 - __clz(top ^ low);  // bits below the shared ones
-  uint32_t t = differ == 32 ? 0u : top >> differ << differ;
-  for (int bit = differ - 1; bit >= 0; --bit)
-    if (at_least(t | 1u << bit) >= want) t |= 1u << bit;
-  // keys above t are all taken, of those equal to t the lowest pages
-  const int ties = want - (t == 0xffffffffu ? 0 : at_least(t + 1));
+  // t: the want-th largest key; ties: how many keys equal to it are taken
+  int ties = want, hi = 32 - __clz(top ^ low);  // bits above hi are settled
+  uint32_t t = hi == 32 ? 0u : top >> hi << hi;
+  while (hi > 0) {
+    const int bits = min(8, hi), lo = hi - bits;
+    for (int i = threadIdx.x; i < 256; i += THREADS) s_hist[i] = 0;
+    __syncthreads();
+    each([&](uint32_t k) {
+      if (((k ^ t) >> (hi - 1) >> 1) == 0) atomicAdd(&s_hist[(k >> lo) & ((1u << bits) - 1)], 1);
+    });
+    __syncthreads();
+    if (warp == 0) {  // lane l: digits 8 l .. 8 l + 7; sums from the top
+      int n[8], sum = 0;
+#pragma unroll
+      for (int d = 7; d >= 0; --d) n[d] = sum += s_hist[8 * lane + d];
+      int above = sum;  // keys of this lane's digits and all higher lanes'
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int y = __shfl_down_sync(0xffffffffu, above, x);
+        if (lane + x < 32) above += y;
+      }
+      above -= sum;  // of higher lanes alone
+      if (above < ties && above + sum >= ties) {  // one lane
+        int d = 7;
+#pragma unroll
+        for (int e = 7; e > 0; --e)
+          if (above + n[e] < ties) d = e - 1;
+        int over = above;  // keys with a higher digit
+#pragma unroll
+        for (int e = 1; e < 8; ++e)
+          if (e == d + 1) over += n[e];
+        s_digit = make_int2(8 * lane + d, over);
+      }
+    }
+    __syncthreads();
+    t |= (uint32_t)s_digit.x << lo;
+    ties -= s_digit.y;
+    hi = lo;
+  }
   if (held) {
     // above (low 16 bits) and equal of each warp's 32 pages, in page order
 #pragma unroll
@@ -308,11 +337,11 @@ __device__ __forceinline__ void select_top(const uint32_t* kp, int all, int32_t*
     const unsigned meq = __ballot_sync(0xffffffffu, eq), mgt = __ballot_sync(0xffffffffu, gt);
     const unsigned below = (1u << lane) - 1;
     __syncthreads();
-    if (lane == 0) s_cnt[0][warp] = make_int2(__popc(mgt), __popc(meq));
+    if (lane == 0) s_cnt[warp] = make_int2(__popc(mgt), __popc(meq));
     __syncthreads();
     int gt_at = __popc(mgt & below), eq_at = __popc(meq & below), gt_all = 0, eq_all = 0;
     for (int w = 0; w < NW; ++w) {
-      const int2 v = s_cnt[0][w];
+      const int2 v = s_cnt[w];
       if (w < warp) gt_at += v.x, eq_at += v.y;
       gt_all += v.x, eq_all += v.y;
     }

@@ -691,3 +691,23 @@ def test_captured_step_and_side_streams():
                 f.v[b][0, :, -1] = f.x[b, :, 0]
             check_attention(f, f.q, got[0], got[1], pages=got[2].cpu().numpy())
     assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,top", [(2048, 100), (2049, 100), (9000, 333), (16385, 16), (20000, 3000)], ids=str)
+def test_select_of_long_tables(count, top):
+    """Tables past the sizes at which the selection changes its form; many pages share bounds,
+    so that ties cross every boundary inside it."""
+    import b200attn
+    D, page, P = 64, 16, 97
+    rng = np.random.default_rng(count)
+    cache = b200attn.QuantCache.empty(P, page, 1, D, dtype=F16, index=True)
+    bounds = np.sort(rng.integers(-127, 128, cache.index.shape).astype(np.int8), axis=2)  # min <= max
+    cache.index.copy_(torch.from_numpy(bounds))
+    cache.index_scale.copy_(torch.from_numpy(rng.uniform(0.01, 1, (P, 1)).astype(np.float32)))
+    table = rng.integers(0, P, (1, count)).astype(np.int32)
+    kl = torch.tensor([count * page - 5], dtype=torch.int32, device="cuda")
+    q = torch.from_numpy(ora.seeded_normal((1, 3, D), 3)).half().cuda()
+    got = b200attn.select_pages(q, cache, torch.from_numpy(table).cuda(), kl, top)[0, 0].cpu().numpy()
+    idx, sc = cache.index.cpu().numpy()[table[0], 0], cache.index_scale.cpu().numpy()[table[0], 0]
+    np.testing.assert_array_equal(got, oq.select(np_of(q)[0], idx, sc, count, top))
