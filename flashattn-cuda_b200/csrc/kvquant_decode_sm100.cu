@@ -79,6 +79,27 @@ __device__ __forceinline__ void score_pages(const ScoreArgs& a, int b, int hkv, 
     return page;
   };
   int mine = lookup(first + warp * 32);
+  const int sub = lane & 7;
+  // NB page quadruples are in flight at a time, the first before the query is
+  // rounded; a slot is loaded again as soon as it is used.
+  constexpr int NB = GP == 8 && D == 128 ? 2 : 4;  // as many as registers hold
+  int lo[NB][W], hi[NB][W];
+  float ps[NB];
+  auto load = [&](int k, int pages, int it) {  // quadruple `it` of a warp's 32 pages into slot k
+    const int page = __shfl_sync(0xffffffffu, pages, 4 * it + (lane >> 3));
+    const size_t row = (size_t)page * a.Hkv + hkv;
+    ps[k] = a.index_scale[row];
+    const int8_t* at = a.index + row * 2 * D;
+    if constexpr (W == 4) {
+      *reinterpret_cast<int4*>(lo[k]) = reinterpret_cast<const int4*>(at)[sub];
+      *reinterpret_cast<int4*>(hi[k]) = reinterpret_cast<const int4*>(at + D)[sub];
+    } else {
+      *reinterpret_cast<int2*>(lo[k]) = reinterpret_cast<const int2*>(at)[sub];
+      *reinterpret_cast<int2*>(hi[k]) = reinterpret_cast<const int2*>(at + D)[sub];
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < NB; ++k) load(k, mine, k);
   if (warp < GP) {  // a warp a head; heads past the group's are zeros
     const int g = warp;
     float v[D / 32], top = 0.f;
@@ -104,7 +125,6 @@ __device__ __forceinline__ void score_pages(const ScoreArgs& a, int b, int hkv, 
     if (lane == 0) s_scale[g] = scale;
   }
   __syncthreads();
-  const int sub = lane & 7;
   int qp[GP][W], qn[GP][W];
 #pragma unroll
   for (int g = 0; g < GP; ++g)
@@ -119,30 +139,22 @@ __device__ __forceinline__ void score_pages(const ScoreArgs& a, int b, int hkv, 
   const bool real = head < G;
   for (int p0 = first + warp * 32; p0 < last; p0 += kScorePages) {
     const int next = p0 + kScorePages < last ? lookup(p0 + kScorePages) : 0;
-#pragma unroll 4
+#pragma unroll
     for (int it = 0; it < 8; ++it) {
-      const int p = p0 + 4 * it + (lane >> 3);
-      const int page = __shfl_sync(0xffffffffu, mine, 4 * it + (lane >> 3));
-      const size_t row = (size_t)page * a.Hkv + hkv;
-      const float ps = a.index_scale[row];
-      int lo[W], hi[W];
-      if constexpr (W == 4) {
-        *reinterpret_cast<int4*>(lo) = reinterpret_cast<const int4*>(a.index + row * 2 * D)[sub];
-        *reinterpret_cast<int4*>(hi) = reinterpret_cast<const int4*>(a.index + row * 2 * D + D)[sub];
-      } else {
-        *reinterpret_cast<int2*>(lo) = reinterpret_cast<const int2*>(a.index + row * 2 * D)[sub];
-        *reinterpret_cast<int2*>(hi) = reinterpret_cast<const int2*>(a.index + row * 2 * D + D)[sub];
-      }
+      const int p = p0 + 4 * it + (lane >> 3), k = it % NB;
       int dot[GP];
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
         dot[g] = 0;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          dot[g] = __dp4a(hi[i], qp[g][i], dot[g]);
-          dot[g] = __dp4a(lo[i], qn[g][i], dot[g]);
+          dot[g] = __dp4a(hi[k][i], qp[g][i], dot[g]);
+          dot[g] = __dp4a(lo[k][i], qn[g][i], dot[g]);
         }
       }
+      const float page_scale = ps[k];
+      if (it + NB < 8) load(k, mine, it + NB);
+      else if (p0 + kScorePages < last) load(k, next, it + NB - 8);
       // lanes that differ in bit x keep the heads whose number agrees with theirs
 #pragma unroll
       for (int x = 4, h = GP; x > 0; x >>= 1) {
@@ -161,7 +173,7 @@ __device__ __forceinline__ void score_pages(const ScoreArgs& a, int b, int hkv, 
             if (g < h) dot[g] += __shfl_xor_sync(0xffffffffu, dot[g], x);
         }
       }
-      float best = real ? __fmul_rn(__fmul_rn((float)dot[0], qs), ps) : -INFINITY;
+      float best = real ? __fmul_rn(__fmul_rn((float)dot[0], qs), page_scale) : -INFINITY;
       if (isnan(best)) best = INFINITY;  // a page or query that is not finite is not hidden
 #pragma unroll
       for (int x = 1; x < GP; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
@@ -172,8 +184,8 @@ __device__ __forceinline__ void score_pages(const ScoreArgs& a, int b, int hkv, 
 }
 
 template <int D, int GP, bool BF16>
-__global__ void __launch_bounds__(32 * kScoreWarps)
-    scores_kernel(ScoreArgs a, uint32_t* __restrict__ keys, int top_k) {
+__global__ void __launch_bounds__(32 * kScoreWarps, 2)
+    scores_kernel(const ScoreArgs a, uint32_t* __restrict__ keys, int top_k) {
   const int b = blockIdx.z, hkv = blockIdx.y;
   pdl_trigger();
   pdl_wait();
@@ -369,8 +381,8 @@ __global__ void __launch_bounds__(THREADS)
 // in shared memory: one launch and no trip through memory.
 constexpr int kFusedPages = 2048;
 template <int D, int GP, bool BF16>
-__global__ void __launch_bounds__(32 * kScoreWarps)
-    score_select_kernel(ScoreArgs a, int32_t* __restrict__ pages, int top_k) {
+__global__ void __launch_bounds__(32 * kScoreWarps, 2)
+    score_select_kernel(const ScoreArgs a, int32_t* __restrict__ pages, int top_k) {
   __shared__ uint32_t s_keys[kFusedPages];
   const int hkv = blockIdx.x, b = blockIdx.y;
   pdl_trigger();
