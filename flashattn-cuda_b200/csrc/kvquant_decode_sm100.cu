@@ -417,8 +417,16 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // Both products run on the tensor cores on the raw codes, and the (scale, min)
 // pairs are applied outside them in fp32:
 //   S[tok, h] = sum_g kscale[tok, g] (code . q)_g + kmin[tok, g] qsum[h, g]
-//   O[h, d]   = sum_tok (p vscale[tok, g]) code[tok, d] + sum_tok p vmin[tok, g]
-// so K is used exactly and p*vscale is the only value rounded to 16 bits.
+//   O[h, d]   = sum_tok (p vscale[tok, g]) (code[tok, d] - mid)
+//             + sum_tok p (vmin[tok, g] + mid vscale[tok, g])
+// so K is used exactly and p*vscale is the only value rounded to 16 bits.  mid, 8
+// or 128, centres the codes: the sums of the rounded p*vscale over a step come
+// from a matrix instruction on ones, and their products with mid are taken off the
+// accumulators step by step.  Without it O is a small difference of two large sums, which
+// costs the accumulators' last bits and weighs each rounding of p*vscale with a
+// code of 0..15 instead of -8..7 (error against 64 bits of fp16 outputs over
+// 16640 tokens 8.3e-4, with it 2.8e-4; 5% of the
+// time).
 //   Codes are not converted: a code c in the low mantissa bits of an fp16 with
 // zero exponent IS the subnormal c * 2^-24, which the tensor cores multiply
 // exactly, so unpacking is one mask a pair (and a shift by 8 every second one).
@@ -726,7 +734,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 
   // --------------------------------------------------------------------- state
   float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
-  float omin[NG][2];  // sum of p * vmin over this lane's tokens
+  float omin[NG][2];  // sum of p * (vmin + mid * vscale) over this lane's tokens
   float m[2], l[2];
   // value scales are multiplied by vmul = 2^(127 - vexp), vexp the biased
   // exponent of the largest so far
@@ -753,6 +761,10 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   const uint32_t par_lo = page_shift == 4 ? blk : 16 * NG * 4;
   const uint32_t par_hi = page_shift == 6 ? 32 * NG * 4 : page_shift == 5 ? blk : 2 * blk;
   const uint32_t v_off = ROW << page_shift, vp_off = (NG * 4) << page_shift;
+  // -mid as the accumulators hold codes: times 2^-24, of odd channels (4 bits) 16 times
+  constexpr float kMid = BITS == 4 ? 8.f : 128.f;
+  constexpr float kMidOdd = -128.f / 16777216.f, kMidEven = BITS == 4 ? kMidOdd / 16.f : kMidOdd;
+  constexpr uint32_t kOnes = 0x3c003c00u;
   const int tok = (g >> 1) + (g & 1) * 4;  // S row g is token `tok` of the slab, row g+8 8 later
   const int vtok = HALF ? tok + 8 * half : tok;  // the first token whose p this lane holds
 
@@ -914,6 +926,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     }
 
     // ---- O += V^T P
+    float psum[NG][4];  // sums of the rounded p * vscale over the step
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) psum[gr][0] = psum[gr][1] = psum[gr][2] = psum[gr][3] = 0.f;
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
       if (!FULL && nv[sl] == 0) continue;
@@ -925,15 +940,16 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const float2 pr = param<BF16>(vpar[sl][r][gr]);
-          const float w = pr.x * vmul;
-          omin[gr][0] = fmaf(s[sl][r][0], pr.y, omin[gr][0]);
-          omin[gr][1] = fmaf(s[sl][r][1], pr.y, omin[gr][1]);
+          const float w = pr.x * vmul, vmid = fmaf(pr.x, kMid, pr.y);
+          omin[gr][0] = fmaf(s[sl][r][0], vmid, omin[gr][0]);
+          omin[gr][1] = fmaf(s[sl][r][1], vmid, omin[gr][1]);
           pb[r] = movmatrix_trans(pack2_u32<false>(s[sl][r][0] * w, s[sl][r][1] * w));
         }
         if constexpr (HALF) {  // columns 0-3: tokens 0-7 of the slab, columns 4-7: tokens 8-15
           pb[1] = g >= 4 ? pb[0] : 0u;
           pb[0] = g >= 4 ? 0u : pb[0];
         }
+        mma16816(psum[gr], kOnes, kOnes, kOnes, kOnes, pb[0], pb[1]);
         if constexpr (BITS == 4) {
           const uint32_t wa = *reinterpret_cast<const uint32_t*>(vc + gr * 32);
           const uint32_t wb = *reinterpret_cast<const uint32_t*>(vc + gr * 32 + 4 * ROW);
@@ -964,6 +980,13 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         }
       }
     }
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[gr][k][e] = fmaf(psum[gr][e & 1], e < 2 ? kMidEven : kMidOdd, o[gr][k][e]);
   };
 
   // Write out what was gathered for (b, hkv): the answer where this warp had all
