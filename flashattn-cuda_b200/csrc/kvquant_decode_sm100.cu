@@ -496,6 +496,8 @@ __device__ __forceinline__ void unpack4(uint32_t x, uint32_t* r) {
   r[2] = x & 0x000f000fu;
   r[3] = x & 0x00f000f0u;
 }
+// two neighbours of an array as a pair, for the two-wide fp32 instructions
+__device__ __forceinline__ float2& pair(float* x) { return *reinterpret_cast<float2*>(x); }
 // 2^e as fp32, e clamped to the normal range
 __device__ __forceinline__ float pow2i(int e) {
   return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
@@ -733,7 +735,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   };
 
   // --------------------------------------------------------------------- state
-  float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
+  alignas(16) float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
   float omin[NG][2];  // sum of p * (vmin + mid * vscale) over this lane's tokens
   float m[2], l[2];
   // value scales are multiplied by vmul = 2^(127 - vexp), vexp the biased
@@ -774,7 +776,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     constexpr bool FULL = decltype(all)::value;
 
     // ---- S = K q^T
-    float s[SL][R][2];
+    alignas(16) float s[SL][R][2];
     uint32_t vpar[SL][R][NG];  // (scale, min) of V of this lane's rows
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     }
 
     // ---- online softmax, per head over the step's tokens
-    float alpha[2];
+    float alpha[2], nmu[2];
     bool moved = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -890,15 +892,19 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       alpha[h] = ex2_mufu(m[h] - mu);
       moved = moved || alpha[h] != 1.f;
       m[h] = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < SL * R; ++k) {
-        const float p = ex2_mufu(fmaf(s[k / R][k % R][h], sl2[h], -mu));
-        s[k / R][k % R][h] = p;
-        sum += p;
-      }
-      l[h] = l[h] * alpha[h] + sum;
+      nmu[h] = -mu;
     }
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < SL * R; ++k) {
+      float2& x = pair(s[k / R][k % R]);
+      x = ffma2(x, make_float2(sl2[0], sl2[1]), make_float2(nmu[0], nmu[1]));
+      x.x = ex2_mufu(x.x);
+      x.y = ex2_mufu(x.y);
+      sum = fadd2(sum, x);
+    }
+    l[0] = fmaf(l[0], alpha[0], sum.x);
+    l[1] = fmaf(l[1], alpha[1], sum.y);
     T2 big = *reinterpret_cast<T2*>(&vpar[0][0][0]);  // largest value scale, in .x
 #pragma unroll
     for (int k = 1; k < SL * R * NG; ++k)
@@ -920,13 +926,13 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         omin[gr][1] *= alpha[1];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[gr][k][e] *= ao[e & 1];
+          for (int e = 0; e < 4; e += 2)
+            pair(&o[gr][k][e]) = fmul2(pair(&o[gr][k][e]), make_float2(ao[0], ao[1]));
       }
     }
 
     // ---- O += V^T P
-    float psum[NG][4];  // sums of the rounded p * vscale over the step
+    alignas(16) float psum[NG][4];  // sums of the rounded p * vscale over the step
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) psum[gr][0] = psum[gr][1] = psum[gr][2] = psum[gr][3] = 0.f;
 #pragma unroll
@@ -984,9 +990,10 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[gr][k][e] = fmaf(psum[gr][e & 1], e < 2 ? kMidEven : kMidOdd, o[gr][k][e]);
+        for (int e = 0; e < 4; e += 2)
+          pair(&o[gr][k][e]) = ffma2(pair(psum[gr]), e ? make_float2(kMidOdd, kMidOdd)
+                                                       : make_float2(kMidEven, kMidEven),
+                                     pair(&o[gr][k][e]));
   };
 
   // Write out what was gathered for (b, hkv): the answer where this warp had all
