@@ -50,26 +50,32 @@ def block_bytes(head_dim: int, page_size: int, bits: int) -> int:
     return n
 
 
+def _strides(*s):
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def _append_ct(k, v, data, index, index_scale, *rest):
+    return _lib.load().b2a_kvq_append_paged(k, v, _strides(*rest[13:16]), _strides(*rest[16:]),
+                                            data, index, index_scale, *rest[:13])
+
+
+def _read_ct(*args):
+    return _lib.load().b2a_kvq_read_paged(*args)
+
+
+def _select_ct(q, *rest):
+    return _lib.load().b2a_kvq_select_pages(q, _strides(*rest[16:]), *rest[:16])
+
+
+def _decode_ct(q, *rest):
+    return _lib.load().b2a_kvq_decode_paged(q, _strides(*rest[19:21]), *rest[:18], rest[21],
+                                            rest[18])
+
+
+_append, _read, _select, _decode = _append_ct, _read_ct, _select_ct, _decode_ct
 if hasattr(_fastcall, "kvq_append"):  # the CPython binding: the same calls, cheaper to make
     _append, _read = _fastcall.kvq_append, _fastcall.kvq_read
     _select, _decode = _fastcall.kvq_select, _fastcall.kvq_decode
-else:
-    def _strides(*s):
-        return (ctypes.c_int64 * len(s))(*s)
-
-    def _append(k, v, data, index, index_scale, *rest):
-        return _lib.load().b2a_kvq_append_paged(k, v, _strides(*rest[13:16]), _strides(*rest[16:]),
-                                                data, index, index_scale, *rest[:13])
-
-    def _read(*args):
-        return _lib.load().b2a_kvq_read_paged(*args)
-
-    def _select(q, *rest):
-        return _lib.load().b2a_kvq_select_pages(q, _strides(*rest[16:]), *rest[:16])
-
-    def _decode(q, *rest):
-        return _lib.load().b2a_kvq_decode_paged(q, _strides(*rest[19:21]), *rest[:18], rest[21],
-                                                rest[18])
 
 
 class QuantCache:

@@ -711,3 +711,116 @@ def test_select_of_long_tables(count, top):
     got = b200attn.select_pages(q, cache, torch.from_numpy(table).cuda(), kl, top)[0, 0].cpu().numpy()
     idx, sc = cache.index.cpu().numpy()[table[0], 0], cache.index_scale.cpu().numpy()[table[0], 0]
     np.testing.assert_array_equal(got, oq.select(np_of(q)[0], idx, sc, count, top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("workers", [1, 2, 5, 64])
+def test_runs_over_many_sequences(workers, monkeypatch):
+    """Few warps, so that a run crosses long, short and empty sequences and all their heads,
+    and its page look-ups cross their ends."""
+    import b200attn
+    from b200attn import quantcache as qc
+    lens = [0, 700, 3, 0, 0, 64, 65, 1, 1500, 16, 17, 0, 130] + [5, 0, 33] * 9 + [400, 0]
+    f = Filled(len(lens), 2, 64, 16, 4, F16, lens, seed=107)
+    q = torch.from_numpy(ora.seeded_normal((len(lens), 6, 64), 109)).half().cuda()
+    lib = __import__("b200attn._lib", fromlist=["load"]).load()
+    monkeypatch.setattr(qc, "_plan", lambda B, H, Hkv, D, bits, most, splits: (
+        workers, lib.b2a_kvq_decode_workspace_floats(B, H, Hkv, D, workers)))
+    O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl)
+    check_attention(f, q, O, L)
+    # the same through page lists, some of whose sequences are empty
+    lists = np.full((len(lens), 2, 9), -1, np.int32)
+    for b, n in enumerate(lens):
+        for h in range(2):
+            got = np.random.default_rng(b).permutation(max(-(-n // 16), 1))[:9]
+            lists[b, h, :len(got)] = got
+    O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, pages=torch.from_numpy(lists).cuda())
+    check_attention(f, q, O, L, pages=lists)
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+def test_chained_steps_without_waiting():
+    """Forty serving steps back to back (append with advance, select, decode), whose kernels may
+    start before the one ahead has ended, give what the same steps give one by one."""
+    import b200attn
+    B, H, Hkv, D, page, n = 3, 8, 2, 128, 16, 40
+    xs = [torch.from_numpy(ora.seeded_normal((B, Hkv, 1, D), 400 + i)).bfloat16().cuda() for i in range(n)]
+    qs = [torch.from_numpy(ora.seeded_normal((B, H, D), 500 + i)).bfloat16().cuda() for i in range(n)]
+
+    def run(wait):
+        f = Filled(B, Hkv, D, page, 8, BF16, [500, 31, 7], seed=97, index=True, width=40)
+        # pages for what is appended: behind the pool's used ones
+        f.cache = b200attn.QuantCache.empty(200, page, Hkv, D, bits=8, dtype=BF16, index=True)
+        bt = torch.arange(3 * 40, dtype=torch.int32, device="cuda").view(3, 40)
+        kl = torch.zeros(B, dtype=torch.int32, device="cuda")
+        for b in range(B):
+            b200attn.append_paged_quant(f.k[b], f.v[b], f.cache, bt[b:b + 1], kl[b:b + 1])
+        outs = []
+        for x, q in zip(xs, qs):
+            b200attn.append_paged_quant(x, x, f.cache, bt, kl)
+            if wait:
+                torch.cuda.synchronize()
+            pages = b200attn.select_pages(q, f.cache, bt, kl, 6)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(b200attn.decode_paged_quant(q, f.cache, bt, kl, pages=pages) + [pages])
+            if wait:
+                torch.cuda.synchronize()
+        assert kl.tolist() == [500 + n, 31 + n, 7 + n]
+        return outs
+
+    for a, b in zip(run(False), run(True)):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_ctypes_and_cpython_bindings_agree(monkeypatch):
+    import b200attn
+    from b200attn import quantcache as qc
+    f = Filled(2, 2, 64, 16, 4, F16, [90, 40], seed=117, index=True)
+    q = torch.from_numpy(ora.seeded_normal((2, 4, 64), 119)).half().cuda()
+    x = torch.from_numpy(ora.seeded_normal((2, 2, 3, 64), 120)).half().cuda()
+    cu = torch.tensor([0, 90, 130], dtype=torch.int32, device="cuda")
+
+    def all_of():
+        b200attn.append_paged_quant(x, x, f.cache, f.btg, f.kl - 3, advance=False)
+        pages = b200attn.select_pages(q, f.cache, f.btg, f.kl, 2)
+        return (b200attn.read_paged_quant(f.cache, f.btg, cu, 130, 90) + [pages]
+                + b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, pages=pages, scale=0.5))
+
+    first = all_of()
+    for name in ("_append", "_read", "_select", "_decode"):
+        monkeypatch.setattr(qc, name, getattr(qc, name + "_ct"))
+    for a, b in zip(first, all_of()):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_value_nan_stays_in_its_channels():
+    """A NaN in one group of one token's V: those 64 channels of its KV head's outputs only."""
+    import b200attn
+    f = Filled(1, 2, 128, 16, 8, BF16, [130], seed=127)
+    v = f.v[0].clone()
+    v[0, 1, 77, 100] = float("nan")
+    b200attn.append_paged_quant(f.k[0], v, f.cache, f.btg, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    q = torch.from_numpy(ora.seeded_normal((1, 4, 128), 129)).bfloat16().cuda()
+    for splits in (1, 3):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        assert O[0, 2:, 64:].isnan().all() and torch.isfinite(O[0, 2:, :64]).all()
+        assert torch.isfinite(O[0, :2]).all() and torch.isfinite(L).all()
+
+
+@pytest.mark.gpu
+def test_queries_of_any_size():
+    """Query amplitudes over the type's range: they are scaled by powers of two inside."""
+    import b200attn
+    for dt, amps in ((F16, (1e-6, 1e-3, 1e3)), (BF16, (1e-30, 1e-9, 1e9, 1e25))):
+        f = Filled(1, 1, 64, 16, 8, dt, [200], seed=137)
+        for amp in amps:
+            q = (torch.from_numpy(ora.seeded_normal((1, 3, 64), 139)) * amp).to(dt).cuda()
+            q[0, 1] = 0
+            scale = 0.125 / amp
+            O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, scale=scale)
+            check_attention(f, q, O, L, scale=scale)
