@@ -1104,10 +1104,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 
 // One CTA of NW warps per (sequence, query head), for those whose KV head was
 // cut; it also writes the answer of empty sequences.  A partial whose l is -inf
-// has no token; a NaN goes through to O and L.  The partials' weights are made
-// first, one a thread; then each row is read as 16 bytes a lane, with eight
-// rows in flight a warp, so that a load's latency is paid a few times and not
-// once per partial.
+// has no token; a NaN goes through to O and L.  Rows are read as 16 bytes a lane,
+// eight in flight a warp, the first eight before their weights are known: two
+// loads' latencies in a row, and not one per partial.
 constexpr int kChunk = 512;  // weights held at a time
 template <int D, int NW, bool BF16>
 __global__ void __launch_bounds__(32 * NW)
@@ -1116,24 +1115,36 @@ __global__ void __launch_bounds__(32 * NW)
                    void* __restrict__ out, float* __restrict__ lse, int G, int Hkv) {
   using T1 = typename Elem<BF16>::T;
   constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
+  constexpr int STEP = NW * RPW;              // rows per round of the CTA
   __shared__ float s_w[kChunk], s_red[2][NW];
-  __shared__ float4 s_acc[NW * RPW][LPR];
+  __shared__ float4 s_acc[STEP][LPR];
   const size_t row = blockIdx.x;
   const int tile = blockIdx.x / G, h = blockIdx.x % G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
   pdl_wait();
-  if (kv_lens[tile / Hkv] <= 0) {
+  const int len = kv_lens[tile / Hkv];
+  const int2 who = reinterpret_cast<const int2*>(meta)[tile];  // first and last worker
+  if (len <= 0) {
     if (threadIdx.x < D) static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(0.f);
     if (threadIdx.x == 0 && lse != nullptr) lse[row] = -INFINITY;
     return;
   }
-  const int first = meta[2 * tile];
-  if (first < 0) return;  // one warp had all of it
-  const int S = meta[2 * tile + 1] - first + 1;
-  const size_t seg0 = (size_t)first + tile;
+  if (who.x < 0) return;  // one warp had all of it
+  const int S = who.y - who.x + 1;
+  const size_t seg0 = (size_t)who.x + tile;
   const float* lp = l_part + seg0 * G + h;  // partial s at s * G
   const float4* op = reinterpret_cast<const float4*>(o_part + (seg0 * G + h) * D);
+  const int sub = warp * RPW + lane / LPR, c = lane % LPR;
+  float4 v[8];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int s = s0 + k * STEP;
+      v[k] = s < S ? op[(size_t)s * G * LPR + c] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  load(sub);
   float M = -INFINITY;
   for (int s = threadIdx.x; s < S; s += 32 * NW) M = fmaxf(M, lp[(size_t)s * G]);
 #pragma unroll
@@ -1143,34 +1154,29 @@ __global__ void __launch_bounds__(32 * NW)
   M = s_red[0][0];
 #pragma unroll
   for (int w = 1; w < NW; ++w) M = fmaxf(M, s_red[0][w]);
-  const int sub = warp * RPW + lane / LPR, c = lane % LPR;
   float L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  static_assert(kChunk % (8 * STEP) == 0, "a batch of rows lies in one chunk");
   for (int c0 = 0; c0 < S; c0 += kChunk) {
     const int cn = min(kChunk, S - c0);
-    __syncthreads();
+    if (c0 > 0) __syncthreads();  // the previous chunk's weights are used
     for (int s = threadIdx.x; s < cn; s += 32 * NW) {
-      const float v = lp[(size_t)(c0 + s) * G];
-      const float w = v == -INFINITY ? 0.f : expf(v - M);
+      const float x = lp[(size_t)(c0 + s) * G];
+      const float w = x == -INFINITY ? 0.f : expf(x - M);
       s_w[s] = w;
       L += w;
     }
     __syncthreads();
-    for (int s0 = sub; s0 < cn; s0 += 8 * NW * RPW) {
-      float4 v[8];
-      float w[8];
+    for (int s0 = sub; s0 < cn; s0 += 8 * STEP) {
+      if (c0 + s0 != sub) load(c0 + s0);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int s = s0 + k * NW * RPW;
-        w[k] = s < cn ? s_w[s] : 0.f;
-        v[k] = s < cn ? op[(size_t)(c0 + s) * G * LPR + c] : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        acc.x = fmaf(w[k], v[k].x, acc.x);
-        acc.y = fmaf(w[k], v[k].y, acc.y);
-        acc.z = fmaf(w[k], v[k].z, acc.z);
-        acc.w = fmaf(w[k], v[k].w, acc.w);
+        const int s = s0 + k * STEP;
+        const float w = s < cn ? s_w[s] : 0.f;
+        acc.x = fmaf(w, v[k].x, acc.x);
+        acc.y = fmaf(w, v[k].y, acc.y);
+        acc.z = fmaf(w, v[k].z, acc.z);
+        acc.w = fmaf(w, v[k].w, acc.w);
       }
     }
   }
@@ -1185,8 +1191,7 @@ __global__ void __launch_bounds__(32 * NW)
   if (threadIdx.x < D) {
     float a = 0.f;
 #pragma unroll
-    for (int k = 0; k < NW * RPW; ++k)
-      a += reinterpret_cast<const float*>(s_acc[k])[threadIdx.x];
+    for (int k = 0; k < STEP; ++k) a += reinterpret_cast<const float*>(s_acc[k])[threadIdx.x];
     static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(L == 0.f ? 0.f : a / L);
   }
   if (threadIdx.x == 0 && lse != nullptr) lse[row] = L == 0.f ? -INFINITY : M + logf(L);
@@ -1247,7 +1252,7 @@ int kvq_decode_workers(int B, int Hkv, int D, int bits, long long max_tokens) {
 // [worker + tile][G][D] o, [worker + tile][G] l, [tile][2] first and last worker.
 int64_t kvq_decode_workspace_floats(int B, int H, int Hkv, int D, int workers) {
   const int64_t tiles = (int64_t)B * Hkv;
-  return (workers + tiles) * (H / Hkv) * (D + 1) + 2 * tiles;
+  return (workers + tiles) * (H / Hkv) * (D + 1) + 2 * tiles + 1;
 }
 
 template <int D, int BITS, bool BF16, bool HALF>
@@ -1271,7 +1276,7 @@ static int launch_kvq_decode(const void* q, int64_t q_b, int64_t q_h, const uint
   }
   const int64_t segs = (int64_t)workers + (int64_t)B * Hkv;
   float* l_part = ws + segs * G * D;
-  int* meta = reinterpret_cast<int*>(l_part + segs * G);
+  int* meta = reinterpret_cast<int*>(l_part + (segs * G + 1) / 2 * 2);  // pairs of ints
   cudaError_t e = launch_pdl(kern, dim3((workers + C::kWarps - 1) / C::kWarps), 32 * C::kWarps,
                              C::kSmem, stream, q, q_b, q_h, data, block_table, kv_lens, pages,
                              n_list, ws, l_part, meta, o, lse, B, G, Hkv, workers, page_shift,

@@ -128,31 +128,31 @@ __global__ void append_kernel(const void* __restrict__ k_new, const void* __rest
     }
     // The steps of K and V are worked out side by side: K's by the lower four
     // lanes of a group, V's by the upper four.
-    T2 ext[2] = {extremes(x[0]), extremes(x[1])};
+    const T2 ext[2] = {extremes(x[0]), extremes(x[1])};
     const bool upper = c & 4;
     const float2 e = Elem<BF16>::unpack(upper ? ext[1] : ext[0]);
     float low = e.x, step;
     if (finite(e.x) && finite(e.y)) step = group_step<BF16, BITS>(e.x, -e.y);
     else low = step = __int_as_float(0x7fc00000);  // a NaN or infinity: the group reads as NaN
     const float inv = step_inverse(step);
-    const float other_low = __shfl_xor_sync(0xffffffffu, low, 4);
-    const float other_step = __shfl_xor_sync(0xffffffffu, step, 4);
-    const float other_inv = __shfl_xor_sync(0xffffffffu, inv, 4);
+    const float other = __shfl_xor_sync(0xffffffffu, inv, 4);
     // lane 0 of a group writes K's pair, lane 4 V's
     if (live && (c & 3) == 0) *par = pack2_u32<BF16>(step, low);
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      const bool own = upper == (side == 1);
-      const float lo = own ? low : other_low;
-      uint2 w = encode8<BF16, BITS>(x[side], lo, own ? inv : other_inv);
-      if (isnan(lo)) w = make_uint2(0u, 0u);
+      const float iv = upper == (side == 1) ? inv : other;
+      const float lo = Elem<BF16>::unpack(ext[side]).x;
+      uint2 w = encode8<BF16, BITS>(x[side], lo, iv);
+      if (iv == 0.f) w = make_uint2(0u, 0u);  // no step, or none that is a number
       if (live) {
         uint8_t* dst = row + (side ? page_size * ROW : 0);
         if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(dst) = w.x;
         else *reinterpret_cast<uint2*>(dst) = w;
       }
-      if (side == 0 && index != nullptr)
-        bound(decode8<BF16, BITS>(w, own ? step : other_step, lo));
+      if (side == 0 && index != nullptr) {
+        const float k_step = __shfl_sync(0xffffffffu, step, lane & ~4);
+        bound(decode8<BF16, BITS>(w, k_step, __shfl_sync(0xffffffffu, low, lane & ~4)));
+      }
     }
     row += RPI * ROW;
     par += RPI * NG;

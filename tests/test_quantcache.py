@@ -103,7 +103,7 @@ def test_library_refuses_bad_formats_without_a_device():
     assert lib.b2a_kvq_decode_workers(1, 8, 128, 4, 16) == 8
     for B, n in ((1, 131072), (64, 32768), (1, 1 << 31)):
         assert 1 <= lib.b2a_kvq_decode_workers(B, 8, 128, 8, n) <= 65535
-    assert lib.b2a_kvq_decode_workspace_floats(2, 8, 2, 128, 5) == (5 + 4) * 4 * 129 + 8
+    assert lib.b2a_kvq_decode_workspace_floats(2, 8, 2, 128, 5) == (5 + 4) * 4 * 129 + 9
 
 
 def test_oracle_quantiser_keeps_within_half_a_step():
