@@ -442,10 +442,10 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // dealt to lanes so that a lane's operand is a run of codes as they lie in
 // memory.
 //   HALF (groups of up to 4 heads): the four spare columns hold the same heads
-// again, with the second half of the contraction in S and of the tokens in O.
-// A lane then keeps one token row instead of two, and the scores, exponentials
-// and products with the scales are done once each instead of half of them for
-// columns that nobody reads.
+// again; in S a lane takes the one or the other token row of its column, in O
+// they take the second half of the tokens.  A lane then keeps one token row
+// instead of two, and the scores, exponentials and products with the scales are
+// done once each instead of half of them for columns that nobody reads.
 template <int D, int BITS>
 struct DecCfg {
   static constexpr int kStep = 64;  // tokens per step
@@ -525,7 +525,6 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   constexpr int ROW = C::kRow, NG = C::kNG, S = C::kStages, STEP = C::kStep;
   constexpr int SL = STEP / 16;         // 16-token slabs per step
   constexpr int R = HALF ? 1 : 2;       // token rows of a slab per lane
-  constexpr int KG = HALF ? 1 : NG;     // channel groups whose scores a lane sums itself
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -666,12 +665,11 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   // ------------------------------------------------------------------ queries
   // B fragments of S: lane (g, t) holds its head's channels 64*grp + 16 t +
   // 0..15 in the order in which a K row's codes unpack, over 16 where those are
-  // 16 c.  Column g is head g; in HALF, head g & 3 with the contraction's half
-  // g >> 2 (group g >> 2, or the g >> 2'th 8 of the 16 channels).
-  const int half = t >> 1;                      // HALF: this lane's token row and half of S
+  // 16 c.  Column g is head g, in HALF head g & 3.
+  const int half = t >> 1;                      // HALF: this lane's token row, g or g + 8
   const int head0 = HALF ? 2 * (t & 1) : 2 * t;  // its heads: head0, head0 + 1
   uint32_t qb[NG * 4][2];
-  float qsum[KG][2], sl2[2];
+  float qsum[NG][2], sl2[2];
   auto load_q = [&]() {
     const int hq = HALF ? g & 3 : g;
     const T1* qp = static_cast<const T1*>(q) + b * q_b + (long long)(hkv * G + hq) * q_h + 16 * t;
@@ -695,16 +693,19 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int shift = 139 - (int)(__float_as_uint(top) >> 23);  // to [2^12, 2^13)
     const float mul = pow2i(shift);
-    float sum[NG][2];
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
-      sum[gr][0] = sum[gr][1] = 0.f;
+      float sum = 0.f;  // of a column's channels
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         f[gr][j] *= mul;
-        if (HALF && (NG == 2 ? gr : j / 8) != (g >> 2)) f[gr][j] = 0.f;
-        sum[gr][0] += f[gr][j];
+        sum += f[gr][j];
       }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= pow2i(-24);  // the codes' factor
+      qsum[gr][0] = __shfl_sync(0xffffffffu, sum, 8 * t);  // columns 2t, 2t + 1
+      qsum[gr][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (BITS == 4) {
@@ -717,17 +718,6 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
           qb[gr * 4 + k][1] = pack2_u32<false>(x[2], x[3]);
         }
       }
-    }
-    // sums of the codes' factors over each column's channels
-#pragma unroll
-    for (int gr = 0; gr < KG; ++gr) {
-      float x = sum[gr][0];
-      if constexpr (HALF && NG == 2) x += sum[1][0];  // the other group's are zeros
-      x += __shfl_xor_sync(0xffffffffu, x, 1);
-      x += __shfl_xor_sync(0xffffffffu, x, 2);
-      x *= pow2i(-24);
-      qsum[gr][0] = __shfl_sync(0xffffffffu, x, 8 * t);  // columns 2t, 2t + 1
-      qsum[gr][1] = __shfl_sync(0xffffffffu, x, 8 * t + 4);
     }
     const int e = 24 - min(max(shift, -126), 127);  // up to 139: in two steps
     // not 0: a masked score is -inf, whose product with it stays -inf
@@ -793,27 +783,21 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       }
       const uint8_t* kc = stage + (sl >> 1) * code_hi + (sl & 1) * code_lo + tok * ROW;
       const uint8_t* pp = stage + 2 * v_off + (sl >> 1) * par_hi + (sl & 1) * par_lo;
-      uint32_t kpar[2][KG];  // of rows g, g+8
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint8_t* kp = pp + (tok + 8 * r) * NG * 4;
-        if constexpr (KG == 2)
-          *reinterpret_cast<uint2*>(kpar[r]) = *reinterpret_cast<const uint2*>(kp);
-        else
-          kpar[r][0] = *reinterpret_cast<const uint32_t*>(kp + (HALF && NG == 2 ? 4 * half : 0));
-      }
+      uint32_t kpar[R][NG];  // of this lane's rows
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const uint8_t* vp = pp + vp_off + (vtok + 8 * r) * NG * 4;
-        if constexpr (NG == 2)
-          *reinterpret_cast<uint2*>(vpar[sl][r]) = *reinterpret_cast<const uint2*>(vp);
-        else
-          vpar[sl][r][0] = *reinterpret_cast<const uint32_t*>(vp);
+        const uint8_t* kp = pp + (vtok + 8 * r) * NG * 4;
+        if constexpr (NG == 2) {
+          *reinterpret_cast<uint2*>(kpar[r]) = *reinterpret_cast<const uint2*>(kp);
+          *reinterpret_cast<uint2*>(vpar[sl][r]) = *reinterpret_cast<const uint2*>(kp + vp_off);
+        } else {
+          kpar[r][0] = *reinterpret_cast<const uint32_t*>(kp);
+          vpar[sl][r][0] = *reinterpret_cast<const uint32_t*>(kp + vp_off);
+        }
       }
-      float part[2][2];  // rows g, g+8
-      float acc[4];
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
+        float acc[4];  // (row g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
         if constexpr (BITS == 4) {
           const uint2 x = *reinterpret_cast<const uint2*>(kc + gr * 32 + t * 8);
           const uint2 y = *reinterpret_cast<const uint2*>(kc + 8 * ROW + gr * 32 + t * 8);
@@ -822,10 +806,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
             uint32_t a[4], z[4];
             unpack4(w ? x.y : x.x, a);
             unpack4(w ? y.y : y.x, z);
-            if (w == 0 && (gr == 0 || !HALF))
-              mma16816_first(acc, a[0], z[0], a[1], z[1], qb[gr * 4][0], qb[gr * 4][1]);
-            else
-              mma16816(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2 * w][0], qb[gr * 4 + 2 * w][1]);
+            if (w == 0) mma16816_first(acc, a[0], z[0], a[1], z[1], qb[gr * 4][0], qb[gr * 4][1]);
+            else mma16816(acc, a[0], z[0], a[1], z[1], qb[gr * 4 + 2][0], qb[gr * 4 + 2][1]);
             mma16816(acc, a[2], z[2], a[3], z[3], qb[gr * 4 + 2 * w + 1][0],
                      qb[gr * 4 + 2 * w + 1][1]);
           }
@@ -837,34 +819,19 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
           for (int w = 0; w < 4; ++w) {
             const uint32_t a0 = __byte_perm(xs[w], 0, 0x4140), a1 = __byte_perm(ys[w], 0, 0x4140);
             const uint32_t a2 = __byte_perm(xs[w], 0, 0x4342), a3 = __byte_perm(ys[w], 0, 0x4342);
-            if (w == 0 && (gr == 0 || !HALF))
-              mma16816_first(acc, a0, a1, a2, a3, qb[gr * 4][0], qb[gr * 4][1]);
-            else
-              mma16816(acc, a0, a1, a2, a3, qb[gr * 4 + w][0], qb[gr * 4 + w][1]);
+            if (w == 0) mma16816_first(acc, a0, a1, a2, a3, qb[gr * 4][0], qb[gr * 4][1]);
+            else mma16816(acc, a0, a1, a2, a3, qb[gr * 4 + w][0], qb[gr * 4 + w][1]);
           }
         }
-        if (!HALF || gr == NG - 1) {
-          constexpr int last = KG - 1;
-          const int kg = HALF ? 0 : min(gr, last);
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float2 pr = param<BF16>(kpar[r][kg]);
+        for (int r = 0; r < R; ++r) {
+          const float2 pr = param<BF16>(kpar[r][gr]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float bias = pr.y * qsum[kg][h];
-              part[r][h] = fmaf(pr.x, acc[2 * r + h], HALF || gr == 0 ? bias : part[r][h] + bias);
-            }
+          for (int h = 0; h < 2; ++h) {
+            const float a = HALF ? (half ? acc[2 + h] : acc[h]) : acc[2 * r + h];
+            s[sl][r][h] = fmaf(pr.x, a, gr == 0 ? pr.y * qsum[gr][h]
+                                                : fmaf(pr.y, qsum[gr][h], s[sl][r][h]));
           }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (HALF) {  // the other half of this lane's row, for this half of the other
-          const float got = __shfl_xor_sync(0xffffffffu, half ? part[0][h] : part[1][h], 2);
-          s[sl][0][h] = (half ? part[1][h] : part[0][h]) + got;
-        } else {
-          s[sl][0][h] = part[0][h];
-          s[sl][R - 1][h] = part[1][h];
         }
       }
       // tokens past the end: whatever their slots hold is dropped here
