@@ -14,7 +14,6 @@
 namespace b2a {
 namespace kvq {
 
-constexpr int kMaxG = 8;  // query heads of one KV head
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kDrainNs = 100000000ull;  // 0.1 s
@@ -422,11 +421,11 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // so K is used exactly and p*vscale is the only value rounded to 16 bits.  mid, 8
 // or 128, centres the codes: the sums of the rounded p*vscale over a step come
 // from a matrix instruction on ones, and their products with mid are taken off the
-// accumulators step by step.  Without it O is a small difference of two large sums, which
-// costs the accumulators' last bits and weighs each rounding of p*vscale with a
-// code of 0..15 instead of -8..7 (error against 64 bits of fp16 outputs over
-// 16640 tokens 8.3e-4, with it 2.8e-4; 5% of the
-// time).
+// accumulators step by step.  Without it O is a small difference of two large sums,
+// which costs the accumulators' last bits and weighs each rounding of p*vscale with
+// a code of 0..15 instead of -8..7.  It takes 5% of the time, and the error of fp16
+// outputs over 16640 tokens falls from 8.3e-4 to 2.8e-4 (2.1e-4 is the rounding of
+// the result alone).
 //   Codes are not converted: a code c in the low mantissa bits of an fp16 with
 // zero exponent IS the subnormal c * 2^-24, which the tensor cores multiply
 // exactly, so unpacking is one mask a pair (and a shift by 8 every second one).
@@ -446,6 +445,18 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // they take the second half of the tokens.  A lane then keeps one token row
 // instead of two, and the scores, exponentials and products with the scales are
 // done once each instead of half of them for columns that nobody reads.
+//
+// What bounds it: at 4 bits and D = 128 a 16-token slab of one KV head is 2304
+// bytes and about 230 instructions, 88 of them the unpacking.  At 12 warps an SM
+// (two 9 KB stages a warp fill shared memory, O and the operands the registers)
+// the rate of instructions and not HBM is the limit: 64 ragged sequences of 8 KV
+// heads, 1285 MB of blocks, take 227 us at 1.8-1.97 GHz, 5.7 TB/s (6.45 TB/s is
+// the measured copy), and 263-269 us in a long run, where the power limit takes
+// the clock to 1.69 GHz.  At 8 bits, with twice the bytes an instruction, 32
+// sequences of 16384 tokens, 1141 MB, take 188 us, 6.1 TB/s.  32-token steps with
+// 16 warps an SM were slower (257 us: what a step costs besides its tokens), so
+// were K and V in separate halves of a stage (273 us: several small copies a page
+// where one does).
 template <int D, int BITS>
 struct DecCfg {
   static constexpr int kStep = 64;  // tokens per step
