@@ -23,6 +23,7 @@ reference has no KV cache; the decode math is its online softmax
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from typing import List, Optional
@@ -30,7 +31,7 @@ from typing import List, Optional
 import torch
 
 from . import _lib
-from .attention import _DT, _decode_q, _fastcall, _on_device, _ptr, _stream
+from .attention import _DT, _decode_q, _fastcall, _ptr, _stream
 from .kvcache import PagePool
 
 GROUP = 64  # channels that share one (scale, min)
@@ -160,16 +161,31 @@ def _check_table(cache: QuantCache, block_table: torch.Tensor, rows: torch.Tenso
     return shape
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_no_guard = contextlib.nullcontext()
+
+
+def _guard(device: torch.device):
+    """Device guard, nothing where `device` is current (these calls are a few microseconds)."""
+    return _no_guard if device.index == _current_device() else torch.cuda.device(device)
+
+
 def _rows_of(t: torch.Tensor, n: int):
     """t, or a copy where its rows are not contiguous or not 16-byte aligned, and the element
     strides of its first n dims; a dim of size 1 has stride 0."""
-    st = t.stride()
-    if st[-1] == 1 and not t.data_ptr() & 15:
-        st = [0 if k == 1 else s for k, s in zip(t.shape, st[:n])]
-        if not any(s & 7 for s in st):
-            return t, st
+    if not t.data_ptr() & 15:
+        shape = t.shape
+        if t.is_contiguous():
+            d = shape[-1]
+            if n == 2:
+                return t, (shape[1] * d, d)
+            return t, (shape[1] * shape[2] * d, shape[2] * d, d)
+        st = t.stride()
+        st = [0 if k == 1 else s for k, s in zip(shape, st)]
+        if st[n] == 1 and not any(s & 7 for s in st[:n]):
+            return t, st[:n]
     t = t.clone(memory_format=torch.contiguous_format)
-    return t, [0 if k == 1 else s for k, s in zip(t.shape, t.stride()[:n])]
+    return _rows_of(t, n)
 
 
 def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCache,
@@ -195,7 +211,7 @@ def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCac
         raise RuntimeError("block_table must have one row per sequence")
     if B == 0 or T == 0:
         return
-    with _on_device(dev):
+    with _guard(dev):
         kn, ks = _rows_of(k_new, 3)
         vn, vs = _rows_of(v_new, 3)
         _lib.check(_append(
@@ -227,10 +243,10 @@ def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: t
                     or t.device != dev):
                 raise RuntimeError("out must be two contiguous [total, Hkv, D] tensors of the "
                                    "cache's dtype on its device")
-    with _on_device(dev):
+    with _guard(dev):
         if out is None:
-            K = torch.empty(shape, dtype=cache.dtype, device=dev)
-            V = torch.empty(shape, dtype=cache.dtype, device=dev)
+            K = cache.data.new_empty(*shape, dtype=cache.dtype)
+            V = cache.data.new_empty(*shape, dtype=cache.dtype)
         if B > 0 and total > 0 and max_len > 0:
             _lib.check(_read(
                 cache.data.data_ptr(), block_table.data_ptr(), _ptr(start),
@@ -268,12 +284,11 @@ def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
     if rows != B:
         raise RuntimeError("block_table must have one row per sequence")
     dev, Hkv = cache.device, cache.num_kv_heads
-    with _on_device(dev):
-        pages = torch.empty((B, Hkv, int(top_k)), dtype=torch.int32, device=dev)
+    with _guard(dev):
+        pages = kv_lens.new_empty(B, Hkv, int(top_k))
         if B == 0:
             return pages
-        keys = (torch.empty(B * Hkv * max_pages, dtype=torch.int32, device=dev)
-                if max_pages > 2048 else None)
+        keys = kv_lens.new_empty(B * Hkv * max_pages) if max_pages > 2048 else None
         qc, qs = _rows_of(q3, 2)
         _lib.check(_select(
             qc.data_ptr(), cache.index.data_ptr(), cache.index_scale.data_ptr(),
@@ -313,9 +328,9 @@ def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Te
                 or pages.device != dev):
             raise RuntimeError("pages must be contiguous int32 [B, Hkv, n] on the cache's device")
         n_pages = shape[2]
-    with _on_device(dev):
-        O = q3.new_empty((B, H, D))
-        L = q3.new_empty((B, H), dtype=torch.float32)
+    with _guard(dev):
+        O = q3.new_empty(B, H, D)
+        L = q3.new_empty(B, H, dtype=torch.float32)
         if B > 0:
             workers, floats = _plan(B, H, Hkv, D, cache.bits,
                                     (n_pages or max_pages) * cache.page_size, splits)

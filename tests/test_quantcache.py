@@ -561,6 +561,12 @@ def test_strided_and_misaligned_inputs():
     odd = torch.zeros(2 * 8 * 64 + 1, dtype=F16, device="cuda")[1:].view(2, 8, 64)
     odd.copy_(q)
     assert torch.equal(want[0], b200attn.decode_paged_quant(odd, f.cache, f.btg, f.kl)[0])
+    one = torch.empty_strided((1, 8, 64), (13, 64, 1), dtype=F16, device="cuda")  # a stride nobody uses
+    one.copy_(q[:1])
+    assert torch.equal(want[0][:1], b200attn.decode_paged_quant(one, f.cache, f.btg[:1], f.kl[:1])[0])
+    wide = torch.zeros(2, 8, 64, 2, dtype=F16, device="cuda")[..., 0]             # rows not contiguous
+    wide.copy_(q)
+    assert torch.equal(want[0], b200attn.decode_paged_quant(wide, f.cache, f.btg, f.kl)[0])
     k = qkv[:, 8:10, None]
     a, b = f.cache.data.clone(), f.cache.data.clone()
     kl = f.kl.clone()
