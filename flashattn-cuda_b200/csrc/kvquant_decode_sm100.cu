@@ -211,7 +211,7 @@ __device__ __forceinline__ void select_top(const uint32_t* kp, int all, int32_t*
   __shared__ int2 s_cnt[NW];
   __shared__ uint32_t s_at[KPT][NW];
   __shared__ __align__(16) int s_hist[256];
-  __shared__ int2 s_digit;
+  __shared__ int4 s_digit;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (all <= top_k) {
     for (int i = threadIdx.x; i < top_k; i += THREADS) out[i] = i < all ? i : -1;
@@ -298,12 +298,22 @@ __device__ __forceinline__ void select_top(const uint32_t* kp, int all, int32_t*
 #pragma unroll
         for (int e = 1; e < 8; ++e)
           if (e == d + 1) over += n[e];
-        s_digit = make_int2(8 * lane + d, over);
+        int upto = 0;  // and with this one
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e == d) upto = above + n[e];
+        s_digit = make_int4(8 * lane + d, over, upto, 0);
       }
     }
     __syncthreads();
-    t |= (uint32_t)s_digit.x << lo;
-    ties -= s_digit.y;
+    const int4 found = s_digit;
+    t |= (uint32_t)found.x << lo;
+    if (found.z == ties) {  // the digit's keys are all taken: no further digit matters
+      --t;
+      ties = 0;
+      break;
+    }
+    ties -= found.y;
     hi = lo;
   }
   if (held) {
@@ -550,10 +560,10 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 
   // ------------------------------------------------------------ this warp's run
   long long total = 0;
-  for (int b0 = 0; b0 < B; b0 += 32) {
-    const int s = b0 + lane < B ? seq_steps(length(b0 + lane, worker == 0), n_list, page_shift) : 0;
-    total += __reduce_add_sync(0xffffffffu, (unsigned)s);
-  }
+#pragma unroll 4
+  for (int k = lane; k < B; k += 32) total += seq_steps(length(k, worker == 0), n_list, page_shift);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
   total *= Hkv;
   const long long per = (total + workers - 1) / workers;
   const long long u0 = worker * per;
@@ -613,12 +623,13 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         lf += ln;
         if (++lh == Hkv) {
           lh = 0;
-          do ln = seq_steps(length(++lb, false), n_list, page_shift);
+          do ln = ++lb < B ? seq_steps(length(lb, false), n_list, page_shift) : n + 1;
           while (ln == 0);
         }
       }
       int lp = ((j - lf) << np_shift) + (k & ((1 << np_shift) - 1));
-      if (n_list > 0)
+      if (lb >= B) lp = -1;  // only where the lengths change under the kernel
+      else if (n_list > 0)
         lp = lp < n_list ? pages[((size_t)lb * Hkv + lh) * n_list + lp] : -1;
       if (lp >= 0 && lp < max_pages) {
         valid = min(max(length(lb, false) - (lp << page_shift), 0), page_size);
@@ -1061,8 +1072,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         i = i0 = 0;
         if (++hkv == Hkv) {
           hkv = 0;
-          do nst = seq_steps(length(++b, false), n_list, page_shift);
+          do nst = ++b < B ? seq_steps(length(b, false), n_list, page_shift) : 1;
           while (nst == 0);
+          if (b >= B) break;  // only where the lengths change under the kernel
         }
         load_q();
         reset();
