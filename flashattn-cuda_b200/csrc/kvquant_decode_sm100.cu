@@ -538,8 +538,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
                   const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ pages,
                   int n_list, float* __restrict__ o_part, float* __restrict__ l_part,
                   int* __restrict__ meta, void* __restrict__ out, float* __restrict__ lse, int B,
-                  int G, int Hkv, int workers, int page_shift, int max_pages, int num_pages,
-                  float scale_log2) {
+                  int G, int Hkv, int workers, int by_tile, int page_shift, int max_pages,
+                  int num_pages, float scale_log2) {
   using C = DecCfg<D, BITS>;
   using T1 = typename Elem<BF16>::T;
   using T2 = typename Elem<BF16>::T2;
@@ -568,6 +568,15 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   const long long per = (total + workers - 1) / workers;
   const long long u0 = worker * per;
   const int n = (int)max(0ll, min(per, total - u0));  // steps
+  // the answer of empty sequences, dealt over the warps
+  for (int k = worker; k < B; k += workers)
+    if (length(k, false) == 0) {
+      for (int x = lane; x < Hkv * G * D; x += 32)
+        static_cast<T1*>(out)[(size_t)k * Hkv * G * D + x] = Elem<BF16>::from(0.f);
+      for (int x = lane; x < Hkv * G && lse != nullptr; x += 32)
+        lse[(size_t)k * Hkv * G + x] = -INFINITY;
+    }
+  if (!by_tile && lane == 0) meta[2 * worker] = -1;
   if (n == 0) return;
   // its first (sequence, head, step)
   int b = 0, hkv = 0, i = 0, nst = 1;
@@ -989,7 +998,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 
   // Write out what was gathered for (b, hkv): the answer where this warp had all
   // of it, else a partial (o normalised, natural log l).
-  auto flush = [&](bool first, bool last) {
+  auto flush = [&](bool first, bool last, int next) {  // next: the step after, in this run
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -1035,8 +1044,13 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       }
     }
     if (lane == 0) {  // which workers hold partials of this (sequence, KV head)
-      if (first) meta[2 * tile] = whole ? -1 : worker;
-      if (last) meta[2 * tile + 1] = worker;
+      if (by_tile) {
+        if (first) meta[2 * tile] = whole ? -1 : worker;
+        if (last) meta[2 * tile + 1] = worker;
+      } else if (!whole) {
+        if (first) meta[2 * worker] = tile;
+        if (last) meta[2 * ((u0 + next - nst) / per) + 1] = worker;  // at the worker it began in
+      }
     }
   };
 
@@ -1067,7 +1081,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       }
     }
     if (++i == nst || j == n - 1) {
-      flush(i0 == 0, i == nst);
+      flush(i0 == 0, i == nst, j + 1);
       if (j < n - 1) {  // the next (sequence, KV head) with a step
         i = i0 = 0;
         if (++hkv == Hkv) {
@@ -1092,37 +1106,34 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   }
 }
 
-// One CTA of NW warps per (sequence, query head), for those whose KV head was
-// cut; it also writes the answer of empty sequences.  A partial whose l is -inf
-// has no token; a NaN goes through to O and L.  Rows are read as 16 bytes a lane,
-// eight in flight a warp, the first eight before their weights are known: two
-// loads' latencies in a row, and not one per partial.
+// One CTA of NW warps per query head of a (sequence, KV head) that was cut: the
+// CTAs go by (sequence, KV head), or, where those are many, by the worker in whose
+// run a cut one began, which are no more than the workers (1024 sequences of 512
+// tokens, 8 KV heads: 170 us by (sequence, KV head), 151 by worker).  A partial
+// whose l is -inf has no token; a NaN goes through to O and L.  Rows are read as 16
+// bytes a lane, eight in flight a warp, the first eight before their weights are
+// known: two loads' latencies in a row, and not one per partial.
 constexpr int kChunk = 512;  // weights held at a time
 template <int D, int NW, bool BF16>
 __global__ void __launch_bounds__(32 * NW)
     combine_kernel(const float* __restrict__ o_part, const float* __restrict__ l_part,
                    const int* __restrict__ meta, const int32_t* __restrict__ kv_lens,
-                   void* __restrict__ out, float* __restrict__ lse, int G, int Hkv) {
+                   void* __restrict__ out, float* __restrict__ lse, int G, int Hkv, int by_tile) {
   using T1 = typename Elem<BF16>::T;
   constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp
   constexpr int STEP = NW * RPW;              // rows per round of the CTA
   __shared__ float s_w[kChunk], s_red[2][NW];
   __shared__ float4 s_acc[STEP][LPR];
-  const size_t row = blockIdx.x;
-  const int tile = blockIdx.x / G, h = blockIdx.x % G;
+  const int at = blockIdx.x / G, h = blockIdx.x % G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
   pdl_wait();
-  const int len = kv_lens[tile / Hkv];
-  const int2 who = reinterpret_cast<const int2*>(meta)[tile];  // first and last worker
-  if (len <= 0) {
-    if (threadIdx.x < D) static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(0.f);
-    if (threadIdx.x == 0 && lse != nullptr) lse[row] = -INFINITY;
-    return;
-  }
-  if (who.x < 0) return;  // one warp had all of it
-  const int S = who.y - who.x + 1;
-  const size_t seg0 = (size_t)who.x + tile;
+  const int2 m = reinterpret_cast<const int2*>(meta)[at];
+  if (by_tile && kv_lens[at / Hkv] <= 0) return;  // no steps: meta was not written
+  if (m.x < 0) return;  // one warp had all of it, or none was cut
+  const int tile = by_tile ? at : m.x, first = by_tile ? m.x : at;
+  const int S = m.y - first + 1;
+  const size_t row = (size_t)tile * G + h, seg0 = (size_t)first + tile;
   const float* lp = l_part + seg0 * G + h;  // partial s at s * G
   const float4* op = reinterpret_cast<const float4*>(o_part + (seg0 * G + h) * D);
   const int sub = warp * RPW + lane / LPR, c = lane % LPR;
@@ -1239,10 +1250,12 @@ int kvq_decode_workers(int B, int Hkv, int D, int bits, long long max_tokens) {
 }
 
 // Partials: a worker's share of a (sequence, KV head) has number worker + tile.
-// [worker + tile][G][D] o, [worker + tile][G] l, [tile][2] first and last worker.
+// [worker + tile][G][D] o, [worker + tile][G] l, then pairs of ints: per tile its
+// first and last worker, or per worker the tile that began in it and was cut and
+// that tile's last worker.
 int64_t kvq_decode_workspace_floats(int B, int H, int Hkv, int D, int workers) {
   const int64_t tiles = (int64_t)B * Hkv;
-  return (workers + tiles) * (H / Hkv) * (D + 1) + 2 * tiles + 1;
+  return (workers + tiles) * (H / Hkv) * (D + 1) + 2 * (workers > tiles ? workers : tiles) + 1;
 }
 
 template <int D, int BITS, bool BF16, bool HALF>
@@ -1267,19 +1280,22 @@ static int launch_kvq_decode(const void* q, int64_t q_b, int64_t q_h, const uint
   const int64_t segs = (int64_t)workers + (int64_t)B * Hkv;
   float* l_part = ws + segs * G * D;
   int* meta = reinterpret_cast<int*>(l_part + (segs * G + 1) / 2 * 2);  // pairs of ints
+  const int64_t tiles = (int64_t)B * Hkv;
+  const int by_tile = tiles <= workers;
   cudaError_t e = launch_pdl(kern, dim3((workers + C::kWarps - 1) / C::kWarps), 32 * C::kWarps,
                              C::kSmem, stream, q, q_b, q_h, data, block_table, kv_lens, pages,
-                             n_list, ws, l_part, meta, o, lse, B, G, Hkv, workers, page_shift,
-                             max_pages, num_pages, scale * kLog2e);
+                             n_list, ws, l_part, meta, o, lse, B, G, Hkv, workers, by_tile,
+                             page_shift, max_pages, num_pages, scale * kLog2e);
   if (e != cudaSuccess) return set_cuda_error(e, "quantised decode kernel launch");
   // Few (sequence, KV head)s have many partials each: more warps for each.
-  // One sequence of 131072 tokens, 222 partials: 9 us with 4 warps.
-  if (workers > 32ll * B * Hkv)
-    e = launch_pdl(combine_kernel<D, 16, BF16>, dim3(B * G * Hkv), 512, 0, stream, ws, l_part,
-                   meta, kv_lens, o, lse, G, Hkv);
+  // One sequence of 131072 tokens, 205 partials: 9 us with 4 warps, 6 with 16.
+  if (workers > 32 * tiles)
+    e = launch_pdl(combine_kernel<D, 16, BF16>, dim3((unsigned)(tiles * G)), 512, 0, stream, ws,
+                   l_part, meta, kv_lens, o, lse, G, Hkv, by_tile);
   else
-    e = launch_pdl(combine_kernel<D, 4, BF16>, dim3(B * G * Hkv), 128, 0, stream, ws, l_part,
-                   meta, kv_lens, o, lse, G, Hkv);
+    e = launch_pdl(combine_kernel<D, 4, BF16>,
+                   dim3((unsigned)((by_tile ? tiles : (int64_t)workers) * G)), 128, 0, stream, ws,
+                   l_part, meta, kv_lens, o, lse, G, Hkv, by_tile);
   if (e != cudaSuccess) return set_cuda_error(e, "quantised decode combine launch");
   return B2A_OK;
 }

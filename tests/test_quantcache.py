@@ -103,7 +103,8 @@ def test_library_refuses_bad_formats_without_a_device():
     assert lib.b2a_kvq_decode_workers(1, 8, 128, 4, 16) == 8
     for B, n in ((1, 131072), (64, 32768), (1, 1 << 31)):
         assert 1 <= lib.b2a_kvq_decode_workers(B, 8, 128, 8, n) <= 65535
-    assert lib.b2a_kvq_decode_workspace_floats(2, 8, 2, 128, 5) == (5 + 4) * 4 * 129 + 9
+    assert lib.b2a_kvq_decode_workspace_floats(2, 8, 2, 128, 5) == (5 + 4) * 4 * 129 + 11
+    assert lib.b2a_kvq_decode_workspace_floats(2, 8, 2, 128, 3) == (3 + 4) * 4 * 129 + 9
 
 
 def test_oracle_quantiser_keeps_within_half_a_step():
@@ -830,3 +831,33 @@ def test_queries_of_any_size():
             scale = 0.125 / amp
             O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, scale=scale)
             check_attention(f, q, O, L, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+def test_many_sequences(dt):
+    """More (sequence, KV head)s than warps run at a time, empty sequences among them; and
+    more sequences than a warp looks at in one go."""
+    import b200attn
+    B, Hkv, D, page = 700, 4, 64, 16
+    rng = np.random.default_rng(3)
+    lens = rng.integers(0, 140, B)
+    lens[::7] = 0
+    bt, P = table_for(lens, page, rng)
+    cache = b200attn.QuantCache.empty(P, page, Hkv, D, bits=8, dtype=dt)
+    k, v = (torch.from_numpy(ora.seeded_normal((B, Hkv, 140, D), s)).to(dt).cuda() for s in (1, 2))
+    btg = torch.from_numpy(bt).cuda()
+    kl = torch.from_numpy(lens.astype(np.int32)).cuda()
+    q = torch.from_numpy(ora.seeded_normal((B, 8, D), 3)).to(dt).cuda()
+    for b in range(B):  # each sequence its own length
+        if lens[b]:
+            b200attn.append_paged_quant(k[b:b + 1, :, :lens[b]], v[b:b + 1, :, :lens[b]], cache, btg[b:b + 1],
+                                        torch.zeros(1, dtype=torch.int32, device="cuda"))
+    f = Filled.__new__(Filled)
+    f.cache, f.lens, f.page, f.bits, f.dt, f.name = cache, lens.tolist(), page, 8, dt, NAME[dt]
+    f.k = [k[b:b + 1, :, :lens[b]] for b in range(B)]
+    f.v = [v[b:b + 1, :, :lens[b]] for b in range(B)]
+    for splits in (None, 1):
+        O, L = b200attn.decode_paged_quant(q, cache, btg, kl, splits=splits)
+        check_attention(f, q, O, L)
+    assert b200attn.device_error_flags() == 0
