@@ -554,14 +554,27 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   if (worker >= workers) return;
   pdl_wait();
   const int page_size = 1 << page_shift;
-  auto length = [&](int b, bool flag) {
-    return table_len(kv_lens, b, page_size, max_pages, flag);
+  const long long cap = (long long)max_pages << page_shift;
+  auto length = [&](int b) {  // as the block table can hold it
+    const int len = kv_lens[b];
+    return len < 0 ? 0 : len > cap ? (int)cap : len;
   };
+  auto steps_of = [&](int b) { return b < B ? seq_steps(length(b), n_list, page_shift) : 0; };
+  if (worker == 0)
+    for (int k = lane; k < B; k += 32)
+      if (kv_lens[k] < 0 || kv_lens[k] > cap) atomicOr(&g_error_flags, 2u);
 
   // ------------------------------------------------------------ this warp's run
+  // Every warp adds up all lengths and finds its place among them, with loads in
+  // flight together: one chunk of 32 after the other, 2048 sequences took 18 us.
   long long total = 0;
-#pragma unroll 4
-  for (int k = lane; k < B; k += 32) total += seq_steps(length(k, worker == 0), n_list, page_shift);
+  for (int b0 = 0; b0 < B; b0 += 256) {
+    int s[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s[u] = steps_of(b0 + 32 * u + lane);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) total += s[u];
+  }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
   total *= Hkv;
@@ -570,7 +583,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   const int n = (int)max(0ll, min(per, total - u0));  // steps
   // the answer of empty sequences, dealt over the warps
   for (int k = worker; k < B; k += workers)
-    if (length(k, false) == 0) {
+    if (length(k) == 0) {
       for (int x = lane; x < Hkv * G * D; x += 32)
         static_cast<T1*>(out)[(size_t)k * Hkv * G * D + x] = Elem<BF16>::from(0.f);
       for (int x = lane; x < Hkv * G && lse != nullptr; x += 32)
@@ -581,28 +594,35 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   // its first (sequence, head, step)
   int b = 0, hkv = 0, i = 0, nst = 1;
   {
-    long long base = 0;  // steps of a head of the sequences before b0
-    for (int b0 = 0; b0 < B; b0 += 32) {
-      const int s = b0 + lane < B ? seq_steps(length(b0 + lane, false), n_list, page_shift) : 0;
-      int inc = s;
+    long long base = 0;  // steps of a head of the sequences before the chunk
+    bool found = false;
+    for (int b0 = 0; !found; b0 += 128) {  // ends: u0 < total
+      int s[4];
 #pragma unroll
-      for (int x = 1; x < 32; x <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, x);
-        if (lane >= x) inc += y;
+      for (int u = 0; u < 4; ++u) s[u] = steps_of(b0 + 32 * u + lane);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long long after = base + __reduce_add_sync(0xffffffffu, (unsigned)s[u]);
+        if (!found && after * Hkv > u0) {
+          found = true;
+          int inc = s[u];
+#pragma unroll
+          for (int x = 1; x < 32; x <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, x);
+            if (lane >= x) inc += y;
+          }
+          const int src = __ffs(__ballot_sync(0xffffffffu, (base + inc) * Hkv > u0)) - 1;
+          nst = __shfl_sync(0xffffffffu, s[u], src);
+          const long long rem = u0 - (base + __shfl_sync(0xffffffffu, inc, src) - nst) * Hkv;
+          b = b0 + 32 * u + src;
+          hkv = (int)(rem / nst);
+          i = (int)(rem % nst);
+        }
+        base = after;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, (base + inc) * Hkv > u0);
-      if (hit != 0) {
-        const int src = __ffs(hit) - 1;
-        nst = __shfl_sync(0xffffffffu, s, src);
-        base += __shfl_sync(0xffffffffu, inc, src) - nst;
-        const long long rem = u0 - base * Hkv;
-        b = b0 + src;
-        hkv = (int)(rem / nst);
-        i = (int)(rem % nst);
-        break;
-      }
-      base += __shfl_sync(0xffffffffu, inc, 31);
+      found = found || b0 >= B;  // only where the lengths change under the kernel
     }
+    if (b >= B) return;
   }
 
   // ---------------------------------------------------------------- the ring
@@ -632,7 +652,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         lf += ln;
         if (++lh == Hkv) {
           lh = 0;
-          do ln = ++lb < B ? seq_steps(length(lb, false), n_list, page_shift) : n + 1;
+          do ln = ++lb < B ? steps_of(lb) : n + 1;
           while (ln == 0);
         }
       }
@@ -641,7 +661,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       else if (n_list > 0)
         lp = lp < n_list ? pages[((size_t)lb * Hkv + lh) * n_list + lp] : -1;
       if (lp >= 0 && lp < max_pages) {
-        valid = min(max(length(lb, false) - (lp << page_shift), 0), page_size);
+        valid = min(max(length(lb) - (lp << page_shift), 0), page_size);
         if (valid > 0) {
           int page = block_table[(size_t)lb * max_pages + lp];
           if (page < 0 || page >= num_pages) {
@@ -1086,7 +1106,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         i = i0 = 0;
         if (++hkv == Hkv) {
           hkv = 0;
-          do nst = ++b < B ? seq_steps(length(b, false), n_list, page_shift) : 1;
+          do nst = ++b < B ? steps_of(b) : 1;
           while (nst == 0);
           if (b >= B) break;  // only where the lengths change under the kernel
         }
