@@ -439,10 +439,12 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 //   Codes are not converted: a code c in the low mantissa bits of an fp16 with
 // zero exponent IS the subnormal c * 2^-24, which the tensor cores multiply
 // exactly, so unpacking is one mask a pair (and a shift by 8 every second one).
-// Codes masked in place at bits 4-7 are 16 c * 2^-24; the 16 is taken out of q
-// (K) or of the finished channel (V).  Both cache dtypes use fp16 operands: a
-// query head is brought to [2^12, 2^13) by a power of two, and p*vscale to at
-// most 2 by a running one, so neither overflows nor loses bits that matter.
+// Codes masked in place at bits 4-7 are 16 c * 2^-24; the 16 is taken out of q (K),
+// or of the finished channel (V, whose odd channels sum whole bytes 16 c' + c and
+// lose the even neighbour's sum at the end: 227 -> 223 us below).  Both cache
+// dtypes use fp16 operands: a query head is brought to [2^12, 2^13) by a power of
+// two, and p*vscale to at most 2 by a running one, so neither overflows nor loses
+// bits that matter.
 //
 // The token dimension is M of both products (A = K codes [tok, d], and A =
 // V codes transposed [d, tok]) and the heads are N = 8, so no row of the
@@ -457,13 +459,14 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // done once each instead of half of them for columns that nobody reads.
 //
 // What bounds it: at 4 bits and D = 128 a 16-token slab of one KV head is 2304
-// bytes and about 230 instructions, 88 of them the unpacking.  At 12 warps an SM
+// bytes and about 225 instructions, 80 of them the unpacking.  At 12 warps an SM
 // (two 9 KB stages a warp fill shared memory, O and the operands the registers)
 // the rate of instructions and not HBM is the limit: 64 ragged sequences of 8 KV
-// heads, 1285 MB of blocks, take 227 us at 1.8-1.97 GHz, 5.7 TB/s (6.45 TB/s is
+// heads, 1285 MB of blocks, take 223 us at 1.8-1.97 GHz, 5.8 TB/s (6.45 TB/s is
 // the measured copy), and 263-269 us in a long run, where the power limit takes
 // the clock to 1.69 GHz.  At 8 bits, with twice the bytes an instruction, 32
-// sequences of 16384 tokens, 1141 MB, take 188 us, 6.1 TB/s.  32-token steps with
+// sequences of 16384 tokens, 1141 MB, take 188 us, 6.1 TB/s.  Warps alone on their
+// scheduler take 1.9 us a step and three together 2.9 each.  32-token steps with
 // 16 warps an SM were slower (257 us: what a step costs besides its tokens), so
 // were K and V in separate halves of a stage (273 us: several small copies a page
 // where one does).
@@ -516,6 +519,14 @@ __device__ __forceinline__ void unpack4(uint32_t x, uint32_t* r) {
   x >>= 8;
   r[2] = x & 0x000f000fu;
   r[3] = x & 0x00f000f0u;
+}
+// The same for V: r[0], r[2] hold c * 2^-24 and r[1], r[3] the whole byte, (16 c' +
+// c) * 2^-24, one operation less; the finished channel of c' is freed of c's.
+__device__ __forceinline__ void unpack4_bytes(uint32_t x, uint32_t* r) {
+  r[0] = x & 0x000f000fu;
+  r[1] = x & 0x00ff00ffu;
+  r[3] = __byte_perm(x, 0, 0x4341);
+  r[2] = r[3] & 0x000f000fu;
 }
 // two neighbours of an array as a pair, for the two-wide fp32 instructions
 __device__ __forceinline__ float2& pair(float* x) { return *reinterpret_cast<float2*>(x); }
@@ -806,9 +817,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   const uint32_t par_lo = page_shift == 4 ? blk : 16 * NG * 4;
   const uint32_t par_hi = page_shift == 6 ? 32 * NG * 4 : page_shift == 5 ? blk : 2 * blk;
   const uint32_t v_off = ROW << page_shift, vp_off = (NG * 4) << page_shift;
-  // -mid as the accumulators hold codes: times 2^-24, of odd channels (4 bits) 16 times
+  // -mid as the accumulators hold codes: times 2^-24, odd channels at 4 bits as bytes
   constexpr float kMid = BITS == 4 ? 8.f : 128.f;
-  constexpr float kMidOdd = -128.f / 16777216.f, kMidEven = BITS == 4 ? kMidOdd / 16.f : kMidOdd;
+  constexpr float kMidEven = -kMid / 16777216.f, kMidOdd = BITS == 4 ? 17.f * kMidEven : kMidEven;
   constexpr uint32_t kOnes = 0x3c003c00u;
   const int tok = (g >> 1) + (g & 1) * 4;  // S row g is token `tok` of the slab, row g+8 8 later
   const int vtok = HALF ? tok + 8 * half : tok;  // the first token whose p this lane holds
@@ -984,8 +995,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {  // channels 8g + 4*hf + 0..3
             uint32_t a[4], z[4];
-            unpack4(__byte_perm(wa, wb, hf ? 0x7632 : 0x5410), a);
-            unpack4(__byte_perm(wc, wd, hf ? 0x7632 : 0x5410), z);
+            unpack4_bytes(__byte_perm(wa, wb, hf ? 0x7632 : 0x5410), a);
+            unpack4_bytes(__byte_perm(wc, wd, hf ? 0x7632 : 0x5410), z);
             mma16816(o[gr][2 * hf], a[0], a[1], z[0], z[1], pb[0], pb[1]);
             mma16816(o[gr][2 * hf + 1], a[2], a[3], z[2], z[3], pb[0], pb[1]);
           }
@@ -1050,6 +1061,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
             x += __shfl_xor_sync(0xffffffffu, x, 2);
             y += __shfl_xor_sync(0xffffffffu, y, 2);
           }
+          if constexpr (BITS == 4) y -= x;  // bytes 16 c' + c: what is left is 16 c'
           x = fmaf(x * kEven, vscale, omin[gr][h]) * inv;
           y = fmaf(y * kOdd, vscale, omin[gr][h]) * inv;
           const size_t at = orow * D + gr * 64 + 8 * g + 2 * k;
