@@ -89,15 +89,16 @@ __device__ __forceinline__ float round_down(float x) {
 // (hi - lo) / n rounded up to dtype, so that n steps from lo reach hi; rounded
 // down where lo + n*step would leave the dtype's range.  Halves keep hi - lo
 // finite for any finite bf16.  Explicit roundings: the result is specified to
-// the bit.
+// the bit.  `down` says that it was rounded down.
 template <bool BF16, int BITS>
-__device__ __forceinline__ float group_step(float lo, float hi) {
+__device__ __forceinline__ float group_step(float lo, float hi, bool& down) {
   constexpr float n = (float)((1 << BITS) - 1);
   const float want = __fmul_rn(__fsub_rn(0.5f * hi, 0.5f * lo), 2.0f / n);
   // the least fp32 that rounds to infinity: max + half a last place
   constexpr float kPast = BF16 ? 3.3961775292304601e38f : 65520.f;
   float s = round_up<BF16>(want);
-  if (__fmaf_rn(n, s, lo) >= kPast) s = round_down<BF16>(want);
+  down = __fmaf_rn(n, s, lo) >= kPast;
+  if (down) s = round_down<BF16>(want);
   return s < kTinyStep ? 0.f : s;
 }
 
@@ -108,20 +109,23 @@ __device__ __forceinline__ float step_inverse(float step) {
 
 // Codes of 8 finite values of a group, min(rint((x/2 - lo/2) * inv), n): one
 // word at 4 bits, two at 8.  Adding 2^23 leaves the value, rounded to nearest
-// even, in the low mantissa bits.
-template <bool BF16, int BITS>
+// even, in the low mantissa bits.  Only a step that was rounded down needs the
+// minimum (CLAMP): any other is at least (hi - lo)/n less the 2^-22 of three fp32
+// roundings, so that the product is at most n (1 + 2^-21) and rounds to n.
+template <bool BF16, int BITS, bool CLAMP>
 __device__ __forceinline__ uint2 encode8(const Vec8<BF16>& x, float lo, float inv) {
   constexpr float n = (float)((1 << BITS) - 1);
   const float lo2 = 0.5f * lo;
   uint32_t c[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = Elem<BF16>::unpack(x.v[i]);
     // x/2 is exact, so the fused form rounds once as the difference does
-    c[2 * i] = __float_as_uint(
-        __fadd_rn(fminf(__fmul_rn(__fmaf_rn(f.x, 0.5f, -lo2), inv), n), 8388608.f));
-    c[2 * i + 1] = __float_as_uint(
-        __fadd_rn(fminf(__fmul_rn(__fmaf_rn(f.y, 0.5f, -lo2), inv), n), 8388608.f));
+    float2 f = ffma2(Elem<BF16>::unpack(x.v[i]), make_float2(0.5f, 0.5f), make_float2(-lo2, -lo2));
+    f = fmul2(f, make_float2(inv, inv));
+    if constexpr (CLAMP) f = make_float2(fminf(f.x, n), fminf(f.y, n));
+    // not as a pair: the product and the sum would be fused, which rounds once
+    c[2 * i] = __float_as_uint(__fadd_rn(f.x, 8388608.f));
+    c[2 * i + 1] = __float_as_uint(__fadd_rn(f.y, 8388608.f));
   }
   uint2 w = make_uint2(0u, 0u);
   if constexpr (BITS == 4) {

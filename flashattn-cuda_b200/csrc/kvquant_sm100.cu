@@ -14,8 +14,10 @@
 //
 // Both are copies.  Measured at D = 128, 4 bits: reading 16 sequences of 512 to
 // 16384 tokens of 8 KV heads back (709 MB read and written) 117 us, 94% of the
-// measured copy rate; appending 4 x 8192 bf16 tokens (172 MB) 43 us, 62%, where
-// some 265 instructions for every two rows of K and of V are the limit.
+// measured copy rate; appending 4 x 8192 bf16 tokens (172 MB) 40 us, 67%, where
+// the instructions, 240 or so for every two rows of K and of V, are the limit (41
+// with one value an instruction and every code clamped; 8 x 8192 fp16 tokens at 8
+// bits with an index: 94 -> 88 us).
 #include <type_traits>
 
 #include "kvquant.cuh"
@@ -139,8 +141,10 @@ __global__ void append_kernel(const void* __restrict__ k_new, const void* __rest
     const bool upper = c & 4;
     const float2 e = Elem<BF16>::unpack(upper ? ext[1] : ext[0]);
     float low = e.x, step;
-    if (finite(e.x) && finite(e.y)) step = group_step<BF16, BITS>(e.x, -e.y);
+    bool down = false;
+    if (finite(e.x) && finite(e.y)) step = group_step<BF16, BITS>(e.x, -e.y, down);
     else low = step = __int_as_float(0x7fc00000);  // a NaN or infinity: the group reads as NaN
+    const bool clamp = __any_sync(0xffffffffu, down);  // values next to the dtype's largest
     const float inv = step_inverse(step);
     const float other = __shfl_xor_sync(0xffffffffu, inv, 4);
     // lane 0 of a group writes K's pair, lane 4 V's
@@ -149,7 +153,8 @@ __global__ void append_kernel(const void* __restrict__ k_new, const void* __rest
     for (int side = 0; side < 2; ++side) {
       const float iv = upper == (side == 1) ? inv : other;
       const float lo = Elem<BF16>::unpack(ext[side]).x;
-      uint2 w = encode8<BF16, BITS>(x[side], lo, iv);
+      uint2 w = clamp ? encode8<BF16, BITS, true>(x[side], lo, iv)
+                      : encode8<BF16, BITS, false>(x[side], lo, iv);
       if (iv == 0.f) w = make_uint2(0u, 0u);  // no step, or none that is a number
       if (live) {
         uint8_t* dst = row + (side ? page_size * ROW : 0);
