@@ -318,9 +318,10 @@ int b2a_kvq_read_paged(const void* data, const int32_t* block_table,
  * score is the largest, over the group's heads, of
  * (sum_d max(q8*min8, q8*max8) * q_scale) * index_scale, with the sum exact
  * and each product rounded to fp32.  The last page of a sequence and any
- * score that is NaN count as +infinity; ties go to the lowest page.  q is [B,H,D] with element strides {batch, head}, multiples of 8;
- * H/Hkv <= 8.  keys is scratch of B*Hkv*max_pages words (not used, and may be
- * NULL, for max_pages <= 2048).
+ * score that is NaN count as +infinity; ties go to the lowest page.  q is
+ * [B,H,D] with element strides {batch, head}, multiples of 8; H/Hkv <= 8.  keys
+ * is scratch of B*Hkv*max_pages words (not used, and may be NULL, for
+ * max_pages <= 2048).
  */
 int b2a_kvq_select_pages(const void* q, const int64_t* q_strides,
                          const int8_t* index, const float* index_scale,

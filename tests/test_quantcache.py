@@ -4,8 +4,9 @@ selection and attention on the GPU against the numpy oracle.
 What the format specifies to the bit is compared to the bit.  Attention is held
 to a bound made of its roundings: with u = eps/2 of the dtype, O is rounded
 once (u |O|), and the attention kernel may round each probability times its
-value's step once (u sum_i p_i step_i code_i, plus, in fp16, half the smallest
-subnormal of a product scaled to at most 1 for every token); scores and sums are fp32.
+value's step once, which multiplies the code less the codes' middle (u sum_i p_i
+step_i |code_i - mid|, plus, in fp16, half the smallest subnormal of a product
+scaled to at most 1 for every token); scores and sums are fp32.
 """
 from __future__ import annotations
 
@@ -204,7 +205,11 @@ def check_attention(f, q, O, L, scale=None, pages=None):
             size = (np.abs(qn[b, heads]).astype(np.float64) @ np.abs(k).T * scale).max(-1, keepdims=True)
             fp32 = 2.0 ** -17 * (1 + size)
             sub = 2.0 ** -25 * len(use) * sc.max() * (2 ** f.bits - 1) / e.sum(-1, keepdims=True) * 2
-            tol = 1.01 * u * (np.abs(Or) + p @ (sc * c)) + fp32 * (p @ np.abs(v) + p @ (sc * c)) \
+            # p * scale is rounded and multiplies c - mid; mid's own share, p * scale * mid, is
+            # kept in fp32, so a rounding weighs |c - mid| and not c (which is less where the
+            # codes of a channel are all small, and more where they are large)
+            off = np.abs(c.astype(np.float64) - 2 ** (f.bits - 1))
+            tol = 1.01 * u * (np.abs(Or) + p @ (sc * off)) + fp32 * (p @ np.abs(v) + p @ (sc * c)) \
                 + (sub if f.dt == F16 else 0) + (2.0 ** -25 if f.dt == F16 else 0)
             bad = np.abs(On[b, heads] - Or) > tol
             assert not bad.any(), (b, h, np.abs(On[b, heads] - Or)[bad][:4], tol[bad][:4])
@@ -394,6 +399,19 @@ def test_decode_amplitudes(dt, amp):
     q = torch.from_numpy(ora.seeded_normal((2, 8, 128), 19)).to(dt).cuda()
     O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, scale=0.01)
     check_attention(f, q, O, L, scale=0.01)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,page,bits,G", [(128, 64, 4, 8), (64, 16, 8, 4), (128, 32, 8, 7)])
+def test_decode_of_a_few_tokens(D, page, bits, G):
+    """Sequences so short that a channel's codes may all be small: there the outputs' rounding
+    errors are those of codes less the middle."""
+    import b200attn
+    lens = [2, 3, 5, 1, 0, 4, 2, 64] * 4
+    f = Filled(len(lens), 3, D, page, bits, F16, lens, seed=97)
+    q = torch.from_numpy(ora.seeded_normal((len(lens), 3 * G, D), 99)).half().cuda()
+    O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl)
+    check_attention(f, q, O, L)
 
 
 @pytest.mark.gpu
