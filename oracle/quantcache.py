@@ -55,7 +55,8 @@ def quantise(x, bits: int, dtype: str):
         lo, hi = g.min(-1), g.max(-1)
         want = (hi * F32(0.5) - lo * F32(0.5)) * F32(2.0 / float(n))
         up, down = _toward(want, dtype, True), _toward(want, dtype, False)
-        past = np.isinf(round_to((n * up + lo).astype(F32), dtype))
+        # in 64 bits: n*up alone may pass fp32's largest where the sum does not
+        past = np.isinf(round_to((np.float64(n) * up + lo).astype(F32), dtype))
         scale = np.where(past, down, up).astype(F32)
         scale = np.where(scale < TINY, F32(0), scale)
         inv = F32(1) / (scale * F32(0.5))

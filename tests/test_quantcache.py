@@ -291,6 +291,33 @@ def test_append_of_extreme_values(dt, bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+def test_append_of_wide_ranges(dt, bits):
+    """Groups whose range passes the type's largest value (and in bf16 fp32's), from one side
+    and the other, beside groups of ordinary size in the same rows: which steps are rounded
+    down and which up, and the codes that go with them."""
+    import b200attn
+    big, T = torch.finfo(dt).max, 96
+    g = torch.Generator().manual_seed(3)
+    x = torch.rand(T, 128, generator=g, dtype=torch.float64) * 2 - 1
+    side = torch.linspace(0, 1, T, dtype=torch.float64)[:, None]
+    x = torch.where(x > 0, x * (1 - side), x * side) * big     # one bound at the largest or less
+    x[::3, 5], x[1::3, 9] = big, -big
+    x[::4, 64:] = torch.randn(T // 4, 64, generator=g, dtype=torch.float64)
+    x = x.to(dt)
+    cache = b200attn.QuantCache.empty(6, 16, 1, 128, bits=bits, dtype=dt, index=True)
+    bt = torch.arange(6, dtype=torch.int32, device="cuda")[None]
+    kl = torch.zeros(1, dtype=torch.int32, device="cuda")
+    xg = x[None, None].cuda()
+    b200attn.append_paged_quant(xg, xg.flip(2), cache, bt, kl)
+    got = oq.unpack(cache.data.cpu().numpy(), 16, 128, bits, NAME[dt])
+    for s, y in ((0, x), (1, x.flip(0))):
+        for a, w in zip(got[s], oq.quantise(np_of(y), bits, NAME[dt])):
+            np.testing.assert_array_equal(a.reshape(T, -1), w)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D,page,bits,dt", [(128, 16, 4, F16), (64, 32, 8, BF16), (64, 64, 4, F16),
                                             (128, 64, 8, F16), (128, 32, 4, BF16)], ids=str)
 def test_read_back(D, page, bits, dt):
