@@ -438,13 +438,17 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // the result alone).
 //   Codes are not converted: a code c in the low mantissa bits of an fp16 with
 // zero exponent IS the subnormal c * 2^-24, which the tensor cores multiply
-// exactly, so unpacking is one mask a pair (and a shift by 8 every second one).
-// Codes masked in place at bits 4-7 are 16 c * 2^-24; the 16 is taken out of q (K),
-// or of the finished channel (V, whose odd channels sum whole bytes 16 c' + c and
-// lose the even neighbour's sum at the end: 227 -> 223 us below).  Both cache
-// dtypes use fp16 operands: a query head is brought to [2^12, 2^13) by a power of
-// two, and p*vscale to at most 2 by a running one, so neither overflows nor loses
-// bits that matter.
+// exactly, so unpacking is one mask a pair (and a shift every second one).  Codes
+// masked where they lie are 4, 16 or 64 c * 2^-24; the factor is taken out of q
+// (K), or of the finished channel (V, whose odd channels sum whole bytes 16 c' + c
+// and lose the even neighbour's sum at the end: 4 us less below).  Where in the
+// mantissa a code lies matters to K's sums, whose last bits go by their operands'
+// exponents, a subnormal's being 2^-14: with K's codes at bits 2-5 and 6-9, not 0-3
+// and 4-7, lse of fp16 caches is off by 0.6e-7 of its size instead of 4e-7 (fp32
+// products: 0.4e-7), for another shift, 4 us below.  Both cache dtypes use fp16
+// operands: a query head is brought to [2^12, 2^13) by a power of two (over 64, a
+// channel is off by 2^-25 at most), and p*vscale to at most 2 by a running one, so
+// neither overflows nor loses bits that matter.
 //
 // The token dimension is M of both products (A = K codes [tok, d], and A =
 // V codes transposed [d, tok]) and the heads are N = 8, so no row of the
@@ -459,10 +463,10 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // done once each instead of half of them for columns that nobody reads.
 //
 // What bounds it: at 4 bits and D = 128 a 16-token slab of one KV head is 2304
-// bytes and about 225 instructions, 80 of them the unpacking.  At 12 warps an SM
+// bytes and about 230 instructions, 84 of them the unpacking.  At 12 warps an SM
 // (two 9 KB stages a warp fill shared memory, O and the operands the registers)
 // the rate of instructions and not HBM is the limit: 64 ragged sequences of 8 KV
-// heads, 1285 MB of blocks, take 223 us at 1.8-1.97 GHz, 5.8 TB/s (6.45 TB/s is
+// heads, 1285 MB of blocks, take 227 us at 1.8-1.97 GHz, 5.7 TB/s (6.45 TB/s is
 // the measured copy), and 263-269 us in a long run, where the power limit takes
 // the clock to 1.69 GHz.  At 8 bits, with twice the bytes an instruction, 32
 // sequences of 16384 tokens, 1141 MB, take 188 us, 6.1 TB/s.  Warps alone on their
@@ -512,16 +516,17 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   return d;
 }
 // The four 4-bit codes at bits 4j of each 16-bit half of x as pairs of fp16
-// subnormals: r[0], r[2] hold c * 2^-24, r[1], r[3] hold 16 c * 2^-24.
+// subnormals and small values: r[0], r[2] hold 4 c * 2^-24, r[1], r[3] 64 c * 2^-24.
 __device__ __forceinline__ void unpack4(uint32_t x, uint32_t* r) {
-  r[0] = x & 0x000f000fu;
-  r[1] = x & 0x00f000f0u;
-  x >>= 8;
-  r[2] = x & 0x000f000fu;
-  r[3] = x & 0x00f000f0u;
+  const uint32_t y = x << 2;
+  r[0] = y & 0x003c003cu;
+  r[1] = y & 0x03c003c0u;
+  x >>= 6;
+  r[2] = x & 0x003c003cu;
+  r[3] = x & 0x03c003c0u;
 }
-// The same for V: r[0], r[2] hold c * 2^-24 and r[1], r[3] the whole byte, (16 c' +
-// c) * 2^-24, one operation less; the finished channel of c' is freed of c's.
+// For V: r[0], r[2] hold c * 2^-24 and r[1], r[3] the whole byte, (16 c' + c) * 2^-24,
+// two operations less; the finished channel of c' is freed of c's.
 __device__ __forceinline__ void unpack4_bytes(uint32_t x, uint32_t* r) {
   r[0] = x & 0x000f000fu;
   r[1] = x & 0x00ff00ffu;
@@ -726,8 +731,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 
   // ------------------------------------------------------------------ queries
   // B fragments of S: lane (g, t) holds its head's channels 64*grp + 16 t +
-  // 0..15 in the order in which a K row's codes unpack, over 16 where those are
-  // 16 c.  Column g is head g, in HALF head g & 3.
+  // 0..15 in the order in which a K row's codes unpack, over 4 or 64 as those are
+  // 4 c or 64 c.  Column g is head g, in HALF head g & 3.
   const int half = t >> 1;                      // HALF: this lane's token row, g or g + 8
   const int head0 = HALF ? 2 * (t & 1) : 2 * t;  // its heads: head0, head0 + 1
   uint32_t qb[NG * 4][2];
@@ -772,8 +777,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       for (int k = 0; k < 4; ++k) {
         if constexpr (BITS == 4) {
           const float* x = &f[gr][8 * (k / 2) + 2 * (k & 1)];
-          qb[gr * 4 + k][0] = pack2_u32<false>(x[0], x[4]);
-          qb[gr * 4 + k][1] = pack2_u32<false>(x[1] * 0.0625f, x[5] * 0.0625f);
+          qb[gr * 4 + k][0] = pack2_u32<false>(x[0] * 0.25f, x[4] * 0.25f);
+          qb[gr * 4 + k][1] = pack2_u32<false>(x[1] * 0.015625f, x[5] * 0.015625f);
         } else {
           const float* x = &f[gr][4 * k];
           qb[gr * 4 + k][0] = pack2_u32<false>(x[0], x[1]);
