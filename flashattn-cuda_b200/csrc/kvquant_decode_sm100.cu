@@ -447,8 +447,13 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // and 4-7, lse of fp16 caches is off by 0.6e-7 of its size instead of 4e-7 (fp32
 // products: 0.4e-7), for another shift, 4 us below.  Both cache dtypes use fp16
 // operands: a query head is brought to [2^12, 2^13) by a power of two (over 64, a
-// channel is off by 2^-25 at most), and p*vscale to at most 2 by a running one, so
-// neither overflows nor loses bits that matter.
+// channel is off by 2^-25 at most), and p*vscale by a running factor of its own for
+// each head and group of channels, which at the last change brought the step's
+// largest product to [2^7, 2^8).  That goes by the products, so a token whose values
+// are large but that has no weight takes no bits from the others, and the factor
+// grows as the maximum does (o stays and its unit changes), so what is left of early
+// tokens takes none from later ones.  A product within 2^-21 of the largest keeps
+// fp16's 11 bits, one below is off by 2^-32 of the largest at most.
 //
 // The token dimension is M of both products (A = K codes [tok, d], and A =
 // V codes transposed [d, tok]) and the heads are N = 8, so no row of the
@@ -795,20 +800,20 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 
   // --------------------------------------------------------------------- state
   alignas(16) float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
-  float omin[NG][2];  // sum of p * (vmin + mid * vscale) over this lane's tokens
+  alignas(8) float omin[NG][2];  // sum of p * (vmin + mid * vscale) over this lane's tokens
   float m[2], l[2];
-  // value scales are multiplied by vmul = 2^(127 - vexp), vexp the biased
-  // exponent of the largest so far
-  int vexp;
-  float vmul;
+  // p * vscale of a head's group is multiplied by vmul before it is rounded; o
+  // holds sums of such products.  Value steps are 0 or 2^-100 and more.
+  alignas(8) float vmul[NG][2];
+  constexpr float kMaxMul = 1.298074214633707e33f;  // 2^110
+  constexpr float kMaxProduct = 32768.f;            // fp16 ends at 65504
   auto reset = [&]() {
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
-    vexp = 1;
-    vmul = pow2i(126);
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
       omin[gr][0] = omin[gr][1] = 0.f;
+      vmul[gr][0] = vmul[gr][1] = 1.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -926,7 +931,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       const float mn = fmaxf(m[h], mx * sl2[h]);
       const float mu = mn == -INFINITY ? 0.f : mn;
       alpha[h] = ex2_mufu(m[h] - mu);
-      moved = moved || alpha[h] != 1.f;
+      moved = moved || mn != m[h];
       m[h] = mn;
       nmu[h] = -mu;
     }
@@ -941,29 +946,55 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     }
     l[0] = fmaf(l[0], alpha[0], sum.x);
     l[1] = fmaf(l[1], alpha[1], sum.y);
-    T2 big = *reinterpret_cast<T2*>(&vpar[0][0][0]);  // largest value scale, in .x
+    // Where a maximum rises o stays, and vmul grows by what p of the tokens so far
+    // shrink by.  Products are bounded by their steps alone as long as that will do.
+    float vbig[NG];  // largest value step of this lane's tokens
+    bool look = moved;
 #pragma unroll
-    for (int k = 1; k < SL * R * NG; ++k)
-      big = __hmax2(big, *reinterpret_cast<T2*>(&vpar[k / (R * NG)][k / NG % R][k % NG]));
-    const float vbig = Elem<BF16>::unpack(big).x;
-    float f = 1.f;
-    if (__any_sync(0xffffffffu, vbig * vmul >= 2.f)) {
-      const int e = min((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vbig)) >> 23), 253);
-      f = pow2i(vexp - e);
-      moved = true;
-      vexp = e;
-      vmul = pow2i(127 - e);
+    for (int gr = 0; gr < NG; ++gr) {
+      T2 big = *reinterpret_cast<T2*>(&vpar[0][0][gr]);
+#pragma unroll
+      for (int k = 1; k < SL * R; ++k)
+        big = __hmax2(big, *reinterpret_cast<T2*>(&vpar[k / R][k % R][gr]));
+      vbig[gr] = Elem<BF16>::unpack(big).x;
+      look = look || vbig[gr] * fmaxf(vmul[gr][0], vmul[gr][1]) >= kMaxProduct;
     }
-    if (__any_sync(0xffffffffu, moved)) {
-      const float ao[2] = {alpha[0] * f, alpha[1] * f};
+    if (__any_sync(0xffffffffu, look)) {
+      bool over = false;
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
-        omin[gr][0] *= alpha[0];
-        omin[gr][1] *= alpha[1];
+      for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          for (int e = 0; e < 4; e += 2)
-            pair(&o[gr][k][e]) = fmul2(pair(&o[gr][k][e]), make_float2(ao[0], ao[1]));
+        for (int h = 0; h < 2; ++h) {
+          omin[gr][h] *= alpha[h];
+          vmul[gr][h] *= __fdividef(1.f, alpha[h]);  // infinite at a head's first token
+          over = over || vmul[gr][h] > kMaxMul || vbig[gr] * vmul[gr][h] >= kMaxProduct;
+        }
+      if (__any_sync(0xffffffffu, over)) {
+        // The products themselves: where one is too large for vmul, the step's
+        // largest goes to [2^7, 2^8).
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float f[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < SL * R; ++k)
+              top = fmaxf(top, s[k / R][k % R][h] * param<BF16>(vpar[k / R][k % R][gr]).x);
+#pragma unroll
+            for (int x = HALF ? 2 : 4; x < 32; x <<= 1)
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float old = vmul[gr][h];
+            const float fit = fminf(pow2i(134 - (int)(__float_as_uint(top) >> 23)), kMaxMul);
+            const bool fits = old <= kMaxMul && top * old < kMaxProduct;
+            f[h] = fits ? 1.f : __fdividef(fit, old);  // 0 for an infinite one
+            vmul[gr][h] = fits ? old : fit;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            for (int e = 0; e < 4; e += 2)
+              pair(&o[gr][k][e]) = fmul2(pair(&o[gr][k][e]), make_float2(f[0], f[1]));
+        }
       }
     }
 
@@ -982,10 +1013,12 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const float2 pr = param<BF16>(vpar[sl][r][gr]);
-          const float w = pr.x * vmul, vmid = fmaf(pr.x, kMid, pr.y);
+          const float vmid = fmaf(pr.x, kMid, pr.y);
           omin[gr][0] = fmaf(s[sl][r][0], vmid, omin[gr][0]);
           omin[gr][1] = fmaf(s[sl][r][1], vmid, omin[gr][1]);
-          pb[r] = movmatrix_trans(pack2_u32<false>(s[sl][r][0] * w, s[sl][r][1] * w));
+          // vmul last: vscale * vmul may pass fp32 where p is next to nothing
+          const float2 w = fmul2(make_float2(s[sl][r][0] * pr.x, s[sl][r][1] * pr.x), pair(vmul[gr]));
+          pb[r] = movmatrix_trans(pack2_u32<false>(w.x, w.y));
         }
         if constexpr (HALF) {  // columns 0-3: tokens 0-7 of the slab, columns 4-7: tokens 8-15
           pb[1] = g >= 4 ? pb[0] : 0u;
@@ -1045,7 +1078,6 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
           omin[gr][h] += __shfl_xor_sync(0xffffffffu, omin[gr][h], x);
       }
     }
-    const float vscale = pow2i(vexp - 127);
     constexpr float kEven = 16777216.f;  // 2^24: the codes' factor
     constexpr float kOdd = BITS == 4 ? 1048576.f : kEven;  // odd channels were 16 c
     const bool whole = first && last;
@@ -1058,7 +1090,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       const float ll = l[h] == 0.f ? -INFINITY : m[h] * kLn2 + logf(l[h]);
       const size_t orow = whole ? (size_t)b * Hkv * G + hkv * G + head : seg * G + head;
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
+      for (int gr = 0; gr < NG; ++gr) {
+        const float unit = __fdividef(1.f, vmul[gr][h]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float x = o[gr][k][h], y = o[gr][k][2 + h];
@@ -1067,14 +1100,15 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
             y += __shfl_xor_sync(0xffffffffu, y, 2);
           }
           if constexpr (BITS == 4) y -= x;  // bytes 16 c' + c: what is left is 16 c'
-          x = fmaf(x * kEven, vscale, omin[gr][h]) * inv;
-          y = fmaf(y * kOdd, vscale, omin[gr][h]) * inv;
+          x = fmaf(x * kEven, unit, omin[gr][h]) * inv;
+          y = fmaf(y * kOdd, unit, omin[gr][h]) * inv;
           const size_t at = orow * D + gr * 64 + 8 * g + 2 * k;
           if (head < G && (!HALF || (k >> 1) == half)) {
             if (whole) *reinterpret_cast<uint32_t*>(static_cast<T1*>(out) + at) = pack2_u32<BF16>(x, y);
             else *reinterpret_cast<float2*>(o_part + at) = make_float2(x, y);
           }
         }
+      }
       if (g == 0 && head < G && (!HALF || half == 0)) {
         if (!whole) l_part[orow] = ll;
         else if (lse != nullptr) lse[orow] = ll;

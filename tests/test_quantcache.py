@@ -906,3 +906,119 @@ def test_many_sequences(dt):
         O, L = b200attn.decode_paged_quant(q, cache, btg, kl, splits=splits)
         check_attention(f, q, O, L)
     assert b200attn.device_error_flags() == 0
+
+
+def check_own_steps(f, q, O, L):
+    """check_attention's bound with nothing in it that another token's or channel group's step
+    enters except by its weight.  A product p * step is rounded to fp16 in a unit that brings the
+    largest product of its head and group to 2^7 or more, so where it falls into the subnormals
+    half of their spacing is 2^-25 * 2^-7 of that largest product (and it multiplies |code - mid|,
+    at most 2^(bits - 1)).  A unit is at least 2^-110: with 2^-25, nothing beside 2^-133."""
+    u = torch.finfo(f.dt).eps / 2
+    Hkv = f.cache.num_kv_heads
+    G = q.shape[1] // Hkv
+    qn, On, Ln = np_of(q), np_of(O), L.cpu().numpy()
+    mid = 2 ** (f.bits - 1)
+    for b, n in enumerate(f.lens):
+        K, V = (f.codes(b, s) for s in (0, 1))
+        for h in range(Hkv):
+            heads = slice(h * G, (h + 1) * G)
+            k, v = oq.values(*(x[h] for x in K)), oq.values(*(x[h] for x in V))
+            Or, Lr = oq.attend(qn[b, heads], k, v, f.D ** -0.5)
+            s = qn[b, heads].astype(np.float64) @ k.T * f.D ** -0.5
+            p = np.exp(s - Lr[:, None])
+            sc, c = np.repeat(V[1][h].astype(np.float64), 64, -1), V[0][h].astype(np.float64)
+            most = (p[:, :, None] * sc).max(1)       # of each head and channel's group
+            fp32 = 2.0 ** -17 * (1 + (np.abs(qn[b, heads]).astype(np.float64) @ np.abs(k).T
+                                      * f.D ** -0.5).max(-1, keepdims=True))
+            tol = 1.01 * u * (np.abs(Or) + p @ (sc * np.abs(c - mid))) \
+                + fp32 * (p @ np.abs(v) + p @ (sc * c)) + 2.0 ** -32 * n * mid * most \
+                + (2.0 ** -25 if f.dt == F16 else 2.0 ** -133)
+            bad = ~(np.abs(On[b, heads] - Or) <= tol)
+            assert not bad.any(), (b, h, np.abs(On[b, heads] - Or)[bad][:4], tol[bad][:4])
+            assert (np.abs(Ln[b, heads] - Lr) <= fp32[:, 0] * 2).all()
+
+
+def with_values(f, v=None, k=None):
+    """Sequence 0 of f written again, with other values or keys."""
+    import b200attn
+    f.v[0], f.k[0] = f.v[0] if v is None else v, f.k[0] if k is None else k
+    b200attn.append_paged_quant(f.k[0], f.v[0], f.cache, f.btg,
+                                torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+RANGE = [(128, 4, F16, 4), (128, 8, BF16, 4), (128, 4, BF16, 8), (128, 8, F16, 6), (64, 4, BF16, 1),
+         (64, 8, F16, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,bits,dt,G", RANGE, ids=str)
+@pytest.mark.parametrize("at", [0, 300, 511])
+def test_a_large_value_without_weight(D, bits, dt, G, at):
+    """One token whose values are very much larger than all others' and whose score leaves it
+    next to no weight: the others' share of the output is as exact as without it."""
+    import b200attn
+    small, large = (0.02, 6e4) if dt == F16 else (0.1, 1e9)
+    f = Filled(1, 2, D, 16, bits, dt, [512], seed=207)
+    q = (0.5 + 0.3 * torch.from_numpy(ora.seeded_normal((1, 2 * G, D), 209))).to(dt).cuda()
+    k, v = f.k[0].clone(), (f.v[0].float() * small).to(dt)
+    k[0, :, at] = -160 / D ** 0.5                            # a score of about -80
+    v[0, :, at] = torch.linspace(-large, large, D).to(dt).cuda()
+    with_values(f, v, k)
+    for splits in (None, 1, 2, 5):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_own_steps(f, q, O, L)
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,bits,dt,G", RANGE, ids=str)
+@pytest.mark.parametrize("rise", [60.0, -60.0])
+def test_values_shrink_while_scores_rise(D, bits, dt, G, rise):
+    """Scores that rise by 60 along the sequence while the values shrink, and the other way round:
+    what counts at the end are the tokens of high score, however small their values are."""
+    import b200attn
+    n = 640
+    f = Filled(1, 2, D, 32, bits, dt, [n], seed=217)
+    q = (0.5 + 0.3 * torch.from_numpy(ora.seeded_normal((1, 2 * G, D), 219))).to(dt).cuda()
+    ramp = torch.linspace(0, 1, n)[None, None, :, None].cuda()
+    k = (0.2 * f.k[0].float() + 2 * rise * ramp / D ** 0.5).to(dt)
+    fall = ramp if rise > 0 else 1 - ramp
+    v = (f.v[0].float() * (3e3 * 10.0 ** (-6 * fall) if dt == F16 else 10.0 ** (9 - 18 * fall))).to(dt)
+    with_values(f, v, k)
+    for splits in (None, 1, 3):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_own_steps(f, q, O, L)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,dt,G", [(4, F16, 4), (8, F16, 8), (4, BF16, 8), (8, BF16, 3)], ids=str)
+@pytest.mark.parametrize("which", [0, 1])
+def test_channel_groups_of_unequal_size(bits, dt, G, which):
+    """One group of 64 channels whose values are a small part of the other's."""
+    import b200attn
+    f = Filled(1, 2, 128, 16, bits, dt, [700], seed=227)
+    q = torch.from_numpy(ora.seeded_normal((1, 2 * G, 128), 229)).to(dt).cuda()
+    size = torch.full((128,), 1e4 if dt == F16 else 1e3)
+    size[64 * which:64 * which + 64] = 1e-2 if dt == F16 else 1e-9
+    with_values(f, (f.v[0].float() * size.cuda()).to(dt))
+    for splits in (None, 1, 4):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_own_steps(f, q, O, L)
+
+
+@pytest.mark.gpu
+def test_values_of_zero_before_others():
+    """Tokens whose groups have no step at all while the scores rise, then tokens that have one."""
+    import b200attn
+    for dt, bits in ((F16, 4), (BF16, 8)):
+        f = Filled(1, 1, 64, 16, bits, dt, [512], seed=237)
+        q = (0.5 + 0.3 * torch.from_numpy(ora.seeded_normal((1, 4, 64), 239))).to(dt).cuda()
+        ramp = torch.linspace(0, 1, 512)[None, None, :, None].cuda()
+        k = (0.2 * f.k[0].float() + 2 * 200 * ramp / 8).to(dt)
+        v = f.v[0].clone()
+        v[:, :, :500] = 0
+        with_values(f, v, k)
+        for splits in (1, 2):
+            O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+            check_own_steps(f, q, O, L)
