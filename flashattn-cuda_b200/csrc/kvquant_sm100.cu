@@ -350,9 +350,12 @@ int kvq_read_dispatch(const void* data, const int32_t* block_table, const int32_
                       int page_size, int max_pages, int num_pages, int total, int max_len,
                       int bits, int dtype, cudaStream_t stream) {
   using namespace kvq;
-  const long long J = ((long long)max_len + page_size - 2) / page_size + 1;
+  // No sequence has more rows than there are, however loose a bound max_len is.
+  const long long longest = max_len < total ? max_len : total;
+  const long long J = (longest + page_size - 2) / page_size + 1;
+  if (J * Hkv > 0x7fffff00ll)  // a warp's unit is an int
+    return set_error(B2A_ERR_INVALID_ARG, "total and max_len too large");
   const long long gx = (J * Hkv + kWarps - 1) / kWarps;
-  if (gx > 0x7fffffffll) return set_error(B2A_ERR_INVALID_ARG, "max_len too large");
   const dim3 grid((unsigned)gx, (unsigned)B);
   const int shift = page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
   auto go = [&](auto kern) {

@@ -300,10 +300,11 @@ int b2a_kvq_append_paged(const void* k_new, const void* v_new,
  * b2a_prefill_fwd_varlen: tokens start[b] .. start[b] + n_b - 1 of sequence b
  * (start == NULL: from 0), n_b = cu_seqlens[b+1] - cu_seqlens[b], go to rows
  * cu_seqlens[b].. of k_out, v_out [total, Hkv, D] (dtype), each value one fp32
- * multiply-add rounded once.  max_len bounds every n_b.  Rows that no sequence
- * owns are left as they were.  A page that the block table lacks sets bit 1 of
- * the device error word and its rows read as zero; a sequence with bad
- * cu_seqlens or start, or longer than max_len, sets bit 3 and is not read.
+ * multiply-add rounded once.  max_len bounds every n_b (one above total counts
+ * as total).  Rows that no sequence owns are left as they were.  A page that
+ * the block table lacks sets bit 1 of the device error word and its rows read
+ * as zero; a sequence with bad cu_seqlens or start, or longer than max_len,
+ * sets bit 3 and is not read.
  */
 int b2a_kvq_read_paged(const void* data, const int32_t* block_table,
                        const int32_t* start, const int32_t* cu_seqlens,

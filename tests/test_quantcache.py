@@ -1022,3 +1022,22 @@ def test_values_of_zero_before_others():
         for splits in (1, 2):
             O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
             check_own_steps(f, q, O, L)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hkv,page", [(16, 16), (32, 16), (3, 64)])
+def test_read_back_with_a_loose_bound(Hkv, page):
+    """max_len only has to bound the lengths: 2^31 - 1 reads what the longest length reads."""
+    import b200attn
+    lens = [40, 0, 7]
+    f = Filled(3, Hkv, 64, page, 4, F16, lens, seed=247)
+    cu = torch.tensor([0, 40, 40, 47], dtype=torch.int32, device="cuda")
+    want = b200attn.read_paged_quant(f.cache, f.btg, cu, 47, 40)
+    got = b200attn.read_paged_quant(f.cache, f.btg, cu, 47, 2 ** 31 - 1)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    start = torch.tensor([39, 0, 5], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 1, 1, 3], dtype=torch.int32, device="cuda")
+    got = b200attn.read_paged_quant(f.cache, f.btg, cu, 3, 2 ** 31 - 1, start=start)
+    for a, w in zip(got, want):
+        assert torch.equal(a, w[[39, 45, 46]])
+    assert b200attn.device_error_flags() == 0
