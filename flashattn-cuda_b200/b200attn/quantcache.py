@@ -40,10 +40,18 @@ GROUP = 64  # channels that share one (scale, min)
 _BLOCK_BYTES = {}
 
 
+def _fit(*ints):
+    """Refuse what a C int does not hold (ctypes would drop its upper bits)."""
+    for x in ints:
+        if not -1 << 31 <= x < 1 << 31:
+            raise RuntimeError(f"{x} does not fit in 32 bits")
+
+
 def block_bytes(head_dim: int, page_size: int, bits: int) -> int:
     """Bytes of one (page, KV head) block."""
     n = _BLOCK_BYTES.get((head_dim, page_size, bits))
     if n is None:
+        _fit(head_dim, page_size, bits)
         n = _lib.load().b2a_kvq_block_bytes(head_dim, page_size, bits)
         if n == 0:
             raise RuntimeError("head_dim must be 64 or 128, page_size 16, 32 or 64 and bits 4 or 8")
@@ -56,19 +64,23 @@ def _strides(*s):
 
 
 def _append_ct(k, v, data, index, index_scale, *rest):
+    _fit(*rest[2:12])
     return _lib.load().b2a_kvq_append_paged(k, v, _strides(*rest[13:16]), _strides(*rest[16:]),
                                             data, index, index_scale, *rest[:13])
 
 
 def _read_ct(*args):
+    _fit(*args[6:16])
     return _lib.load().b2a_kvq_read_paged(*args)
 
 
 def _select_ct(q, *rest):
+    _fit(*rest[6:15])
     return _lib.load().b2a_kvq_select_pages(q, _strides(*rest[16:]), *rest[:16])
 
 
 def _decode_ct(q, *rest):
+    _fit(rest[4], *rest[8:18])
     return _lib.load().b2a_kvq_decode_paged(q, _strides(*rest[19:21]), *rest[:18], rest[21],
                                             rest[18])
 
@@ -251,7 +263,7 @@ def read_paged_quant(cache: QuantCache, block_table: torch.Tensor, cu_seqlens: t
             _lib.check(_read(
                 cache.data.data_ptr(), block_table.data_ptr(), _ptr(start),
                 cu_seqlens.data_ptr(), K.data_ptr(), V.data_ptr(), B, shape[1], shape[2],
-                cache.page_size, max_pages, cache.num_pages, shape[0], int(max_len),
+                cache.page_size, max_pages, cache.num_pages, shape[0], int(min(max_len, total)),
                 cache.bits, _DT[cache.dtype], _stream(dev)))
     return [K, V]
 
@@ -278,8 +290,8 @@ def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
     q3, _, B, H, D = _check_query(q, cache)
     if cache.index is None:
         raise RuntimeError("select_pages needs a cache with an index")
-    if top_k <= 0:
-        raise RuntimeError("top_k must be > 0")
+    if not 0 < top_k < 1 << 31:
+        raise RuntimeError("top_k must be > 0 and < 2^31")
     rows, max_pages = _check_table(cache, block_table, kv_lens, "kv_lens")
     if rows != B:
         raise RuntimeError("block_table must have one row per sequence")
@@ -302,6 +314,8 @@ def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
 def _plan(B: int, H: int, Hkv: int, D: int, bits: int, max_tokens: int, splits):
     """(warps that share a decode, floats of its workspace): functions of the sizes alone."""
     lib = _lib.load()
+    if splits is not None:
+        _fit(int(splits) * B * Hkv)
     workers = (lib.b2a_kvq_decode_workers(B, Hkv, D, bits, max_tokens) if splits is None
                else int(splits) * B * Hkv)
     return workers, max(lib.b2a_kvq_decode_workspace_floats(B, H, Hkv, D, workers), 1)

@@ -30,9 +30,11 @@ static PyObject* prefill_fwd_kv(PyObject* self, PyObject* args) {
   return PyLong_FromLong(rc);
 }
 
-/* The quantised cache's entry points take n integers (pointers, the stream and
- * strides among them; 0 for a null pointer) and, decode, one float last. */
-static int parse_ints(PyObject* const* args, Py_ssize_t nargs, Py_ssize_t n, long long* v) {
+/* The quantised cache's entry points take n integers and, decode, one float last.
+ * `wide` has a bit for each of 64 bits: pointers (0 for a null one), the stream and
+ * strides.  The others are ints: a value that does not fit one is refused. */
+static int parse_ints(PyObject* const* args, Py_ssize_t nargs, Py_ssize_t n, unsigned wide,
+                      long long* v) {
   if (nargs < n) {
     PyErr_Format(PyExc_TypeError, "expected at least %zd arguments, got %zd", n, nargs);
     return -1;
@@ -44,18 +46,23 @@ static int parse_ints(PyObject* const* args, Py_ssize_t nargs, Py_ssize_t n, lon
     }
     v[i] = PyLong_AsLongLong(args[i]);
     if (v[i] == -1 && PyErr_Occurred()) return -1;
+    if (!(wide >> i & 1u) && v[i] != (int)v[i]) {
+      PyErr_Format(PyExc_RuntimeError, "%lld does not fit in 32 bits", v[i]);
+      return -1;
+    }
   }
   return 0;
 }
 #define PTR(i) ((void*)(uintptr_t)v[i])
 #define INT(i) ((int)v[i])
+#define BITS(from, to) ((1u << (to)) - (1u << (from))) /* from .. to - 1 */
 
 /* kvq_append(k, v, data, index, index_scale, table, lens, B, Hkv, T, D, page, max_pages,
  * num_pages, bits, dtype, advance, stream, k strides x 3, v strides x 3) -> status */
 static PyObject* kvq_append(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   long long v[24];
   (void)self;
-  if (parse_ints(args, nargs, 24, v) != 0) return NULL;
+  if (parse_ints(args, nargs, 24, BITS(0, 7) | BITS(17, 24), v) != 0) return NULL;
   const int64_t ks[3] = {v[18], v[19], v[20]}, vs[3] = {v[21], v[22], v[23]};
   return PyLong_FromLong(b2a_kvq_append_paged(
       PTR(0), PTR(1), ks, vs, PTR(2), (int8_t*)PTR(3), (float*)PTR(4), (const int32_t*)PTR(5),
@@ -68,7 +75,7 @@ static PyObject* kvq_append(PyObject* self, PyObject* const* args, Py_ssize_t na
 static PyObject* kvq_read(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   long long v[17];
   (void)self;
-  if (parse_ints(args, nargs, 17, v) != 0) return NULL;
+  if (parse_ints(args, nargs, 17, BITS(0, 6) | BITS(16, 17), v) != 0) return NULL;
   return PyLong_FromLong(b2a_kvq_read_paged(
       PTR(0), (const int32_t*)PTR(1), (const int32_t*)PTR(2), (const int32_t*)PTR(3), PTR(4),
       PTR(5), INT(6), INT(7), INT(8), INT(9), INT(10), INT(11), INT(12), INT(13), INT(14),
@@ -80,7 +87,7 @@ static PyObject* kvq_read(PyObject* self, PyObject* const* args, Py_ssize_t narg
 static PyObject* kvq_select(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   long long v[19];
   (void)self;
-  if (parse_ints(args, nargs, 19, v) != 0) return NULL;
+  if (parse_ints(args, nargs, 19, BITS(0, 7) | BITS(16, 19), v) != 0) return NULL;
   const int64_t qs[2] = {v[17], v[18]};
   return PyLong_FromLong(b2a_kvq_select_pages(
       PTR(0), qs, (const int8_t*)PTR(1), (const float*)PTR(2), (const int32_t*)PTR(3),
@@ -97,7 +104,7 @@ static PyObject* kvq_decode(PyObject* self, PyObject* const* args, Py_ssize_t na
     PyErr_Format(PyExc_TypeError, "expected 23 arguments, got %zd", nargs);
     return NULL;
   }
-  if (parse_ints(args, nargs, 22, v) != 0) return NULL;
+  if (parse_ints(args, nargs, 22, BITS(0, 5) | BITS(6, 9) | BITS(19, 22), v) != 0) return NULL;
   const double scale = PyFloat_AsDouble(args[22]);
   if (scale == -1.0 && PyErr_Occurred()) return NULL;
   const int64_t qs[2] = {v[20], v[21]};

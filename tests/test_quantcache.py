@@ -1041,3 +1041,29 @@ def test_read_back_with_a_loose_bound(Hkv, page):
     for a, w in zip(got, want):
         assert torch.equal(a, w[[39, 45, 46]])
     assert b200attn.device_error_flags() == 0
+
+
+def test_numbers_past_32_bits_are_refused():
+    """No argument reaches the library without its upper bits, through either binding."""
+    from b200attn import quantcache as qc
+    big = (1 << 32) + 16
+    with pytest.raises(RuntimeError, match="32 bits"):
+        qc.block_bytes((1 << 32) + 128, 16, 4)
+    with pytest.raises(RuntimeError, match="32 bits"):
+        qc._plan(1, 8, 8, 128, 4, 100, 1 << 29)
+    # places of the ints among the arguments
+    calls = {"_append": (24, range(7, 17)), "_read": (17, range(6, 16)),
+             "_select": (19, range(7, 16)), "_decode": (23, [5, *range(9, 19)])}
+    for name, (n, ints) in calls.items():
+        for f in {getattr(qc, name), getattr(qc, name + "_ct")}:
+            for i in range(n):
+                for value in (big, -big):
+                    args = [0] * n
+                    args[i] = value
+                    if name == "_decode" and i == 22:
+                        continue                     # the scale
+                    if i in ints:
+                        with pytest.raises(RuntimeError, match="32 bits"):
+                            f(*args)
+                    else:
+                        assert f(*args) != 0         # refused by the library: no device, or no such shape
