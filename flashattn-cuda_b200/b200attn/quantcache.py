@@ -205,7 +205,8 @@ def append_paged_quant(k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCac
                        advance: bool = True) -> None:
     """Quantise k_new, v_new [B, Hkv, T, D] (cache.dtype, any strides) and write them at
     positions kv_lens[b] + t of the sequences in block_table (b2a_kvq_append_paged); with
-    `advance`, kv_lens += T on the device.  Updates the index of a cache that has one.
+    `advance`, kv_lens += T on the device (a negative length stays, its tokens are dropped).
+    Updates the index of a cache that has one.
     No page may be owned by two of the sequences that write to it."""
     shape = k_new.shape
     if len(shape) != 4 or shape != v_new.shape:

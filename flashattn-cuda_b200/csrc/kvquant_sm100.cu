@@ -32,6 +32,12 @@ struct NewRows {  // element strides of k_new / v_new [B, Hkv, T, D]
   long long b, h, t;
 };
 
+// A length after T more tokens: a negative one, whose tokens are dropped, stays, so
+// that it does not turn into one that looks valid; nor does one pass 2^31 - 1.
+__device__ __forceinline__ int advanced(int len, int T) {
+  return len < 0 ? len : (int)min((long long)len + T, 0x7fffffffll);
+}
+
 template <int D, int BITS, bool BF16>
 __global__ void append_kernel(const void* __restrict__ k_new, const void* __restrict__ v_new,
                               NewRows ks, NewRows vs, uint8_t* __restrict__ data,
@@ -58,7 +64,7 @@ __global__ void append_kernel(const void* __restrict__ k_new, const void* __rest
   // only after every warp has read it.
   if (advance) {
     __syncthreads();
-    if (threadIdx.x == 0) kv_lens[b] = len + T;
+    if (threadIdx.x == 0) kv_lens[b] = advanced(len, T);
   }
   if (j >= J) return;
   if (len < 0) {
@@ -223,7 +229,7 @@ __global__ void advance_kernel(int32_t* __restrict__ kv_lens, int B, int T) {
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  if (b < B) kv_lens[b] += T;
+  if (b < B) kv_lens[b] = advanced(kv_lens[b], T);
 }
 
 template <int D, int BITS, bool BF16>

@@ -274,7 +274,8 @@ int64_t b2a_kvq_block_bytes(int D, int page_size, int bits);
 /*
  * Quantise and append T new tokens per sequence: the write path of the cache,
  * with b2a_kv_append_paged's block table, lengths, advance_lens and error bit
- * 2 (a sequence whose kv_lens is negative is dropped too).  k_new, v_new are
+ * 2.  The tokens of a sequence whose kv_lens is negative are dropped too, and
+ * its length stays; no length is advanced past 2^31 - 1.  k_new, v_new are
  * [B,Hkv,T,D] with element strides k_strides / v_strides = {batch, head,
  * token}, multiples of 8; rows are contiguous and 16-byte aligned.
  *   With n = 2^bits - 1 and a group's extremes lo, hi: scale = (hi - lo)/n

@@ -1067,3 +1067,23 @@ def test_numbers_past_32_bits_are_refused():
                             f(*args)
                     else:
                         assert f(*args) != 0         # refused by the library: no device, or no such shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 200])
+def test_lengths_that_do_not_advance(T):
+    """A negative length stays what it is, for one token and for many (which take two ways to the
+    lengths); one next to 2^31 stops there.  Their tokens are dropped, the others' are not."""
+    import b200attn
+    cache = b200attn.QuantCache.empty(16, 16, 3, 64, dtype=F16)
+    bt = torch.full((4, 14), -1, dtype=torch.int32, device="cuda")
+    bt[1] = torch.arange(14)
+    top = 2 ** 31 - 1
+    kl = torch.tensor([-4, 3, top - T + 1, -2 ** 31], dtype=torch.int32, device="cuda")
+    k = torch.ones(4, 3, T, 64, dtype=F16, device="cuda")
+    b200attn.device_error_flags()
+    b200attn.append_paged_quant(k, k, cache, bt, kl)
+    assert kl.tolist() == [-4, 3 + T, top, -2 ** 31]
+    assert b200attn.device_error_flags() == 4
+    got = cache.params(0)[:14, 0, :, 0, 1].flatten()
+    assert (got[3:3 + T] == 1).all() and not got[:3].any() and not got[3 + T:].any()
