@@ -28,7 +28,10 @@ __host__ __device__ constexpr int block_bytes(int D, int page, int bits) {
 // as soon as all its own blocks run (pdl_trigger), and a kernel that was started
 // so waits for the one before it, and its memory, before it touches any
 // (pdl_wait).  Only the launch itself overlaps; after a foreign kernel both do
-// nothing.
+// nothing.  A kernel may thus be alive while the one before writes what it will
+// read: no pointer that it reads through is both const and __restrict__, which would
+// promise memory that nobody writes while the kernel lives, and let loads of it
+// pass the wait.
 __device__ __forceinline__ void pdl_trigger() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

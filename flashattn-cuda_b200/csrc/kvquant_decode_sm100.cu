@@ -380,7 +380,7 @@ __device__ __forceinline__ void select_top(const uint32_t* kp, int all, int32_t*
 
 template <int THREADS, int KPT>
 __global__ void __launch_bounds__(THREADS)
-    select_kernel(const uint32_t* __restrict__ keys, const int32_t* __restrict__ kv_lens,
+    select_kernel(const uint32_t* keys, const int32_t* kv_lens,
                   int32_t* __restrict__ pages, int Hkv, int page_size, int max_pages, int top_k) {
   const int hkv = blockIdx.x, b = blockIdx.y;
   pdl_trigger();
@@ -554,9 +554,9 @@ __device__ __forceinline__ int seq_steps(int len, int n_list, int page_shift) {
 
 template <int D, int BITS, bool BF16, bool HALF>
 __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>::kCtas)
-    decode_kernel(const void* __restrict__ q, long long q_b, long long q_h,
-                  const uint8_t* __restrict__ data, const int32_t* __restrict__ block_table,
-                  const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ pages,
+    decode_kernel(const void* q, long long q_b, long long q_h,
+                  const uint8_t* data, const int32_t* block_table,
+                  const int32_t* kv_lens, const int32_t* pages,
                   int n_list, float* __restrict__ o_part, float* __restrict__ l_part,
                   int* __restrict__ meta, void* __restrict__ out, float* __restrict__ lse, int B,
                   int G, int Hkv, int workers, int by_tile, int page_shift, int max_pages,
@@ -1187,8 +1187,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 constexpr int kChunk = 512;  // weights held at a time
 template <int D, int NW, bool BF16>
 __global__ void __launch_bounds__(32 * NW)
-    combine_kernel(const float* __restrict__ o_part, const float* __restrict__ l_part,
-                   const int* __restrict__ meta, const int32_t* __restrict__ kv_lens,
+    combine_kernel(const float* o_part, const float* l_part,
+                   const int* meta, const int32_t* kv_lens,
                    void* __restrict__ out, float* __restrict__ lse, int G, int Hkv, int by_tile) {
   using T1 = typename Elem<BF16>::T;
   constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp

@@ -39,10 +39,10 @@ __device__ __forceinline__ int advanced(int len, int T) {
 }
 
 template <int D, int BITS, bool BF16>
-__global__ void append_kernel(const void* __restrict__ k_new, const void* __restrict__ v_new,
+__global__ void append_kernel(const void* k_new, const void* v_new,
                               NewRows ks, NewRows vs, uint8_t* __restrict__ data,
                               int8_t* __restrict__ index, float* __restrict__ index_scale,
-                              const int32_t* __restrict__ block_table, int32_t* kv_lens, int Hkv,
+                              const int32_t* block_table, int32_t* kv_lens, int Hkv,
                               int T, int J, int page_shift, int max_pages, int num_pages,
                               int one_cta, int advance) {
   using T1 = typename Elem<BF16>::T;
@@ -234,8 +234,8 @@ __global__ void advance_kernel(int32_t* __restrict__ kv_lens, int B, int T) {
 
 template <int D, int BITS, bool BF16>
 __global__ void __launch_bounds__(32 * kWarps)
-    read_kernel(const uint8_t* __restrict__ data, const int32_t* __restrict__ block_table,
-                const int32_t* __restrict__ start, const int32_t* __restrict__ cu,
+    read_kernel(const uint8_t* data, const int32_t* block_table,
+                const int32_t* start, const int32_t* cu,
                 void* __restrict__ k_out, void* __restrict__ v_out, int Hkv, int J, int page_shift,
                 int max_pages, int num_pages, int total, int max_len) {
   using T1 = typename Elem<BF16>::T;

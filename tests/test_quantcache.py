@@ -1087,3 +1087,16 @@ def test_lengths_that_do_not_advance(T):
     assert b200attn.device_error_flags() == 4
     got = cache.params(0)[:14, 0, :, 0, 1].flatten()
     assert (got[3:3 + T] == 1).all() and not got[:3].any() and not got[3 + T:].any()
+
+
+def test_kernels_promise_no_constant_memory():
+    """Kernels that may start before the one ahead has ended (griddepcontrol) must not declare
+    what that one writes as constant while they live: `const T* __restrict__`."""
+    import os
+    import re
+    from conftest import PKG_PARENT
+    for name in ("kvquant.cuh", "kvquant_sm100.cu", "kvquant_decode_sm100.cu"):
+        text = open(os.path.join(PKG_PARENT, "csrc", name)).read()
+        assert "pdl_wait" in text
+        assert not re.findall(r"const\s+\w+\s*\*\s*(?:const\s+)?__restrict__", text), name
+        assert "__ldg(" not in text and "ld.global.nc" not in text
