@@ -1133,7 +1133,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   int st = 0;
   uint32_t phase = 0;
   for (int j = 0; j < n; ++j) {
-    ok = ok && mbar_wait(bar0 + 8 * st, phase, abort_flag);
+    // one answer for the warp: a copy that lands between two lanes' last looks must
+    // not leave it divided before its shuffles
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(bar0 + 8 * st, phase, abort_flag));
     if (ok) {
       const uint8_t* stage = ring + st * C::kStage;
       if (full >> st & 1u) {

@@ -1100,3 +1100,15 @@ def test_kernels_promise_no_constant_memory():
         assert "pdl_wait" in text
         assert not re.findall(r"const\s+\w+\s*\*\s*(?:const\s+)?__restrict__", text), name
         assert "__ldg(" not in text and "ld.global.nc" not in text
+
+
+def test_a_warp_agrees_on_its_waits():
+    """A bounded wait may run out in some lanes of a warp only; what the warp does next has
+    shuffles, so the lanes' answers are made one by a vote.  (Read from the source: no test can
+    place a copy's arrival between two lanes' looks.)"""
+    import os
+    import re
+    from conftest import PKG_PARENT
+    text = open(os.path.join(PKG_PARENT, "csrc", "kvquant_decode_sm100.cu")).read()
+    waits = re.findall(r"^.*\bmbar_wait\(.*$", text, re.M)
+    assert waits and all("__all_sync(0xffffffffu," in w for w in waits)
