@@ -394,8 +394,10 @@ class QuantPagePool(PagePool):
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, seqs: Optional[List[int]] = None):
         """Quantise and append k_new, v_new [B, Hkv, T, D] to `seqs` (default 0..B-1), each
         sequence at most once."""
-        if seqs is not None and len(set(seqs)) != len(list(seqs)):
-            raise RuntimeError("a sequence may appear only once in one append")
+        if seqs is not None:
+            seqs = [range(len(self._lens))[s] for s in seqs]  # -1 and its positive name are one
+            if len(set(seqs)) != len(seqs):
+                raise RuntimeError("a sequence may appear only once in one append")
         super().append(k_new, v_new, seqs)
 
     def read(self, seqs: Optional[List[int]] = None) -> list:
@@ -412,7 +414,9 @@ class QuantPagePool(PagePool):
     def decode(self, q: torch.Tensor, seqs: Optional[List[int]] = None,
                scale: Optional[float] = None, top_k: Optional[int] = None) -> list:
         """[O, L] of the queries q [B, H, D], one per sequence of `seqs` (default 0..B-1);
-        with top_k over that many pages of each KV head only."""
+        with top_k over that many pages of each KV head only.  The table is cut to the pages
+        that the sequences have now: a captured step is decode_paged_quant over `block_table`
+        and `kv_lens`, whose width does not change."""
         seqs, bt, lens = self._rows(seqs, q.shape[0])
         most = max((len(self._pages[s]) for s in seqs), default=0)
         bt = bt[:, :max(most, 1)].contiguous()  # the widest sequence's pages: fewer empty splits

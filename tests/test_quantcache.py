@@ -1112,3 +1112,22 @@ def test_a_warp_agrees_on_its_waits():
     text = open(os.path.join(PKG_PARENT, "csrc", "kvquant_decode_sm100.cu")).read()
     waits = re.findall(r"^.*\bmbar_wait\(.*$", text, re.M)
     assert waits and all("__all_sync(0xffffffffu," in w for w in waits)
+
+
+def test_pool_takes_any_iterable_of_sequences():
+    """A generator is as good as a list; one sequence under two names is one sequence."""
+    from b200attn.quantcache import QuantPagePool
+    pool = QuantPagePool(10, 16, 2, 64, max_seqs=3, max_pages=8, device="cpu")
+    wrote = []
+    pool._write = lambda k, v, bt, lens: (wrote.append(k.shape[0]), lens.add_(k.shape[2]))
+    k = torch.zeros(2, 2, 5, 64, dtype=F16)
+    pool.append(k, k, seqs=(s for s in (2, 0)))
+    pool.append(k, k, seqs=torch.tensor([1, 2]))
+    pool.append(k, k, seqs=[-1, 0])
+    assert wrote == [2, 2, 2] and pool.lengths() == [10, 5, 15]
+    for bad in ([2, -1], torch.tensor([1, 1]), iter([0, 0])):
+        with pytest.raises(RuntimeError, match="once"):
+            pool.append(k, k, seqs=bad)
+    with pytest.raises(IndexError):
+        pool.append(k, k, seqs=[0, 3])
+    assert pool.lengths() == [10, 5, 15]
