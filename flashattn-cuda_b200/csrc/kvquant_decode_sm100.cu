@@ -801,7 +801,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   // --------------------------------------------------------------------- state
   alignas(16) float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
   alignas(8) float omin[NG][2];  // sum of p * (vmin + mid * vscale) over this lane's tokens
-  float m[2], l[2];
+  float m[2], l[2];  // the largest score, in the units of S, and the sum of p
   // p * vscale of a head's group is multiplied by vmul before it is rounded; o
   // holds sums of such products.  Value steps are 0 or 2^-100 and more.
   alignas(8) float vmul[NG][2];
@@ -928,9 +928,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       for (int k = 1; k < SL * R; ++k) mx = fmaxf(mx, s[k / R][k % R][h]);
 #pragma unroll
       for (int x = HALF ? 2 : 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float mn = fmaxf(m[h], mx * sl2[h]);
+      const float mn = fmaxf(m[h], mx);
       const float mu = mn == -INFINITY ? 0.f : mn;
-      alpha[h] = ex2_mufu(m[h] - mu);
+      alpha[h] = ex2_mufu((m[h] - mu) * sl2[h]);
       moved = moved || mn != m[h];
       m[h] = mn;
       nmu[h] = -mu;
@@ -939,7 +939,10 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 #pragma unroll
     for (int k = 0; k < SL * R; ++k) {
       float2& x = pair(s[k / R][k % R]);
-      x = ffma2(x, make_float2(sl2[0], sl2[1]), make_float2(nmu[0], nmu[1]));
+      // The difference first: the largest score's is 0 whatever its size.  (s * sl2 - m in
+      // one instruction leaves what a maximum in log2 units lost in rounding: past 2^31 p
+      // of all tokens is 0 or infinite.)
+      x = fmul2(fadd2(x, make_float2(nmu[0], nmu[1])), make_float2(sl2[0], sl2[1]));
       x.x = ex2_mufu(x.x);
       x.y = ex2_mufu(x.y);
       sum = fadd2(sum, x);
@@ -1087,7 +1090,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     for (int h = 0; h < 2; ++h) {
       const int head = head0 + h;
       const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
-      const float ll = l[h] == 0.f ? -INFINITY : m[h] * kLn2 + logf(l[h]);
+      const float ll = l[h] == 0.f ? -INFINITY : m[h] * sl2[h] * kLn2 + logf(l[h]);
       const size_t orow = whole ? (size_t)b * Hkv * G + hkv * G + head : seg * G + head;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {

@@ -1131,3 +1131,26 @@ def test_pool_takes_any_iterable_of_sequences():
     with pytest.raises(IndexError):
         pool.append(k, k, seqs=[0, 3])
     assert pool.lengths() == [10, 5, 15]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,bits,dt,G", RANGE, ids=str)
+@pytest.mark.parametrize("power", [18, 26, 33, 60])
+def test_scores_of_any_size(D, bits, dt, G, power):
+    """Scores up to 2^60: one token's is the largest by 2 percent, and it takes all the weight."""
+    import b200attn
+    if dt == F16 and power == 60:
+        power = 36
+    n = 300
+    f = Filled(1, 2, D, 16, bits, dt, [n], seed=257)
+    q = torch.full((1, 2 * G, D), 2.0 ** (power // 2 - 3), dtype=dt, device="cuda")
+    rows = torch.from_numpy(np.random.default_rng(5).permutation(n)) / n
+    size = 0.9 - 0.4 * rows                                  # 0.5 .. 0.9 and one at 0.92
+    size[211] = 0.92
+    k = (size[None, None, :, None].cuda() * 2.0 ** (power - power // 2 - 3)).to(dt).expand(1, 2, n, D)
+    with_values(f, k=k)
+    assert float(q.max()) * float(k.max()) * D ** 0.5 > 2.0 ** (power - 4)
+    for splits in (None, 1, 2):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_own_steps(f, q, O, L)
+    assert b200attn.device_error_flags() == 0
