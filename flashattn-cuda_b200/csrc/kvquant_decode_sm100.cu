@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     }
     const int e = 24 - min(max(shift, -126), 127);  // up to 139: in two steps
     // not 0: a masked score is -inf, whose product with it stays -inf
-    const float s2 = fmaxf(scale_log2 * pow2i(e / 2) * pow2i(e - e / 2), 1.17549435e-38f);
+    const float s2 = fmaxf(scale_log2 * pow2i(e / 2) * pow2i(e - e / 2), 1.401298464e-45f);
     sl2[0] = __shfl_sync(0xffffffffu, s2, 8 * t);  // what a score in these units is in log2
     sl2[1] = __shfl_sync(0xffffffffu, s2, 8 * t + 4);
   };

@@ -1154,3 +1154,16 @@ def test_scores_of_any_size(D, bits, dt, G, power):
         O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
         check_own_steps(f, q, O, L)
     assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+def test_tiny_queries_and_scales():
+    """Queries next to the smallest of bf16 with keys next to the largest and a tiny scale: the
+    factor that takes a score to log2 units is a subnormal number, and counts as it is."""
+    import b200attn
+    f = Filled(1, 1, 64, 16, 8, BF16, [100], seed=267)
+    with_values(f, k=(f.k[0].float().abs() * 2.0 ** 124).to(BF16))  # all of one sign: sums count
+    q = (torch.from_numpy(ora.seeded_normal((1, 4, 64), 269)).abs() * 2.0 ** -118).bfloat16().cuda()
+    for scale in (1e-6, 1e-9, 1e-11):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, scale=scale)
+        check_attention(f, q, O, L, scale=scale)
