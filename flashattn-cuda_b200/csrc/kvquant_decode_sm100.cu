@@ -446,14 +446,15 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // exponents, a subnormal's being 2^-14: with K's codes at bits 2-5 and 6-9, not 0-3
 // and 4-7, lse of fp16 caches is off by 0.6e-7 of its size instead of 4e-7 (fp32
 // products: 0.4e-7), for another shift, 4 us below.  Both cache dtypes use fp16
-// operands: a query head is brought to [2^12, 2^13) by a power of two (over 64, a
-// channel is off by 2^-25 at most), and p*vscale by a running factor of its own for
-// each head and group of channels, which at the last change brought the step's
-// largest product to [2^7, 2^8).  That goes by the products, so a token whose values
-// are large but that has no weight takes no bits from the others, and the factor
-// grows as the maximum does (o stays and its unit changes), so what is left of early
-// tokens takes none from later ones.  A product within 2^-21 of the largest keeps
-// fp16's 11 bits, one below is off by 2^-32 of the largest at most.
+// operands: each group of a query head is brought to [2^12, 2^13) by a power of two
+// (over 64, a channel is off by 2^-25 of the group's largest at most; the groups'
+// sums meet in fp32), and p*vscale by a running factor of its own for each head and
+// group, which at the last change brought the step's largest product to [2^7, 2^8).
+// That goes by the products, so a token whose values are large but that has no weight
+// takes no bits from the others, and the factor grows as the maximum does (o stays and
+// its unit changes), so what is left of early tokens takes none from later ones.  A
+// product within 2^-21 of the largest keeps fp16's 11 bits, one below is off by 2^-32
+// of the largest at most.
 //
 // The token dimension is M of both products (A = K codes [tok, d], and A =
 // V codes transposed [d, tok]) and the heads are N = 8, so no row of the
@@ -494,7 +495,8 @@ struct DecCfg {
   static constexpr int kOffBar = kWarps * kRing;
   static constexpr int kOffValid = kOffBar + kWarps * kStages * 8;    // [warp][stage] int4
   static constexpr int kOffAbort = kOffValid + kWarps * kStages * 16;  // [warp] int
-  static constexpr int kSmem = kOffAbort + kWarps * 4;
+  static constexpr int kOffQuery = (kOffAbort + kWarps * 4 + 15) / 16 * 16;  // [warp][4][8] float
+  static constexpr int kSmem = kOffQuery + kWarps * 128;
 };
 
 // D[16x8] += A[16x16] B[16x8], fp16 operands, fp32 accumulators
@@ -741,13 +743,18 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   const int half = t >> 1;                      // HALF: this lane's token row, g or g + 8
   const int head0 = HALF ? 2 * (t & 1) : 2 * t;  // its heads: head0, head0 + 1
   uint32_t qb[NG * 4][2];
-  float qsum[NG][2], sl2[2];
+  // Of columns 2t and 2t + 1, in shared memory: sums of the groups' channels, the
+  // factor from the second group's units of S to the first's, and what a score in
+  // these units is in log2.
+  float* s_q = reinterpret_cast<float*>(smem + C::kOffQuery) + warp * 32;
   auto load_q = [&]() {
     const int hq = HALF ? g & 3 : g;
     const T1* qp = static_cast<const T1*>(q) + b * q_b + (long long)(hkv * G + hq) * q_h + 16 * t;
-    float f[NG][16], top = 0.f;
+    float f[NG][16];
+    int shift[NG];  // to [2^12, 2^13)
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
+      float top = 0.f;
       uint32_t u[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
       if (hq < G) {
         *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(qp + gr * 64);
@@ -760,13 +767,21 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         f[gr][2 * j + 1] = v.y;
         top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
       }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      shift[gr] = min(139 - (int)(__float_as_uint(top) >> 23), 127);
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int shift = 139 - (int)(__float_as_uint(top) >> 23);  // to [2^12, 2^13)
-    const float mul = pow2i(shift);
+    float fac = 1.f;
+    if constexpr (NG == 2) {  // units at most 2^30 apart: sums of both stay in fp32's range
+      const int least = min(shift[0], shift[1]);
+      shift[0] = min(shift[0], least + 30);
+      shift[1] = min(shift[1], least + 30);
+      fac = pow2i(shift[0] - shift[1]);
+    }
+    float* mine = s_q + (g >> 1) * 8 + (g & 1);  // column g's, written by one of its lanes
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
+      const float mul = pow2i(shift[gr]);
       float sum = 0.f;  // of a column's channels
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -776,8 +791,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       sum *= pow2i(-24);  // the codes' factor
-      qsum[gr][0] = __shfl_sync(0xffffffffu, sum, 8 * t);  // columns 2t, 2t + 1
-      qsum[gr][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      if (t == 0) mine[2 * gr] = sum;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (BITS == 4) {
@@ -791,11 +805,14 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
         }
       }
     }
-    const int e = 24 - min(max(shift, -126), 127);  // up to 139: in two steps
+    const int e = 24 - max(shift[0], -126);  // up to 140: in two steps
     // not 0: a masked score is -inf, whose product with it stays -inf
     const float s2 = fmaxf(scale_log2 * pow2i(e / 2) * pow2i(e - e / 2), 1.401298464e-45f);
-    sl2[0] = __shfl_sync(0xffffffffu, s2, 8 * t);  // what a score in these units is in log2
-    sl2[1] = __shfl_sync(0xffffffffu, s2, 8 * t + 4);
+    if (t == 0) {
+      if (NG == 2) mine[4] = fac;
+      mine[6] = s2;
+    }
+    __syncwarp();
   };
 
   // --------------------------------------------------------------------- state
@@ -839,6 +856,11 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   auto step = [&](auto all, const uint8_t* stage, const int (&nv)[4]) {
     constexpr bool FULL = decltype(all)::value;
 
+    const float4 qa = *reinterpret_cast<const float4*>(s_q + 8 * t);
+    const float4 qc = *reinterpret_cast<const float4*>(s_q + 8 * t + 4);
+    const float2 qsum[2] = {make_float2(qa.x, qa.y), make_float2(qa.z, qa.w)};
+    const float2 qfac = make_float2(qc.x, qc.y), sl2 = make_float2(qc.z, qc.w);
+
     // ---- S = K q^T
     alignas(16) float s[SL][R][2];
     uint32_t vpar[SL][R][NG];  // (scale, min) of V of this lane's rows
@@ -869,7 +891,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       }
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        float acc[4];  // (row g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
+        alignas(8) float acc[4];  // (row g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
         if constexpr (BITS == 4) {
           const uint2 x = *reinterpret_cast<const uint2*>(kc + gr * 32 + t * 8);
           const uint2 y = *reinterpret_cast<const uint2*>(kc + 8 * ROW + gr * 32 + t * 8);
@@ -898,12 +920,10 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const float2 pr = param<BF16>(kpar[r][gr]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float a = HALF ? (half ? acc[2 + h] : acc[h]) : acc[2 * r + h];
-            s[sl][r][h] = fmaf(pr.x, a, gr == 0 ? pr.y * qsum[gr][h]
-                                                : fmaf(pr.y, qsum[gr][h], s[sl][r][h]));
-          }
+          const float2 a = HALF ? (half ? pair(acc + 2) : pair(acc)) : pair(acc + 2 * r);
+          const float2 x = ffma2(make_float2(pr.x, pr.x), a,
+                                 fmul2(make_float2(pr.y, pr.y), qsum[gr]));
+          pair(s[sl][r]) = gr == 0 ? x : ffma2(x, qfac, pair(s[sl][r]));
         }
       }
       // tokens past the end: whatever their slots hold is dropped here
@@ -930,7 +950,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       for (int x = HALF ? 2 : 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       const float mn = fmaxf(m[h], mx);
       const float mu = mn == -INFINITY ? 0.f : mn;
-      alpha[h] = ex2_mufu((m[h] - mu) * sl2[h]);
+      alpha[h] = ex2_mufu((m[h] - mu) * (h ? sl2.y : sl2.x));
       moved = moved || mn != m[h];
       m[h] = mn;
       nmu[h] = -mu;
@@ -942,7 +962,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       // The difference first: the largest score's is 0 whatever its size.  (s * sl2 - m in
       // one instruction leaves what a maximum in log2 units lost in rounding: past 2^31 p
       // of all tokens is 0 or infinite.)
-      x = fmul2(fadd2(x, make_float2(nmu[0], nmu[1])), make_float2(sl2[0], sl2[1]));
+      x = fmul2(fadd2(x, make_float2(nmu[0], nmu[1])), sl2);
       x.x = ex2_mufu(x.x);
       x.y = ex2_mufu(x.y);
       sum = fadd2(sum, x);
@@ -1090,7 +1110,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     for (int h = 0; h < 2; ++h) {
       const int head = head0 + h;
       const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
-      const float ll = l[h] == 0.f ? -INFINITY : m[h] * sl2[h] * kLn2 + logf(l[h]);
+      const float ll = l[h] == 0.f ? -INFINITY : m[h] * s_q[8 * t + 6 + h] * kLn2 + logf(l[h]);
       const size_t orow = whole ? (size_t)b * Hkv * G + hkv * G + head : seg * G + head;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {

@@ -1167,3 +1167,22 @@ def test_tiny_queries_and_scales():
     for scale in (1e-6, 1e-9, 1e-11):
         O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, scale=scale)
         check_attention(f, q, O, L, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,dt,G", [(4, F16, 4), (8, F16, 8), (4, BF16, 8), (8, BF16, 3)], ids=str)
+@pytest.mark.parametrize("which", [0, 1])
+def test_query_groups_of_unequal_size(bits, dt, G, which):
+    """One group of 64 channels whose queries are a small part of the other's, and whose keys are
+    as much larger: both count for the scores."""
+    import b200attn
+    f = Filled(1, 2, 128, 16, bits, dt, [300], seed=277)
+    part = 1e-7 if dt == F16 else 1e-12
+    most = 1e3 if dt == F16 else 1e6
+    size = torch.full((128,), most)
+    size[64 * which:64 * which + 64] = part * most
+    q = (torch.from_numpy(ora.seeded_normal((1, 2 * G, 128), 279)) * size).to(dt).cuda()
+    with_values(f, k=(f.k[0].float() / size.cuda()).to(dt))
+    for splits in (None, 1, 3):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_own_steps(f, q, O, L)
