@@ -64,6 +64,7 @@ _SIGNATURES = {
     # q q_strides index index_scale bt lens keys pages
     # | B H Hkv D page max_pages num_pages top_k dtype | stream
     "b2a_kvq_select_pages": (_c_int, [_vp] * 8 + [_c_int] * 9 + [_vp]),
+    "b2a_kvq_select_keys_words": (ctypes.c_int64, [_c_int] * 3),
     "b2a_kvq_decode_workers": (_c_int, [_c_int] * 4 + [ctypes.c_int64]),
     "b2a_kvq_decode_workspace_floats": (ctypes.c_int64, [_c_int] * 5),
     # q q_strides data bt lens pages | n_pages | workspace o lse

@@ -282,6 +282,12 @@ def _check_query(q: torch.Tensor, cache: QuantCache):
     return q3, had_len, B, H, D
 
 
+@functools.lru_cache(maxsize=256)
+def _keys_words(B: int, Hkv: int, max_pages: int) -> int:
+    """Words of scratch that a selection needs."""
+    return _lib.load().b2a_kvq_select_keys_words(B, Hkv, max_pages)
+
+
 def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
                  kv_lens: torch.Tensor, top_k: int) -> torch.Tensor:
     """The top_k pages of every (sequence, KV head) for the queries q [B, H, D] (or
@@ -301,7 +307,8 @@ def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
         pages = kv_lens.new_empty(B, Hkv, int(top_k))
         if B == 0:
             return pages
-        keys = kv_lens.new_empty(B * Hkv * max_pages) if max_pages > 2048 else None
+        words = _keys_words(B, Hkv, max_pages)
+        keys = kv_lens.new_empty(words) if words else None
         qc, qs = _rows_of(q3, 2)
         _lib.check(_select(
             qc.data_ptr(), cache.index.data_ptr(), cache.index_scale.data_ptr(),

@@ -100,6 +100,7 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
                         const int32_t* kv_lens, uint32_t* keys, int32_t* pages, int B, int H,
                         int Hkv, int D, int page_size, int max_pages, int num_pages, int top_k,
                         int dtype, cudaStream_t stream);
+int64_t kvq_select_keys_words(int B, int Hkv, int max_pages);
 int kvq_decode_workers(int B, int Hkv, int D, int bits, long long max_tokens);
 int64_t kvq_decode_workspace_floats(int B, int H, int Hkv, int D, int workers);
 int kvq_decode_dispatch(const void* q, int64_t q_b, int64_t q_h, const void* data,

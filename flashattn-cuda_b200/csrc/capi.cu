@@ -561,11 +561,16 @@ int b2a_kvq_select_pages(const void* q, const int64_t* q_strides, const int8_t* 
   B2A_TRY(check_ptr_align(index_scale, "index_scale", 4));
   B2A_TRY(check_ptr_align(block_table, "block_table", 4));
   B2A_TRY(check_ptr_align(kv_lens, "kv_lens", 4));
-  if (max_pages > 2048) B2A_TRY(check_ptr_align(keys, "keys", 4));
+  if (max_pages > kvq::kFusedPages) B2A_TRY(check_ptr_align(keys, "keys", 4));
   B2A_TRY(check_ptr_align(pages, "pages", 4));
   return kvq_select_dispatch(q, q_strides[0], q_strides[1], index, index_scale, block_table,
                              kv_lens, keys, pages, B, H, Hkv, D, page_size, max_pages, num_pages,
                              top_k, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int64_t b2a_kvq_select_keys_words(int B, int Hkv, int max_pages) {
+  if (B <= 0 || Hkv <= 0 || max_pages <= 0) return 0;
+  return kvq_select_keys_words(B, Hkv, max_pages);
 }
 
 int b2a_kvq_decode_workers(int B, int Hkv, int D, int bits, int64_t max_tokens) {

@@ -14,6 +14,7 @@
 namespace b2a {
 namespace kvq {
 
+constexpr int kFusedPages = 2048;  // tables up to this width are selected from in one launch
 constexpr int kGroup = 64;  // channels sharing one (scale, min): 4.5 / 8.5 bits an element
 // Steps below this are stored as 0 (the group reads back as its min), so that
 // the reciprocal of a step is always a finite fp32.

@@ -393,10 +393,16 @@ __global__ void __launch_bounds__(THREADS)
 }
 
 // Scores and selection of tables of up to kFusedPages pages in one CTA, the keys
-// in shared memory: one launch, no trip through memory and the query rounded once
-// (256 tables of up to 1024 pages: 16.7 us, in two steps with CTAs of 256 pages
-// 20.8).
-constexpr int kFusedPages = 2048;
+// in shared memory: one launch, no trip through memory and the query rounded once.
+// The table's width decides, which the host knows; the lengths lie on the device.
+// Measured at D = 128, 4 heads a group, us in one CTA / in two steps:
+//   pages     100        300         1000        2048        4096        8192
+//   256 sets  7.1/16.3   10.2/19.7   17.9/26.5   35.8/46.8   64.7/85.4   -
+//   64 sets   -          8.6/10.6    13.5/11.3   21.3/14.8   39.7/24.5   88.0/44.5
+//   8 sets    -          8.4/8.6     12.7/8.6    20.4/9.7    36.9/11.6   67.5/13.7
+// (a set is a (sequence, KV head); past 2048 with the bound moved).  One CTA a set
+// fills the GPU where sets are many and is a long walk where they are few; 2048 caps
+// what that walk costs at 11 us.
 template <int D, int GP, bool BF16>
 __global__ void __launch_bounds__(32 * kScoreWarps, 2)
     score_select_kernel(const ScoreArgs a, int32_t* __restrict__ pages, int top_k) {
@@ -1337,10 +1343,18 @@ int kvq_select_dispatch(const void* q, int64_t q_b, int64_t q_h, const int8_t* i
   return B2A_OK;
 }
 
-// Warps that the GPU runs at a time; no more than there can be steps.
+int64_t kvq_select_keys_words(int B, int Hkv, int max_pages) {
+  return max_pages <= kvq::kFusedPages ? 0 : (int64_t)B * Hkv * max_pages;
+}
+
+// Warps that the GPU (148 SMs) runs at a time; no more than there can be steps.
+template <int D, int BITS>
+constexpr long long resident_warps() {
+  return 148ll * kvq::DecCfg<D, BITS>::kCtas * kvq::DecCfg<D, BITS>::kWarps;
+}
 int kvq_decode_workers(int B, int Hkv, int D, int bits, long long max_tokens) {
-  const long long resident =
-      148ll * (D == 128 && bits == 8 ? 3 * 2 : D == 64 && bits == 4 ? 4 * 4 : 3 * 4);
+  const long long resident = D == 64 ? (bits == 4 ? resident_warps<64, 4>() : resident_warps<64, 8>())
+                                     : (bits == 4 ? resident_warps<128, 4>() : resident_warps<128, 8>());
   const long long steps = (long long)B * Hkv * ((max_tokens + 63) / 64);
   return (int)(steps < resident ? steps : resident);
 }
@@ -1383,8 +1397,10 @@ static int launch_kvq_decode(const void* q, int64_t q_b, int64_t q_h, const uint
                              n_list, ws, l_part, meta, o, lse, B, G, Hkv, workers, by_tile,
                              page_shift, max_pages, num_pages, scale * kLog2e);
   if (e != cudaSuccess) return set_cuda_error(e, "quantised decode kernel launch");
-  // Few (sequence, KV head)s have many partials each: more warps for each.
-  // One sequence of 131072 tokens, 205 partials: 9 us with 4 warps, 6 with 16.
+  // Few (sequence, KV head)s have many partials each: more warps for each.  Decode
+  // and merge of 131072 tokens in all, 8 KV heads, us with 16 warps / with 4, by workers
+  // per (sequence, KV head): 222 46.8/48.8, 111 45.3/46.9, 56 45.5/47.8, 37 45.9/48.2,
+  // 28 45.7/46.6, 19 48.8/46.8, 14 49.0/46.1, 7 53.4/46.1.
   if (workers > 32 * tiles)
     e = launch_pdl(combine_kernel<D, 16, BF16>, dim3((unsigned)(tiles * G)), 512, 0, stream, ws,
                    l_part, meta, kv_lens, o, lse, G, Hkv, by_tile);

@@ -322,9 +322,10 @@ int b2a_kvq_read_paged(const void* data, const int32_t* block_table,
  * and each product rounded to fp32.  The last page of a sequence and any
  * score that is NaN count as +infinity; ties go to the lowest page.  q is
  * [B,H,D] with element strides {batch, head}, multiples of 8; H/Hkv <= 8.  keys
- * is scratch of B*Hkv*max_pages words (not used, and may be NULL, for
+ * is scratch of b2a_kvq_select_keys_words words (0, and keys may be NULL, for
  * max_pages <= 2048).
  */
+int64_t b2a_kvq_select_keys_words(int B, int Hkv, int max_pages);
 int b2a_kvq_select_pages(const void* q, const int64_t* q_strides,
                          const int8_t* index, const float* index_scale,
                          const int32_t* block_table, const int32_t* kv_lens,

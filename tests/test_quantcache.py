@@ -1186,3 +1186,16 @@ def test_query_groups_of_unequal_size(bits, dt, G, which):
     for splits in (None, 1, 3):
         O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
         check_own_steps(f, q, O, L)
+
+
+def test_scratch_and_warps_follow_the_kernels():
+    """Sizes that the host asks the library for, at the bounds where they change."""
+    from b200attn import _lib
+    from b200attn import quantcache as qc
+    lib = _lib.load()
+    assert lib.b2a_kvq_select_keys_words(3, 8, 2048) == 0 == qc._keys_words(3, 8, 2048)
+    assert lib.b2a_kvq_select_keys_words(3, 8, 2049) == 3 * 8 * 2049 == qc._keys_words(3, 8, 2049)
+    assert lib.b2a_kvq_select_keys_words(65535, 8, 1 << 20) == 65535 * 8 << 20
+    assert lib.b2a_kvq_select_keys_words(0, 8, 4096) == 0
+    for D, bits, warps in ((128, 4, 12), (128, 8, 6), (64, 4, 16), (64, 8, 12)):
+        assert lib.b2a_kvq_decode_workers(64, 8, D, bits, 1 << 20) == 148 * warps
