@@ -1199,3 +1199,99 @@ def test_scratch_and_warps_follow_the_kernels():
     assert lib.b2a_kvq_select_keys_words(0, 8, 4096) == 0
     for D, bits, warps in ((128, 4, 12), (128, 8, 6), (64, 4, 16), (64, 8, 12)):
         assert lib.b2a_kvq_decode_workers(64, 8, D, bits, 1 << 20) == 148 * warps
+
+
+@pytest.mark.gpu
+def test_captured_fork_and_join():
+    """A capture that forks: two caches' steps on two streams that meet in one decode each, and
+    a second join over both; replays give what the same calls give eagerly."""
+    import b200attn
+    B, H, Hkv, D = 2, 8, 2, 64
+    fs = [Filled(B, Hkv, D, 16, 4, F16, [300, 90], seed=287 + i, index=True, width=24) for i in (0, 1)]
+    x = torch.from_numpy(ora.seeded_normal((B, Hkv, 1, D), 289)).half().cuda()
+    q = torch.from_numpy(ora.seeded_normal((B, H, D), 290)).half().cuda()
+    at = fs[0].kl - 1
+    side = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        b200attn.append_paged_quant(x, x, fs[0].cache, fs[0].btg, at, advance=False)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b200attn.append_paged_quant(x, x, fs[1].cache, fs[1].btg, at, advance=False)
+            pages = b200attn.select_pages(q, fs[1].cache, fs[1].btg, fs[1].kl, 5)
+        first = b200attn.decode_paged_quant(q, fs[0].cache, fs[0].btg, fs[0].kl)
+        main.wait_stream(side)
+        return first + b200attn.decode_paged_quant(q, fs[1].cache, fs[1].btg, fs[1].kl, pages=pages) + [pages]
+
+    warm = torch.cuda.Stream()
+    with torch.cuda.stream(warm):
+        step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for it in range(3):
+        x.copy_(torch.from_numpy(ora.seeded_normal((B, Hkv, 1, D), 291 + it)).half())
+        q.copy_(torch.from_numpy(ora.seeded_normal((B, H, D), 295 + it)).half())
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, w in zip(got, step()):
+            torch.cuda.synchronize()
+            assert torch.equal(a, w)
+        for f in fs:
+            for b in range(B):
+                f.k[b][0, :, -1] = f.v[b][0, :, -1] = x[b, :, 0]
+        check_attention(fs[0], q, got[0], got[1])
+        check_attention(fs[1], q, got[2], got[3], pages=got[4].cpu().numpy())
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+def test_shared_pages_and_repeated_entries():
+    """Sequences that share the pages of a common beginning; a page that a list names twice."""
+    import b200attn
+    f = Filled(1, 2, 128, 16, 8, BF16, [64 + 21], seed=307)
+    extra = b200attn.QuantCache.empty(8, 16, 2, 128, bits=8, dtype=BF16)
+    extra.data[:f.cache.num_pages - 2] = f.cache.data[f.btg[0].long()]   # in order: 0 .. 5
+    bt = torch.tensor([[0, 1, 2, 3, 4, 5], [0, 1, 2, 3, 6, 7]], dtype=torch.int32, device="cuda")
+    kl = torch.tensor([85, 64], dtype=torch.int32, device="cuda")
+    k, v = (torch.from_numpy(ora.seeded_normal((1, 2, 21, 128), s)).bfloat16().cuda() for s in (308, 309))
+    b200attn.append_paged_quant(k, v, extra, bt[1:], kl[1:])
+    assert kl.tolist() == [85, 85]
+    q = torch.from_numpy(ora.seeded_normal((2, 4, 128), 310)).bfloat16().cuda()
+    both = Filled.__new__(Filled)
+    both.cache, both.lens, both.page, both.bits, both.dt, both.name = extra, [85, 85], 16, 8, BF16, "bfloat16"
+    both.k = [f.k[0], torch.cat((f.k[0][:, :, :64], k), 2)]
+    both.v = [f.v[0], torch.cat((f.v[0][:, :, :64], v), 2)]
+    O, L = b200attn.decode_paged_quant(q, extra, bt, kl)
+    check_attention(both, q, O, L)
+    lists = np.array([[[2, 2, 5, 0], [1, 4, 1, 1]], [[5, 5, 5, 5], [-1, 3, 3, 9]]], np.int32)
+    for splits in (None, 1, 3):
+        O, L = b200attn.decode_paged_quant(q, extra, bt, kl, pages=torch.from_numpy(lists).cuda(),
+                                           splits=splits)
+        check_attention(both, q, O, L, pages=lists)
+    assert b200attn.device_error_flags() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 7])
+def test_decode_without_lse(splits):
+    """The C entry with lse == NULL gives the same O."""
+    import ctypes
+    import b200attn
+    from b200attn import _lib
+    f = Filled(3, 2, 64, 16, 4, F16, [0, 300, 33], seed=317)
+    q = torch.from_numpy(ora.seeded_normal((3, 6, 64), 319)).half().cuda()
+    want = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+    lib = _lib.load()
+    workers = splits * 6
+    ws = torch.empty(lib.b2a_kvq_decode_workspace_floats(3, 6, 2, 64, workers), device="cuda")
+    O = torch.empty_like(q)
+    strides = (ctypes.c_int64 * 2)(6 * 64, 64)
+    _lib.check(lib.b2a_kvq_decode_paged(
+        q.data_ptr(), strides, f.cache.data.data_ptr(), f.btg.data_ptr(), f.kl.data_ptr(), None, 0,
+        ws.data_ptr(), O.data_ptr(), None, 3, 6, 2, 64, 16, f.btg.shape[1], f.cache.num_pages, workers,
+        4, 0, 0.125, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(O, want[0])
