@@ -16,6 +16,11 @@ namespace kvq {
 
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.4426950408889634f;
+// Exponentials are of scores less their maximum less kDown: values next to the
+// type's largest can be summed over 2^kDown tokens, or merged from as many warps,
+// before their sum is divided by that of the exponentials.  What that costs lies
+// below bf16's smallest normal number.
+constexpr float kDown = 16.f, kUp = 65536.f;
 constexpr uint64_t kDrainNs = 100000000ull;  // 0.1 s
 
 // The length of sequence b as the block table can hold it.
@@ -460,7 +465,11 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // takes no bits from the others, and the factor grows as the maximum does (o stays and
 // its unit changes), so what is left of early tokens takes none from later ones.  A
 // product within 2^-21 of the largest keeps fp16's 11 bits, one below is off by 2^-32
-// of the largest at most.
+// of the largest at most; V's codes lie at bits 0-3, and a sum of 16 tokens is off by
+// some 2^-14 of its largest product besides.
+//   Products are bounded by their value steps as long as that will do, and looked at
+// one by one where it will not (heavy tokens of small values beside large ones without
+// weight: in every step, 12% of the time; elsewhere in the first).
 //
 // The token dimension is M of both products (A = K codes [tok, d], and A =
 // V codes transposed [d, tok]) and the heads are N = 8, so no row of the
@@ -828,8 +837,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   // p * vscale of a head's group is multiplied by vmul before it is rounded; o
   // holds sums of such products.  Value steps are 0 or 2^-100 and more.
   alignas(8) float vmul[NG][2];
-  constexpr float kMaxMul = 1.298074214633707e33f;  // 2^110
+  constexpr float kMaxMul = 4.253529586511731e37f;  // 2^125
   constexpr float kMaxProduct = 32768.f;            // fp16 ends at 65504
+  constexpr float kMaxStep = kMaxProduct * kUp;     // p is at most 1 / kUp
   auto reset = [&]() {
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
@@ -968,7 +978,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       // The difference first: the largest score's is 0 whatever its size.  (s * sl2 - m in
       // one instruction leaves what a maximum in log2 units lost in rounding: past 2^31 p
       // of all tokens is 0 or infinite.)
-      x = fmul2(fadd2(x, make_float2(nmu[0], nmu[1])), sl2);
+      x = ffma2(fadd2(x, make_float2(nmu[0], nmu[1])), sl2, make_float2(-kDown, -kDown));
       x.x = ex2_mufu(x.x);
       x.y = ex2_mufu(x.y);
       sum = fadd2(sum, x);
@@ -986,17 +996,19 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       for (int k = 1; k < SL * R; ++k)
         big = __hmax2(big, *reinterpret_cast<T2*>(&vpar[k / R][k % R][gr]));
       vbig[gr] = Elem<BF16>::unpack(big).x;
-      look = look || vbig[gr] * fmaxf(vmul[gr][0], vmul[gr][1]) >= kMaxProduct;
+      look = look || vbig[gr] * fmaxf(vmul[gr][0], vmul[gr][1]) >= kMaxStep;
     }
     if (__any_sync(0xffffffffu, look)) {
       bool over = false;
+      float was[NG][2];
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          was[gr][h] = vmul[gr][h];
           omin[gr][h] *= alpha[h];
           vmul[gr][h] *= __fdividef(1.f, alpha[h]);  // infinite at a head's first token
-          over = over || vmul[gr][h] > kMaxMul || vbig[gr] * vmul[gr][h] >= kMaxProduct;
+          over = over || vmul[gr][h] > kMaxMul || vbig[gr] * vmul[gr][h] >= kMaxStep;
         }
       if (__any_sync(0xffffffffu, over)) {
         // The products themselves: where one is too large for vmul, the step's
@@ -1016,7 +1028,8 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
             const float old = vmul[gr][h];
             const float fit = fminf(pow2i(134 - (int)(__float_as_uint(top) >> 23)), kMaxMul);
             const bool fits = old <= kMaxMul && top * old < kMaxProduct;
-            f[h] = fits ? 1.f : __fdividef(fit, old);  // 0 for an infinite one
+            // fit / old, which may be infinite where was[][] / alpha is
+            f[h] = fits ? 1.f : alpha[h] == 0.f ? 0.f : __fdividef(fit, was[gr][h]) * alpha[h];
             vmul[gr][h] = fits ? old : fit;
           }
 #pragma unroll
@@ -1116,7 +1129,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     for (int h = 0; h < 2; ++h) {
       const int head = head0 + h;
       const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
-      const float ll = l[h] == 0.f ? -INFINITY : m[h] * s_q[8 * t + 6 + h] * kLn2 + logf(l[h]);
+      const float ll = l[h] == 0.f ? -INFINITY : m[h] * s_q[8 * t + 6 + h] * kLn2 + logf(l[h] * kUp);
       const size_t orow = whole ? (size_t)b * Hkv * G + hkv * G + head : seg * G + head;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
@@ -1265,7 +1278,7 @@ __global__ void __launch_bounds__(32 * NW)
     if (c0 > 0) __syncthreads();  // the previous chunk's weights are used
     for (int s = threadIdx.x; s < cn; s += 32 * NW) {
       const float x = lp[(size_t)(c0 + s) * G];
-      const float w = x == -INFINITY ? 0.f : expf(x - M);
+      const float w = x == -INFINITY ? 0.f : expf(x - M) * (1.f / kUp);
       s_w[s] = w;
       L += w;
     }
@@ -1297,7 +1310,7 @@ __global__ void __launch_bounds__(32 * NW)
     for (int k = 0; k < STEP; ++k) a += reinterpret_cast<const float*>(s_acc[k])[threadIdx.x];
     static_cast<T1*>(out)[row * D + threadIdx.x] = Elem<BF16>::from(L == 0.f ? 0.f : a / L);
   }
-  if (threadIdx.x == 0 && lse != nullptr) lse[row] = L == 0.f ? -INFINITY : M + logf(L);
+  if (threadIdx.x == 0 && lse != nullptr) lse[row] = L == 0.f ? -INFINITY : M + logf(L * kUp);
 }
 
 }  // namespace kvq

@@ -913,7 +913,8 @@ def check_own_steps(f, q, O, L):
     enters except by its weight.  A product p * step is rounded to fp16 in a unit that brings the
     largest product of its head and group to 2^7 or more, so where it falls into the subnormals
     half of their spacing is 2^-25 * 2^-7 of that largest product (and it multiplies |code - mid|,
-    at most 2^(bits - 1)).  A unit is at least 2^-110: with 2^-25, nothing beside 2^-133."""
+    at most 2^(bits - 1)).  No unit is below 2^-125, of weights that are at most 2^-16: with 2^-25
+    that is 2^-134, half of bf16's smallest number."""
     u = torch.finfo(f.dt).eps / 2
     Hkv = f.cache.num_kv_heads
     G = q.shape[1] // Hkv
@@ -1295,3 +1296,67 @@ def test_decode_without_lse(splits):
         ws.data_ptr(), O.data_ptr(), None, 3, 6, 2, 64, 16, f.btg.shape[1], f.cache.num_pages, workers,
         4, 0, 0.125, torch.cuda.current_stream().cuda_stream))
     assert torch.equal(O, want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,bits,dt,G", RANGE, ids=str)
+@pytest.mark.parametrize("n", [3, 70, 3000])
+def test_values_next_to_the_largest(D, bits, dt, G, n):
+    """Values up to the type's largest: their weighted mean is finite, whatever the sums of their
+    products with unnormalised weights are."""
+    import b200attn
+    big = torch.finfo(dt).max
+    f = Filled(1, 2, D, 16, bits, dt, [n], seed=327)
+    g = torch.Generator().manual_seed(n)
+    v = (1 - 0.3 * torch.rand(1, 2, n, D, generator=g)) * big
+    v[..., 1::3] *= -1
+    v[:, :, 0, 0] = big
+    with_values(f, v=v.to(dt).cuda(), k=f.k[0] * 0.1)       # weights all alike
+    q = torch.from_numpy(ora.seeded_normal((1, 2 * G, D), 329)).to(dt).cuda()
+    for splits in (None, 1, 7):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        assert torch.isfinite(O).all()
+        check_own_steps(f, q, O, L)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,G", [(4, 4), (8, 8)])
+def test_values_next_to_the_smallest_steps(bits, G):
+    """Values whose steps are next to 2^-100, the smallest that are kept, and zeros among them;
+    scores of one size, and some that rise and fall by 40."""
+    import b200attn
+    for power, rise in ((-80, 0), (-92, 0), (-97, 0), (-80, 40), (-92, 40), (-92, -40), (-97, 40),
+                        (-101, 0), (-101, 40), (-101, -40)):
+        f = Filled(1, 1, 128, 16, bits, BF16, [400], seed=337)
+        v = f.v[0].float() * 2.0 ** (power + bits)
+        v[:, :, 100:140] = 0
+        v[:, :, :, 64:] *= 2.0 ** -4
+        q = torch.from_numpy(ora.seeded_normal((1, G, 128), 339))
+        q = (q if rise == 0 else 0.5 + 0.3 * q).bfloat16().cuda()
+        ramp = torch.linspace(0, 1, 400)[None, None, :, None].cuda() * 2 * rise / 128 ** 0.5
+        with_values(f, v=v.to(BF16), k=(f.k[0].float() * (0.2 if rise else 1) + ramp).to(BF16))
+        for splits in (None, 1, 5):
+            O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+            check_own_steps(f, q, O, L)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(6))
+def test_values_spread_over_the_range(seed):
+    """Values whose size differs from token to token by up to 10^70 (bf16) or 10^8 (fp16), up to
+    the type's largest: whatever counts at a head's end is there."""
+    import b200attn
+    rng = np.random.default_rng(seed)
+    D, bits, dt, G = RANGE[seed]
+    n = 900
+    f = Filled(1, 2, D, 64, bits, dt, [n], seed=347 + seed)
+    ten = rng.uniform(-38, 38, (1, 2, n, 1)) if dt == BF16 else rng.uniform(-4, 4.5, (1, 2, n, 1))
+    if seed & 1:                                   # most of them small, a few at the upper end
+        ten = np.where(rng.random(ten.shape) < 0.02, ten, ten.min() / 2)
+    big = torch.finfo(dt).max
+    v = f.v[0].double() * 10.0 ** torch.from_numpy(ten).cuda()
+    with_values(f, v=v.clamp(-big, big).to(dt))
+    q = torch.from_numpy(ora.seeded_normal((1, 2 * G, D), 349)).to(dt).cuda()
+    for splits in (None, 1, 4):
+        O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+        check_own_steps(f, q, O, L)
