@@ -596,6 +596,9 @@ int b2a_kvq_decode_paged(const void* q, const int64_t* q_strides, const void* da
   if (pages != nullptr && (n_pages <= 0 || (int64_t)n_pages * page_size > 0x7fff0000))
     return set_error(B2A_ERR_INVALID_ARG, "n_pages must be > 0 and n_pages * page_size < 2^31");
   if ((int64_t)B * H > 0x7fffffff / 2) return set_error(B2A_ERR_INVALID_ARG, "B*H too large");
+  const int64_t cap = (int64_t)(pages != nullptr ? n_pages : max_pages) * page_size;
+  if ((int64_t)B * Hkv * ((cap + 63) / 64) > ((int64_t)workers << 28))  // a worker's steps are an int
+    return set_error(B2A_ERR_INVALID_ARG, "too few workers (splits) for this many tokens");
   if ((int64_t)num_pages * Hkv > 0x7fffffff)
     return set_error(B2A_ERR_INVALID_ARG, "num_pages * Hkv too large");
   if (!(scale > 0.f)) return set_error(B2A_ERR_INVALID_ARG, "scale must be > 0");

@@ -342,7 +342,7 @@ int b2a_kvq_select_pages(const void* q, const int64_t* q_strides,
  * page listed twice counts twice).  The tokens of all sequences are divided
  * evenly among `workers` warps whatever the lengths; b2a_kvq_decode_workers
  * gives the number that fills the GPU, max_tokens being the most that one
- * sequence can attend to, and b2a_kvq_decode_workspace_floats the scratch that
+ * sequence can attend to (a worker takes at most 2^28 * 64 tokens), and b2a_kvq_decode_workspace_floats the scratch that
  * a call needs.  A bad block-table entry sets bit 1 of the device error word
  * and reads page 0 instead.  H/Hkv <= 8.
  */

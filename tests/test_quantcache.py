@@ -1360,3 +1360,19 @@ def test_values_spread_over_the_range(seed):
     for splits in (None, 1, 4):
         O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
         check_own_steps(f, q, O, L)
+
+
+@pytest.mark.gpu
+def test_too_few_workers_for_the_table():
+    """A worker counts its steps in 32 bits: a call that could pass that is refused."""
+    from b200attn import _lib
+    from b200attn import quantcache as qc
+    # q data table lens pages | n_pages | workspace o lse | B H Hkv D page max_pages num_pages workers bits dtype
+    args = [0] * 5 + [0] + [0] * 3 + [65535, 64, 8, 64, 64, 1 << 24, 100, 1, 4, 0, 0, 64, 64, 0.125]
+    for f in (qc._decode, qc._decode_ct):
+        with pytest.raises(RuntimeError, match="too few workers"):
+            _lib.check(f(*args))
+        args[16] = 65535 * 8
+        with pytest.raises(RuntimeError, match="q must not be null"):
+            _lib.check(f(*args))
+        args[16] = 1
