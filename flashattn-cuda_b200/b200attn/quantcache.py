@@ -293,7 +293,7 @@ def select_pages(q: torch.Tensor, cache: QuantCache, block_table: torch.Tensor,
     """The top_k pages of every (sequence, KV head) for the queries q [B, H, D] (or
     [B, H, 1, D]): int32 [B, Hkv, top_k], logical page numbers, ascending, -1 behind the
     last.  A page's score is an upper bound, from the cache's index, of its keys' products
-    with the group's query heads, in 8 bits (b2a_kvq_select_pages)."""
+    with the group's query heads, in 8 bits (b2a_kvq_select_pages).  Groups of up to 8 heads."""
     q3, _, B, H, D = _check_query(q, cache)
     if cache.index is None:
         raise RuntimeError("select_pages needs a cache with an index")
@@ -334,7 +334,7 @@ def decode_paged_quant(q: torch.Tensor, cache: QuantCache, block_table: torch.Te
                        pages: Optional[torch.Tensor] = None,
                        splits: Optional[int] = None) -> list:
     """Decode attention over a quantised cache: [O, L] shaped like q ([B, H, D] or
-    [B, H, 1, D]); kv_lens may hold zeros (O = 0, L = -inf).  `pages` int32 [B, Hkv, n]
+    [B, H, 1, D], H / Hkv at most 8); kv_lens may hold zeros (O = 0, L = -inf).  `pages` int32 [B, Hkv, n]
     (from select_pages) restricts each KV head to those pages; negative entries are skipped.
     `splits` overrides the number of warps that share the work, as a multiple of B * Hkv."""
     q3, had_len, B, H, D = _check_query(q, cache)

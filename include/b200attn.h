@@ -278,15 +278,23 @@ int64_t b2a_kvq_block_bytes(int D, int page_size, int bits);
  * its length stays; no length is advanced past 2^31 - 1.  k_new, v_new are
  * [B,Hkv,T,D] with element strides k_strides / v_strides = {batch, head,
  * token}, multiples of 8; rows are contiguous and 16-byte aligned.
- *   With n = 2^bits - 1 and a group's extremes lo, hi: scale = (hi - lo)/n
- * rounded up to dtype (down where lo + n*scale would leave its range; 0 below
- * 2^-100), min = lo, code = rint((x - lo)/scale), each step in fp32: the codes
- * are the same to the bit on every call.  A group that holds a NaN or an
- * infinity reads back as NaN.
+ *   With n = 2^bits - 1 and a group's extremes lo, hi, in fp32 and rounded to
+ * nearest even at each step that rounds:
+ *   w     = (hi/2 - lo/2) * c, c being 2/n rounded to fp32
+ *   scale = w rounded up to dtype; rounded down where lo + n*scale, rounded
+ *           once to dtype, would be infinite; 0 where that is below 2^-100
+ *   min   = lo
+ *   r     = 1 / (scale/2)
+ *   code  = min(rint((x/2 - lo/2) * r), n), 0 for a scale of 0
+ * so a product with a reciprocal and not a division: near a tie the two give
+ * different codes.  The bits are the same on every call.  A group that holds a
+ * NaN or an infinity has scale = min = NaN and codes 0, and reads back as NaN.
  *   With index != NULL the bounds of every page that is written to are set
  * from all its tokens (those already there are read back): symmetric int8
- * codes of the read-back keys' minima and maxima with one scale.  A page must
- * not appear twice among the pages written by one call.
+ * codes of the read-back keys' minima and maxima with one scale, the largest
+ * magnitude times 1/127 rounded to fp32; code = rint(v * (1/scale)), 0 for a
+ * scale below 2^-100, and scale NaN, codes 0 where a bound is not finite.  A
+ * page must not appear twice among the pages written by one call.
  */
 int b2a_kvq_append_paged(const void* k_new, const void* v_new,
                          const int64_t* k_strides, const int64_t* v_strides,
@@ -318,8 +326,9 @@ int b2a_kvq_read_paged(const void* data, const int32_t* block_table,
  * [B, Hkv, top_k] int32, logical page numbers in ascending order, -1 behind
  * the last.  Query heads are rounded to int8 with one scale each; a page's
  * score is the largest, over the group's heads, of
- * (sum_d max(q8*min8, q8*max8) * q_scale) * index_scale, with the sum exact
- * and each product rounded to fp32.  The last page of a sequence and any
+ * (sum_d (q8 > 0 ? q8*max8 : q8*min8) * q_scale) * index_scale, with the sum
+ * exact and each product rounded to fp32 (a minimum above its maximum is
+ * outside the format, and no append writes one).  The last page of a sequence and any
  * score that is NaN count as +infinity; ties go to the lowest page.  q is
  * [B,H,D] with element strides {batch, head}, multiples of 8; H/Hkv <= 8.  keys
  * is scratch of b2a_kvq_select_keys_words words (0, and keys may be NULL, for
