@@ -793,6 +793,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       shift[1] = min(shift[1], least + 30);
       fac = pow2i(shift[0] - shift[1]);
     }
+    __syncwarp();  // every lane is done with the last head's
     float* mine = s_q + (g >> 1) * 8 + (g & 1);  // column g's, written by one of its lanes
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
