@@ -462,11 +462,11 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // sums meet in fp32), and p*vscale by a running factor of its own for each head and
 // group, which at the last change brought the step's largest product to [2^7, 2^8).
 // That goes by the products, so a token whose values are large but that has no weight
-// takes no bits from the others, and the factor grows as the maximum does (o stays and
-// its unit changes), so what is left of early tokens takes none from later ones.  A
-// product within 2^-21 of the largest keeps fp16's 11 bits, one below is off by 2^-32
-// of the largest at most; V's codes lie at bits 0-3, and a sum of 16 tokens is off by
-// some 2^-14 of its largest product besides.
+// takes no bits from the others, and the factor grows as the maximum does, so what is
+// left of early tokens takes none from later ones.  A product within 2^-21 of the
+// largest keeps fp16's 11 bits, one below is off by 2^-32 of the largest at most; V's
+// codes lie at bits 0-3, and a sum of 16 tokens is off by some 2^-14 of its largest
+// product besides.
 //   Products are bounded by their value steps as long as that will do, and looked at
 // one by one where it will not (heavy tokens of small values beside large ones without
 // weight: in every step, 12% of the time; elsewhere in the first).
@@ -557,6 +557,10 @@ __device__ __forceinline__ void unpack4_bytes(uint32_t x, uint32_t* r) {
 }
 // two neighbours of an array as a pair, for the two-wide fp32 instructions
 __device__ __forceinline__ float2& pair(float* x) { return *reinterpret_cast<float2*>(x); }
+// the power of two in x > 0
+__device__ __forceinline__ float pow2_of(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0x7f800000u);
+}
 // 2^e as fp32, e clamped to the normal range
 __device__ __forceinline__ float pow2i(int e) {
   return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
@@ -835,8 +839,11 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   alignas(16) float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
   alignas(8) float omin[NG][2];  // sum of p * (vmin + mid * vscale) over this lane's tokens
   float m[2], l[2];  // the largest score, in the units of S, and the sum of p
-  // p * vscale of a head's group is multiplied by vmul before it is rounded; o
-  // holds sums of such products.  Value steps are 0 or 2^-100 and more.
+  // p * vscale of a head's group is multiplied by vmul's power of two before it is
+  // rounded; o holds sums of such products.  A power of two, for the product of a head's
+  // largest score is then its step, which is not rounded (vmul itself as the factor:
+  // error of fp16 outputs over 16000 tokens 2.96e-4, so 2.75e-4).  Steps are 0 or 2^-100
+  // and more.
   alignas(8) float vmul[NG][2];
   constexpr float kMaxMul = 4.253529586511731e37f;  // 2^125
   constexpr float kMaxProduct = 32768.f;            // fp16 ends at 65504
@@ -986,8 +993,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     }
     l[0] = fmaf(l[0], alpha[0], sum.x);
     l[1] = fmaf(l[1], alpha[1], sum.y);
-    // Where a maximum rises o stays, and vmul grows by what p of the tokens so far
-    // shrink by.  Products are bounded by their steps alone as long as that will do.
+    // Where a maximum rises, vmul grows by what p of the tokens so far shrink by, and o
+    // takes what of that is no power of two.  Products are bounded by their steps alone
+    // as long as that will do.
     float vbig[NG];  // largest value step of this lane's tokens
     bool look = moved;
 #pragma unroll
@@ -1002,21 +1010,24 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     if (__any_sync(0xffffffffu, look)) {
       bool over = false;
       float was[NG][2];
+      alignas(8) float f[NG][2];
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          was[gr][h] = vmul[gr][h];
           omin[gr][h] *= alpha[h];
+          was[gr][h] = pow2_of(vmul[gr][h]);
           vmul[gr][h] *= __fdividef(1.f, alpha[h]);  // infinite at a head's first token
+          const float now = pow2_of(vmul[gr][h]);
+          f[gr][h] = alpha[h] * __uint_as_float(__float_as_uint(now) - __float_as_uint(was[gr][h]) +
+                                                0x3f800000u);  // now / was
           over = over || vmul[gr][h] > kMaxMul || vbig[gr] * vmul[gr][h] >= kMaxStep;
         }
       if (__any_sync(0xffffffffu, over)) {
         // The products themselves: where one is too large for vmul, the step's
         // largest goes to [2^7, 2^8).
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          float f[2];
+        for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float top = 0.f;
@@ -1028,20 +1039,27 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             const float old = vmul[gr][h];
             const float fit = fminf(pow2i(134 - (int)(__float_as_uint(top) >> 23)), kMaxMul);
-            const bool fits = old <= kMaxMul && top * old < kMaxProduct;
-            // fit / old, which may be infinite where was[][] / alpha is
-            f[h] = fits ? 1.f : alpha[h] == 0.f ? 0.f : __fdividef(fit, was[gr][h]) * alpha[h];
-            vmul[gr][h] = fits ? old : fit;
+            if (!(old <= kMaxMul && top * old < kMaxProduct)) {
+              vmul[gr][h] = fit;
+              f[gr][h] = alpha[h] == 0.f ? 0.f : __fdividef(fit, was[gr][h]) * alpha[h];
+            }
           }
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            for (int e = 0; e < 4; e += 2)
-              pair(&o[gr][k][e]) = fmul2(pair(&o[gr][k][e]), make_float2(f[0], f[1]));
-        }
       }
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          for (int e = 0; e < 4; e += 2)
+            pair(&o[gr][k][e]) = fmul2(pair(&o[gr][k][e]), pair(f[gr]));
     }
 
     // ---- O += V^T P
+    alignas(8) float mul[NG][2];
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) {
+      mul[gr][0] = pow2_of(vmul[gr][0]);
+      mul[gr][1] = pow2_of(vmul[gr][1]);
+    }
     alignas(16) float psum[NG][4];  // sums of the rounded p * vscale over the step
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) psum[gr][0] = psum[gr][1] = psum[gr][2] = psum[gr][3] = 0.f;
@@ -1060,7 +1078,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
           omin[gr][0] = fmaf(s[sl][r][0], vmid, omin[gr][0]);
           omin[gr][1] = fmaf(s[sl][r][1], vmid, omin[gr][1]);
           // vmul last: vscale * vmul may pass fp32 where p is next to nothing
-          const float2 w = fmul2(make_float2(s[sl][r][0] * pr.x, s[sl][r][1] * pr.x), pair(vmul[gr]));
+          const float2 w = fmul2(make_float2(s[sl][r][0] * pr.x, s[sl][r][1] * pr.x), pair(mul[gr]));
           pb[r] = movmatrix_trans(pack2_u32<false>(w.x, w.y));
         }
         if constexpr (HALF) {  // columns 0-3: tokens 0-7 of the slab, columns 4-7: tokens 8-15
@@ -1134,7 +1152,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       const size_t orow = whole ? (size_t)b * Hkv * G + hkv * G + head : seg * G + head;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        const float unit = __fdividef(1.f, vmul[gr][h]);
+        const float unit = __fdividef(1.f, pow2_of(vmul[gr][h]));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float x = o[gr][k][h], y = o[gr][k][2 + h];

@@ -1376,3 +1376,51 @@ def test_too_few_workers_for_the_table():
         with pytest.raises(RuntimeError, match="q must not be null"):
             _lib.check(f(*args))
         args[16] = 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_scores_creep_up_while_values_shrink(bits):
+    """The maximum rises by less than one at every step and the values shrink by as much or more:
+    what o holds and what its products are scaled by stay together over many small changes."""
+    import b200attn
+    n = 64 * 120
+    f = Filled(1, 1, 64, 64, bits, BF16, [n], seed=357)
+    q = torch.ones(1, 4, 64, dtype=BF16, device="cuda")
+    rise = torch.arange(n).float()[None, None, :, None].cuda() / 64 * 0.4     # in all 48
+    k = (0.05 * f.k[0].float() + rise / 8).to(BF16)
+    for fall in (0.4, 1.2):
+        with_values(f, v=(f.v[0].float() * torch.exp(30 - rise * fall / 0.4 * 0.8)).to(BF16), k=k)
+        for splits in (1, 2, 9):
+            O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl, splits=splits)
+            check_own_steps(f, q, O, L)
+
+
+@pytest.mark.gpu
+def test_the_heaviest_token_is_not_rounded():
+    """fp16 outputs' mean square error is that of one rounding of O and one of each product p *
+    step but the heaviest token's, which is its step times a power of two.
+
+    A rounding to a spacing h has mean square h^2 / 12.  For O the spacing is known,
+    2^(floor(log2 |O|) - 10).  A product x in [2^e, 2^(e+1)) has h = 2^(e - 10), and its mantissa,
+    that of an exponential, is spread evenly over its logarithm: the mean of (2^e / x)^2 is
+    (3 / 8) / ln 2 and the mean square 2^-20 / 12 * 0.541 of x^2.  Over 2^16 outputs, of which the
+    64 channels of a head share their products' errors, the sum is within some percent of that."""
+    import b200attn
+    f = Filled(8, 4, 128, 16, 8, F16, [4000] * 8, seed=367)
+    q = torch.from_numpy(ora.seeded_normal((8, 16, 128), 369) * 3).half().cuda()
+    O, L = b200attn.decode_paged_quant(q, f.cache, f.btg, f.kl)
+    got = result = products = 0.0
+    for b in range(8):
+        K, V = (f.codes(b, s) for s in (0, 1))
+        for h in range(4):
+            k, v = oq.values(*(x[h] for x in K)), oq.values(*(x[h] for x in V))
+            Or, Lr = oq.attend(np_of(q)[b, 4 * h:4 * h + 4], k, v, 128 ** -0.5)
+            s = np_of(q)[b, 4 * h:4 * h + 4].astype(np.float64) @ k.T * 128 ** -0.5
+            p = np.exp(s - Lr[:, None])
+            p[np.arange(4), p.argmax(-1)] = 0
+            off = np.repeat(V[1][h].astype(np.float64), 64, -1) * (V[0][h] - 128.0)
+            got += ((np_of(O)[b, 4 * h:4 * h + 4] - Or) ** 2).sum()
+            result += (2.0 ** (2 * np.floor(np.log2(np.abs(Or))) - 20) / 12).sum()
+            products += (p ** 2 @ off ** 2).sum() * 2.0 ** -20 / 12 * 0.375 / np.log(2)
+    assert got <= 1.04 * (result + products), (got, result, products)
