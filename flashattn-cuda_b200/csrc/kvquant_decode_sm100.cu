@@ -511,7 +511,8 @@ struct DecCfg {
   static constexpr int kOffValid = kOffBar + kWarps * kStages * 8;    // [warp][stage] int4
   static constexpr int kOffAbort = kOffValid + kWarps * kStages * 16;  // [warp] int
   static constexpr int kOffQuery = (kOffAbort + kWarps * 4 + 15) / 16 * 16;  // [warp][4][8] float
-  static constexpr int kSmem = kOffQuery + kWarps * 128;
+  static constexpr int kOffLag = kOffQuery + kWarps * 128;  // [thread] float2
+  static constexpr int kSmem = kOffLag + kWarps * 256;
 };
 
 // D[16x8] += A[16x16] B[16x8], fp16 operands, fp32 accumulators
@@ -839,18 +840,20 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   alignas(16) float o[NG][4][4];  // [group][tile][(d even, column 2t), (even, 2t+1), (odd, 2t), (odd, 2t+1)]
   alignas(8) float omin[NG][2];  // sum of p * (vmin + mid * vscale) over this lane's tokens
   float m[2], l[2];  // the largest score, in the units of S, and the sum of p
-  // p * vscale of a head's group is multiplied by vmul's power of two before it is
-  // rounded; o holds sums of such products.  A power of two, for the product of a head's
-  // largest score is then its step, which is not rounded (vmul itself as the factor:
-  // error of fp16 outputs over 16000 tokens 2.96e-4, so 2.75e-4).  Steps are 0 or 2^-100
-  // and more.
+  // p * vscale of a head's group is multiplied by vmul before it is rounded; o holds
+  // sums of such products.  A power of two, for the product of a head's largest score is
+  // then its step, which is not rounded (with any other factor the error of fp16 outputs
+  // over 16000 tokens is 2.96e-4, so 2.75e-4); lag is what vmul is behind the growth of
+  // the maximum, 1 to 2.  Steps are 0 or 2^-100 and more.
   alignas(8) float vmul[NG][2];
+  float2* s_lag = reinterpret_cast<float2*>(smem + C::kOffLag) + threadIdx.x;
   constexpr float kMaxMul = 4.253529586511731e37f;  // 2^125
   constexpr float kMaxProduct = 32768.f;            // fp16 ends at 65504
   constexpr float kMaxStep = kMaxProduct * kUp;     // p is at most 1 / kUp
   auto reset = [&]() {
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
+    *s_lag = make_float2(1.f, 1.f);
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
       omin[gr][0] = omin[gr][1] = 0.f;
@@ -875,19 +878,19 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
   const int tok = (g >> 1) + (g & 1) * 4;  // S row g is token `tok` of the slab, row g+8 8 later
   const int vtok = HALF ? tok + 8 * half : tok;  // the first token whose p this lane holds
 
-  // One step; nv: tokens of each slab.  FULL: all of them, known by the caller,
-  // which leaves one run of straight code whose slabs overlap.
-  auto step = [&](auto all, const uint8_t* stage, const int (&nv)[4]) {
+  // The scores of a step; nvs: tokens of each slab.  FULL: all of them, known by the
+  // caller, which leaves one run of straight code whose slabs overlap.
+  alignas(16) float s[SL][R][2];
+  uint32_t vpar[SL][R][NG];  // (scale, min) of V of this lane's rows
+  auto scores = [&](auto all, const uint8_t* stage, const int4 nvs) {
     constexpr bool FULL = decltype(all)::value;
+    const int nv[4] = {nvs.x, nvs.y, nvs.z, nvs.w};
 
     const float4 qa = *reinterpret_cast<const float4*>(s_q + 8 * t);
-    const float4 qc = *reinterpret_cast<const float4*>(s_q + 8 * t + 4);
     const float2 qsum[2] = {make_float2(qa.x, qa.y), make_float2(qa.z, qa.w)};
-    const float2 qfac = make_float2(qc.x, qc.y), sl2 = make_float2(qc.z, qc.w);
+    const float2 qfac = *reinterpret_cast<const float2*>(s_q + 8 * t + 4);
 
     // ---- S = K q^T
-    alignas(16) float s[SL][R][2];
-    uint32_t vpar[SL][R][NG];  // (scale, min) of V of this lane's rows
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
       if (!FULL && nv[sl] == 0) {  // the same in every lane
@@ -961,6 +964,14 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
           }
       }
     }
+  };
+  // One step.  What follows the scores is there once, for partial steps too, whose
+  // tokens past the end weigh nothing: twice the code costs sequences of a few steps
+  // more in instruction fetches (2048 of 100 to 200 tokens: 201 us, so 181).
+  auto step = [&](const uint8_t* stage, bool whole, const int4 nvs) {
+    if (whole) scores(std::true_type{}, stage, nvs);
+    else scores(std::false_type{}, stage, nvs);
+    const float2 sl2 = *reinterpret_cast<const float2*>(s_q + 8 * t + 6);
 
     // ---- online softmax, per head over the step's tokens
     float alpha[2], nmu[2];
@@ -1009,41 +1020,53 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     }
     if (__any_sync(0xffffffffu, look)) {
       bool over = false;
+      const float2 lag2 = *s_lag;
+      float lag[2] = {lag2.x, lag2.y};
       float was[NG][2];
       alignas(8) float f[NG][2];
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
+      for (int h = 0; h < 2; ++h) {
+        const float grow = lag[h] * __fdividef(1.f, alpha[h]);  // infinite at a head's first token
+        const float up = pow2_of(grow);
+        lag[h] = __uint_as_float((__float_as_uint(grow) & 0x7fffffu) | 0x3f800000u);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int gr = 0; gr < NG; ++gr) {
           omin[gr][h] *= alpha[h];
-          was[gr][h] = pow2_of(vmul[gr][h]);
-          vmul[gr][h] *= __fdividef(1.f, alpha[h]);  // infinite at a head's first token
-          const float now = pow2_of(vmul[gr][h]);
-          f[gr][h] = alpha[h] * __uint_as_float(__float_as_uint(now) - __float_as_uint(was[gr][h]) +
-                                                0x3f800000u);  // now / was
+          f[gr][h] = alpha[h] * up;
+          was[gr][h] = vmul[gr][h];
+          vmul[gr][h] *= up;
           over = over || vmul[gr][h] > kMaxMul || vbig[gr] * vmul[gr][h] >= kMaxStep;
         }
+      }
+      *s_lag = make_float2(lag[0], lag[1]);
       if (__any_sync(0xffffffffu, over)) {
-        // The products themselves: where one is too large for vmul, the step's
-        // largest goes to [2^7, 2^8).
+        // The products themselves (bf16 has their range and bits enough): where one is
+        // too large for vmul, the step's largest goes to [2^7, 2^8).
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
+        for (int gr = 0; gr < NG; ++gr) {
+          uint32_t top2 = 0u;  // of both heads, in bf16
+          auto larger = [&](uint32_t w) {
+            const __nv_bfloat162 y = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&top2),
+                                             *reinterpret_cast<__nv_bfloat162*>(&w));
+            top2 = *reinterpret_cast<const uint32_t*>(&y);
+          };
+#pragma unroll
+          for (int k = 0; k < SL * R; ++k) {
+            const float vs = param<BF16>(vpar[k / R][k % R][gr]).x;
+            larger(pack2_u32<true>(s[k / R][k % R][0] * vs, s[k / R][k % R][1] * vs));
+          }
+#pragma unroll
+          for (int x = HALF ? 2 : 4; x < 32; x <<= 1) larger(__shfl_xor_sync(0xffffffffu, top2, x));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float top = 0.f;
-#pragma unroll
-            for (int k = 0; k < SL * R; ++k)
-              top = fmaxf(top, s[k / R][k % R][h] * param<BF16>(vpar[k / R][k % R][gr]).x);
-#pragma unroll
-            for (int x = HALF ? 2 : 4; x < 32; x <<= 1)
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float old = vmul[gr][h];
-            const float fit = fminf(pow2i(134 - (int)(__float_as_uint(top) >> 23)), kMaxMul);
-            if (!(old <= kMaxMul && top * old < kMaxProduct)) {
-              vmul[gr][h] = fit;
-              f[gr][h] = alpha[h] == 0.f ? 0.f : __fdividef(fit, was[gr][h]) * alpha[h];
+            const float top = __uint_as_float(h ? top2 & 0xffff0000u : top2 << 16);
+            if (!(vmul[gr][h] <= kMaxMul && top * vmul[gr][h] < kMaxProduct)) {
+              const int fit = max(min(261 - (int)(__float_as_uint(top) >> 23), 252), 1);  // biased
+              f[gr][h] = alpha[h] * pow2i(fit - (int)(__float_as_uint(was[gr][h]) >> 23));
+              vmul[gr][h] = __uint_as_float((uint32_t)fit << 23);
             }
           }
+        }
       }
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr)
@@ -1054,18 +1077,11 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     }
 
     // ---- O += V^T P
-    alignas(8) float mul[NG][2];
-#pragma unroll
-    for (int gr = 0; gr < NG; ++gr) {
-      mul[gr][0] = pow2_of(vmul[gr][0]);
-      mul[gr][1] = pow2_of(vmul[gr][1]);
-    }
     alignas(16) float psum[NG][4];  // sums of the rounded p * vscale over the step
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) psum[gr][0] = psum[gr][1] = psum[gr][2] = psum[gr][3] = 0.f;
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
-      if (!FULL && nv[sl] == 0) continue;
       const uint8_t* vc =
           stage + v_off + (sl >> 1) * code_hi + (sl & 1) * code_lo + g * BITS + t * ROW;
 #pragma unroll
@@ -1078,7 +1094,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
           omin[gr][0] = fmaf(s[sl][r][0], vmid, omin[gr][0]);
           omin[gr][1] = fmaf(s[sl][r][1], vmid, omin[gr][1]);
           // vmul last: vscale * vmul may pass fp32 where p is next to nothing
-          const float2 w = fmul2(make_float2(s[sl][r][0] * pr.x, s[sl][r][1] * pr.x), pair(mul[gr]));
+          const float2 w = fmul2(make_float2(s[sl][r][0] * pr.x, s[sl][r][1] * pr.x), pair(vmul[gr]));
           pb[r] = movmatrix_trans(pack2_u32<false>(w.x, w.y));
         }
         if constexpr (HALF) {  // columns 0-3: tokens 0-7 of the slab, columns 4-7: tokens 8-15
@@ -1152,7 +1168,7 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
       const size_t orow = whole ? (size_t)b * Hkv * G + hkv * G + head : seg * G + head;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        const float unit = __fdividef(1.f, pow2_of(vmul[gr][h]));
+        const float unit = __fdividef(1.f, vmul[gr][h]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float x = o[gr][k][h], y = o[gr][k][2 + h];
@@ -1199,14 +1215,9 @@ __global__ void __launch_bounds__(32 * DecCfg<D, BITS>::kWarps, DecCfg<D, BITS>:
     ok = __all_sync(0xffffffffu, ok && mbar_wait(bar0 + 8 * st, phase, abort_flag));
     if (ok) {
       const uint8_t* stage = ring + st * C::kStage;
-      if (full >> st & 1u) {
-        const int nv[4] = {16, 16, 16, 16};
-        step(std::true_type{}, stage, nv);
-      } else {
-        const int4 v = *reinterpret_cast<const int4*>(s_valid + 4 * st);
-        const int nv[4] = {v.x, v.y, v.z, v.w};
-        step(std::false_type{}, stage, nv);
-      }
+      const bool whole = full >> st & 1u;
+      const int4 v = *reinterpret_cast<const int4*>(s_valid + 4 * st);
+      step(stage, whole, v);
       __syncwarp();  // every lane has read the stage
       if (j + S < n) issue(j + S, st);
       if (++st == S) {
