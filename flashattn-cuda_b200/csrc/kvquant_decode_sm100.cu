@@ -484,25 +484,26 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 2)
 // done once each instead of half of them for columns that nobody reads.
 //
 // What bounds it: at 4 bits and D = 128 a 16-token slab of one KV head is 2304
-// bytes and about 230 instructions, 84 of them the unpacking.  At 12 warps an SM
-// (two 9 KB stages a warp fill shared memory, O and the operands the registers)
-// the rate of instructions and not HBM is the limit: 64 ragged sequences of 8 KV
-// heads, 1285 MB of blocks, take 227 us at 1.8-1.97 GHz, 5.7 TB/s (6.45 TB/s is
-// the measured copy), and 263-269 us in a long run, where the power limit takes
-// the clock to 1.69 GHz.  At 8 bits, with twice the bytes an instruction, 32
-// sequences of 16384 tokens, 1141 MB, take 188 us, 6.1 TB/s.  Warps alone on their
-// scheduler take 1.9 us a step and three together 2.9 each.  32-token steps with
-// 16 warps an SM were slower (257 us: what a step costs besides its tokens), so
-// were K and V in separate halves of a stage (273 us: several small copies a page
-// where one does).
+// bytes and about 250 instructions, 84 of them the unpacking.  12 warps an SM fit
+// (two 9 KB stages a warp fill shared memory, O and the operands the registers),
+// three a scheduler, and those issue in half of the cycles: their own dependences and
+// latencies are the limit, not HBM nor one unit (ALU 50%, tensor 28%).  64 ragged
+// sequences of 8 KV heads, 1285 MB of blocks, take 240 us in short runs, 5.4 TB/s
+// (6.45 TB/s is the measured copy), and 276 us in a long run, where the power limit
+// takes the clock from 1.97 to about 1.7 GHz.  At 8 bits, with twice the bytes an
+// instruction, 32 sequences of 16384 tokens, 1141 MB, take 189 us, 6.0 TB/s.  Warps
+// alone on their scheduler take 2.4 us a step and three together 3.1 each.  32-token
+// steps with 16 warps an SM were slower (257 us where 64-token ones took 221: what a
+// step costs besides its tokens), so were K and V in separate halves of a stage (273
+// us: several small copies a page where one does).
 template <int D, int BITS>
 struct DecCfg {
   static constexpr int kStep = 64;  // tokens per step
   static constexpr int kRow = row_bytes(D, BITS);
   static constexpr int kNG = D / kGroup;
   static constexpr int kStage = kStep * (2 * kRow + 2 * kNG * 4);
-  // Two stages of 4.6 to 17 KB a warp: three CTAs of 74 or 70 KB fit an SM, four
-  // of 37.
+  // Two stages of 4.6 to 17 KB a warp: three CTAs of 76 or 71 KB fit an SM, four
+  // of 39.
   static constexpr int kWarps = (D == 128 && BITS == 8) ? 2 : 4;
   static constexpr int kStages = 2;
   static constexpr int kCtas = (D == 64 && BITS == 4) ? 4 : 3;  // per SM

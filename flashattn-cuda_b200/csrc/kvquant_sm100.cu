@@ -15,9 +15,9 @@
 // Both are copies.  Measured at D = 128, 4 bits: reading 16 sequences of 512 to
 // 16384 tokens of 8 KV heads back (709 MB read and written) 117 us, 94% of the
 // measured copy rate; appending 4 x 8192 bf16 tokens (172 MB) 40 us, 67%, where
-// the instructions, 240 or so for every two rows of K and of V, are the limit (41
-// with one value an instruction and every code clamped; 8 x 8192 fp16 tokens at 8
-// bits with an index: 94 -> 88 us).
+// the instructions, 247 for every two rows of K and of V, are the limit: they issue in
+// 78% of the cycles, DRAM is active in 45% (41 us with one value an instruction and
+// every code clamped; 8 x 8192 fp16 tokens at 8 bits with an index: 94 -> 88 us).
 #include <type_traits>
 
 #include "kvquant.cuh"
